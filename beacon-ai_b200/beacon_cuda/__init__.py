@@ -6,8 +6,8 @@
 - ``model.CudaModel``: the fused, graph-captured decoder runtime (the fast path).
 """
 from . import _lib
-from .backend import ContextOverflow, CudaBackend, EngineError, ShapeMismatch, Stream, Tensor
+from .backend import ContextOverflow, CudaBackend, EngineError, Rope, ShapeMismatch, Stream, Tensor
 from .model import CudaModel, DecoderConfig
 
-__all__ = ["_lib", "CudaBackend", "CudaModel", "DecoderConfig", "EngineError", "ShapeMismatch",
+__all__ = ["_lib", "CudaBackend", "CudaModel", "DecoderConfig", "EngineError", "Rope", "ShapeMismatch",
            "ContextOverflow", "Stream", "Tensor"]

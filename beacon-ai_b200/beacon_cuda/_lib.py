@@ -33,6 +33,9 @@ DTYPE_Q4_1, DTYPE_Q5_0, DTYPE_Q5_1, DTYPE_Q2_K, DTYPE_Q3_K, DTYPE_Q8_K = 105, 10
 NIBBLE_REF_INTERLEAVED, NIBBLE_GGUF_SPLIT = 0, 1
 NUMERICS_FAST, NUMERICS_EXACT, NUMERICS_REF_RTZ = 0, 1, 2
 
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+ROPE_SCALING_NONE, ROPE_SCALING_LINEAR, ROPE_SCALING_YARN, ROPE_SCALING_BANDS = 0, 1, 2, 3
+
 W_EMBED, W_FINAL_NORM, W_LM_HEAD = 0, 1, 2
 W_ATTN_NORM, W_Q, W_K, W_V, W_O, W_FFN_NORM, W_GATE, W_UP, W_DOWN = 10, 11, 12, 13, 14, 15, 16, 17, 18
 
@@ -49,6 +52,14 @@ def sampling_params(temperature=0.0, top_k=None, top_p=None, min_p=None, repeat_
     return SamplingParams(temperature, top_k is not None, top_k or 0, top_p is not None,
                           0.0 if top_p is None else top_p, min_p is not None, 0.0 if min_p is None else min_p,
                           repeat_penalty)
+
+
+class RopeParams(ctypes.Structure):
+    """BeaconCudaRopeParams: one rotation's layout, frequencies and scaling."""
+    _fields_ = [("theta", ctypes.c_float), ("rotary_dim", ctypes.c_int32), ("layout", ctypes.c_int32),
+                ("scaling", ctypes.c_int32), ("factor", ctypes.c_float), ("original_context", ctypes.c_int32),
+                ("beta_fast", ctypes.c_float), ("beta_slow", ctypes.c_float), ("low_freq_factor", ctypes.c_float),
+                ("high_freq_factor", ctypes.c_float), ("attention_factor", ctypes.c_float)]
 
 
 class BeaconCudaError(RuntimeError):
@@ -117,6 +128,12 @@ SIGNATURES = {
     "beacon_cuda_op_quantize": (_I32, [_P, _P, _P, _I32, _I32, _PP]),
     "beacon_cuda_quantize_blocks": (_I32, [_P, _P, _P, _I64, _I64, _I32, _I32, _P]),
     "beacon_cuda_quantized_matvec_noalloc": (_I32, [_P, _P, _P, _I32, _I32, _P]),
+    "beacon_cuda_rope_create": (_I32, [_P, _P, _P, _PP]),
+    "beacon_cuda_rope_destroy": (None, [_P]),
+    "beacon_cuda_op_rope_scaled": (_I32, [_P, _P, _P, _P, _P, _PP]),
+    "beacon_cuda_op_qk_norm_rope": (_I32, [_P, _P, _P, _P, _P, _P, ctypes.c_float, _P, _P, _PP, _PP]),
+    "beacon_cuda_op_paged_append": (_I32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "beacon_cuda_op_paged_attention": (_I32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_float, _PP]),
     "beacon_cuda_model_create": (_I32, [_P, _P, _PP]),
     "beacon_cuda_model_destroy": (None, [_P]),
     "beacon_cuda_model_set_weight": (_I32, [_P, _I32, _I32, _P, _I32, _I32, _I32]),

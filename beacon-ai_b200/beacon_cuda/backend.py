@@ -140,6 +140,28 @@ class Stream:
             self._h = ctypes.c_void_p()
 
 
+class Rope:
+    """Owning handle of a BeaconCudaRope: the frequency table of one rotation."""
+
+    __slots__ = ("_h",)
+
+    def __init__(self, handle: int):
+        self._h = ctypes.c_void_p(handle)
+
+    @property
+    def handle(self):
+        return self._h
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h is not None and h.value:
+            try:
+                L.lib().beacon_cuda_rope_destroy(h)
+            except Exception:
+                pass
+            self._h = ctypes.c_void_p()
+
+
 def _shape_arr(shape):
     arr = (ctypes.c_int64 * max(1, len(shape)))(*shape)
     return arr, len(shape)
@@ -194,6 +216,20 @@ class CudaBackend:
         h = ctypes.c_void_p()
         _raise(L.lib().beacon_cuda_tensor_zeros(self.ctx, arr, nd, dtype, ctypes.byref(h)))
         return Tensor(h.value)
+
+    def wrap(self, device_ptr: int, shape, dtype: int) -> Tensor:
+        """A view of the caller's device memory (plain dtypes), which must outlive it."""
+        arr, nd = _shape_arr(shape)
+        h = ctypes.c_void_p()
+        _raise(L.lib().beacon_cuda_tensor_wrap_device(self.ctx, ctypes.c_void_p(device_ptr), arr, nd, dtype,
+                                                      ctypes.byref(h)))
+        return Tensor(h.value)
+
+    def wrap_stream(self, cuda_stream: int) -> Stream:
+        """A stream handle on the caller's cudaStream_t (0: the default stream)."""
+        h = ctypes.c_void_p()
+        _raise(L.lib().beacon_cuda_stream_wrap(self.ctx, ctypes.c_void_p(cuda_stream), ctypes.byref(h)))
+        return Stream(h.value)
 
     # --- ComputeBackend ----------------------------------------------------------
     def new_stream(self) -> Stream:
@@ -300,6 +336,60 @@ class CudaBackend:
     def quantize(self, stream: Stream, x: Tensor, dtype: int,
                  nibble_order: int = L.NIBBLE_REF_INTERLEAVED) -> Tensor:
         return self._op(L.lib().beacon_cuda_op_quantize, stream.handle, x.handle, dtype, nibble_order)
+
+    # --- rotary positions and paged caches ----------------------------------------
+    def rope_create(self, theta: float, rotary_dim: int, layout: int = L.ROPE_INTERLEAVED,
+                    scaling: int = L.ROPE_SCALING_NONE, factor: float = 1.0, original_context: int = 0,
+                    beta_fast: float = 32.0, beta_slow: float = 1.0, low_freq_factor: float = 1.0,
+                    high_freq_factor: float = 4.0, attention_factor: float = 0.0, freq_factors=None) -> Rope:
+        """The frequency table of a rotation, kept by the caller for its model's layers and steps."""
+        p = L.RopeParams(theta, rotary_dim, layout, scaling, factor, original_context, beta_fast, beta_slow,
+                         low_freq_factor, high_freq_factor, attention_factor)
+        ff = None if freq_factors is None else np.ascontiguousarray(freq_factors, dtype=np.float32)
+        if ff is not None and ff.size != rotary_dim // 2:
+            raise ShapeMismatch("rope_create: one frequency factor per pair is needed")
+        h = ctypes.c_void_p()
+        _raise(L.lib().beacon_cuda_rope_create(self.ctx, ctypes.byref(p), None if ff is None else ff.ctypes.data,
+                                               ctypes.byref(h)))
+        return Rope(h.value)
+
+    def rope_scaled(self, stream: Stream, x: Tensor, positions: Tensor, rope: Rope, out: Tensor | None = None) -> Tensor:
+        """x [T, heads, dim] turned to positions [T]; `out` (may be x) is written in place when given."""
+        h = ctypes.c_void_p(out.handle.value if out else None)
+        _raise(L.lib().beacon_cuda_op_rope_scaled(self.ctx, stream.handle, x.handle, positions.handle, rope.handle,
+                                                  ctypes.byref(h)))
+        return out or Tensor(h.value)
+
+    def qk_norm_rope(self, stream: Stream, q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, eps: float,
+                     positions: Tensor | None = None, rope: Rope | None = None, out_q: Tensor | None = None,
+                     out_k: Tensor | None = None) -> tuple[Tensor, Tensor]:
+        """RMS norm of every head of q and k, then the rotation (none without `rope`)."""
+        hq = ctypes.c_void_p(out_q.handle.value if out_q else None)
+        hk = ctypes.c_void_p(out_k.handle.value if out_k else None)
+        _raise(L.lib().beacon_cuda_op_qk_norm_rope(self.ctx, stream.handle, q.handle, k.handle, q_weight.handle,
+                                                   k_weight.handle, eps, positions.handle if positions else None,
+                                                   rope.handle if rope else None, ctypes.byref(hq), ctypes.byref(hk)))
+        return out_q or Tensor(hq.value), out_k or Tensor(hk.value)
+
+    def paged_append(self, stream: Stream, cache_k: Tensor, cache_v: Tensor, new_k: Tensor, new_v: Tensor,
+                     page_table: Tensor, positions: Tensor, seq_ids: Tensor | None = None,
+                     rope: Rope | None = None) -> None:
+        """Writes new rows into their sequences' pages, the keys turned to their positions on the way."""
+        _raise(L.lib().beacon_cuda_op_paged_append(
+            self.ctx, stream.handle, cache_k.handle, cache_v.handle, new_k.handle, new_v.handle, page_table.handle,
+            seq_ids.handle if seq_ids else None, positions.handle, rope.handle if rope else None))
+
+    def paged_attention(self, stream: Stream, q: Tensor, cache_k: Tensor, cache_v: Tensor, page_table: Tensor,
+                        kv_lens: Tensor, scale: float, query_starts: Tensor | None = None,
+                        group_starts: Tensor | None = None, prefix_lens: Tensor | None = None,
+                        out: Tensor | None = None) -> Tensor:
+        """Causal attention over a paged cache; prefixes shared by groups of sequences are read once."""
+        h = ctypes.c_void_p(out.handle.value if out else None)
+        _raise(L.lib().beacon_cuda_op_paged_attention(
+            self.ctx, stream.handle, q.handle, cache_k.handle, cache_v.handle, page_table.handle, kv_lens.handle,
+            query_starts.handle if query_starts else None, group_starts.handle if group_starts else None,
+            prefix_lens.handle if prefix_lens else None, scale, ctypes.byref(h)))
+        return out or Tensor(h.value)
 
     def __del__(self):
         try:

@@ -152,6 +152,10 @@ struct BeaconCudaContext {
     bool comm_aborted = false;  // a failed or timed-out collective aborted the communicator
     int nranks = 1, rank = 0;
     int comm_timeout_ms = 60000;
+    // host-mapped error words handed to streams (stream_error_word); slots are
+    // never reused, so a graph that outlives its stream reports to nobody else
+    std::vector<int*> err_slabs;
+    int err_used = 0;  // words taken from the last slab
 };
 
 struct BeaconCudaStream {
@@ -159,6 +163,9 @@ struct BeaconCudaStream {
     cudaStream_t s = nullptr;
     bool owned = false;
     bc::Workspace ws;  // split-K scratch, arrival counters and error flags of ops on this stream
+    // word that kernels set when an index held in a device tensor is out of
+    // range; host memory, so reading it costs no copy. Null until first needed.
+    int* err_word = nullptr;
 };
 
 struct BeaconCudaTensor {
@@ -190,7 +197,11 @@ inline cudaStream_t stream_of(BeaconCudaStream* s) { return s ? s->s : nullptr; 
 // device wait of an op on this stream gave up, clear the flag, re-zero the
 // stream's arrival counters (a warp that gave up never arrived) and throw
 // BEACON_CUDA_ERR_DEVICE_TIMEOUT.
+// An index error that a kernel recorded in the stream's error word is thrown
+// as SHAPE_MISMATCH and cleared.
 void check_stream_timeout(BeaconCudaStream* stream);
+// The stream's error word, made at its first use (also during capture).
+int* stream_error_word(BeaconCudaStream* stream);
 // The same for every stream of the context (after a device synchronisation).
 void check_context_timeouts(BeaconCudaContext* ctx);
 

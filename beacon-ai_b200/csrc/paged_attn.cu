@@ -1,0 +1,197 @@
+// paged_attn.cu -- causal attention over paged key/value caches with prefixes
+// shared by groups of sequences (beacon_cuda_op_paged_attention): the argument
+// checks and the kernel of any dtype and head size.
+#include <cuda_bf16.h>
+
+#include <cmath>
+#include <string>
+
+#include "common.cuh"
+#include "internal.h"
+#include "kernels.h"
+#include "paged_attn.h"
+#include "rotary.h"
+
+namespace bc {
+namespace {
+
+constexpr int kAnyWarps = 4;
+constexpr int kAnyMaxDim = 256;
+
+template <typename T>
+__device__ __forceinline__ float as_f32(T v);
+template <>
+__device__ __forceinline__ float as_f32(float v) { return v; }
+template <>
+__device__ __forceinline__ float as_f32(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float as_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// One query row and head per block. Each warp takes every fourth key, its
+// lanes the head's values, with its own running maximum and sum; the warps'
+// parts are joined at the end. f32 throughout.
+template <typename TQ, typename TK>
+__global__ void __launch_bounds__(kAnyWarps * 32) paged_attn_any_kernel(const PagedArgs a) {
+    constexpr int N = kAnyMaxDim / 32;
+    __shared__ float m_s[kAnyWarps], l_s[kAnyWarps], o_s[kAnyWarps][kAnyMaxDim];
+    const int t = blockIdx.x, h = blockIdx.y, kvh = h / a.G;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = a.qstarts ? span_of(a.qstarts, a.B, t) : t;
+    if (b < 0) return;  // behind the last sequence
+    const SeqInfo s = seq_info(a, b);
+    const int limit = min(s.len, s.len - s.nq + (t - s.q0) + 1);
+    const TQ* q = static_cast<const TQ*>(a.q) + ((int64_t)t * a.H + h) * a.D;
+    float qv[N], o[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int d = lane + 32 * i;
+        qv[i] = d < a.D ? as_f32(q[d]) * a.scale : 0.0f;
+        o[i] = 0.0f;
+    }
+    float m = -INFINITY, l = 0.0f;
+    for (int p = warp; p < limit; p += kAnyWarps) {
+        const int64_t row = page_row(a, p < s.prefix ? s.first : b, p);
+        if (row < 0) continue;
+        const int64_t at = (row * a.Hkv + kvh) * a.D;
+        const TK* k = static_cast<const TK*>(a.ck) + at;
+        const TK* v = static_cast<const TK*>(a.cv) + at;
+        float dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int d = lane + 32 * i;
+            if (d < a.D) dot = fmaf(qv[i], as_f32(k[d]), dot);
+        }
+        dot = warp_sum(dot);
+        const float mn = fmaxf(m, dot);
+        // a row whose scores so far are all -inf keeps its empty sums
+        const float keep = m == -INFINITY ? 0.0f : expf(m - mn);
+        const float e = mn == -INFINITY ? 0.0f : expf(dot - mn);
+        m = mn;
+        l = l * keep + e;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int d = lane + 32 * i;
+            if (d < a.D) o[i] = fmaf(e, as_f32(v[d]), o[i] * keep);
+        }
+    }
+    if (lane == 0) {
+        m_s[warp] = m;
+        l_s[warp] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) o_s[warp][lane + 32 * i] = o[i];
+    __syncthreads();
+    float mx = m_s[0];
+    for (int w = 1; w < kAnyWarps; ++w) mx = fmaxf(mx, m_s[w]);
+    float total = 0.0f, wt[kAnyWarps];
+#pragma unroll
+    for (int w = 0; w < kAnyWarps; ++w) {
+        wt[w] = m_s[w] == -INFINITY ? 0.0f : expf(m_s[w] - mx);
+        total += l_s[w] * wt[w];
+    }
+    TQ* out = static_cast<TQ*>(a.out) + ((int64_t)t * a.H + h) * a.D;
+    for (int d = threadIdx.x; d < a.D; d += kAnyWarps * 32) {
+        float r = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kAnyWarps; ++w) r = fmaf(o_s[w][d], wt[w], r);
+        put(out + d, total == 0.0f ? 0.0f : r / total);
+    }
+}
+
+void check_i32(const BeaconCudaContext* ctx, const BeaconCudaTensor* t, int64_t n, const char* what) {
+    check_tensor(ctx, t, what);
+    if (t->dtype != BEACON_CUDA_DTYPE_I32) fail(BEACON_CUDA_ERR_UNSUPPORTED_DTYPE, std::string(what) + " must be I32");
+    if (n >= 0 && (t->shape.size() != 1 || t->numel() != n)) shape_err(std::string(what) + " has the wrong length");
+}
+
+}  // namespace
+}  // namespace bc
+
+using namespace bc;
+
+extern "C" int32_t beacon_cuda_op_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream,
+                                                  const BeaconCudaTensor* q, const BeaconCudaTensor* cache_k,
+                                                  const BeaconCudaTensor* cache_v, const BeaconCudaTensor* page_table,
+                                                  const BeaconCudaTensor* kv_lens, const BeaconCudaTensor* query_starts,
+                                                  const BeaconCudaTensor* group_starts,
+                                                  const BeaconCudaTensor* prefix_lens, float scale,
+                                                  BeaconCudaTensor** inout_out) {
+    return guard([&]() -> int32_t {
+        require(ctx && stream && q && cache_k && cache_v && page_table && kv_lens && inout_out,
+                "paged_attention: null argument");
+        require((group_starts != nullptr) == (prefix_lens != nullptr),
+                "paged_attention: group_starts and prefix_lens come together");
+        check_stream(ctx, stream, "paged_attention");
+        for (const BeaconCudaTensor* t : {q, cache_k, cache_v}) check_tensor(ctx, t, "paged_attention");
+        const int32_t F32 = BEACON_CUDA_DTYPE_F32, F16 = BEACON_CUDA_DTYPE_F16, BF16 = BEACON_CUDA_DTYPE_BF16;
+        const int32_t tq = q->dtype, tk = cache_k->dtype;
+        if (cache_v->dtype != tk || !((tq == F32 && (tk == F16 || tk == F32)) || (tq == F16 && tk == F16) || (tq == BF16 && tk == BF16)))
+            fail(BEACON_CUDA_ERR_UNSUPPORTED_DTYPE,
+                 "paged_attention: (q, caches) must be (F32, F16), (F16, F16), (BF16, BF16) or (F32, F32)");
+        if (q->shape.size() != 3) shape_err("paged_attention: q must be [T, H, D]");
+        if (cache_k->shape.size() != 4 || cache_v->shape != cache_k->shape)
+            shape_err("paged_attention: caches must be alike, [pages, page_size, Hkv, D]");
+        const int64_t T = q->shape[0], H = q->shape[1], D = q->shape[2], Hkv = cache_k->shape[2];
+        if (cache_k->shape[3] != D) shape_err("paged_attention: q and the caches differ in head size");
+        if (D < 8 || D > kAnyMaxDim || D % 8) shape_err("paged_attention: the head size must be a multiple of 8, 8 to 256");
+        if (Hkv < 1 || H < 1 || H % Hkv || H > 65535) shape_err("paged_attention: H must be a multiple of Hkv, at most 65535");
+        if (cache_k->shape[1] < 1 || cache_k->shape[1] > 0x7FFFFFFF) shape_err("paged_attention: empty pages");
+        check_i32(ctx, page_table, -1, "paged_attention: page_table");
+        if (page_table->shape.size() != 2) shape_err("paged_attention: page_table must be [B, max_pages]");
+        const int64_t B = page_table->shape[0], max_pages = page_table->shape[1];
+        if (T > 0x3FFFFFFF || B > 0x3FFFFFFF || max_pages > 0x7FFFFFFF) shape_err("paged_attention: too many rows or pages");
+        check_i32(ctx, kv_lens, B, "paged_attention: kv_lens");
+        if (query_starts) check_i32(ctx, query_starts, B + 1, "paged_attention: query_starts");
+        else if (T != B) shape_err("paged_attention: without query_starts every sequence has one query row");
+        int64_t groups = 0;
+        if (group_starts) {
+            groups = prefix_lens->numel();
+            if (groups < 1 || groups > 0x3FFFFFFF) shape_err("paged_attention: no groups");
+            check_i32(ctx, prefix_lens, groups, "paged_attention: prefix_lens");
+            check_i32(ctx, group_starts, groups + 1, "paged_attention: group_starts");
+        }
+        if (!std::isfinite(scale)) invalid("paged_attention: scale must be finite");
+        for (const BeaconCudaTensor* t : {q, cache_k, cache_v})
+            if (!aligned16(t->data())) invalid("paged_attention: tensors must be 16-byte aligned");
+        DeviceScope dev(ctx);
+        OutTensor out(ctx, inout_out, q->shape, tq, "paged_attention");
+        if (!aligned16(out.data())) invalid("paged_attention: tensors must be 16-byte aligned");
+        for (const BeaconCudaTensor* t : {q, cache_k, cache_v, page_table, kv_lens, query_starts, group_starts, prefix_lens})
+            out.check_overlap(t, false, "paged_attention");
+        PagedArgs a;
+        a.q = q->data();
+        a.ck = cache_k->data();
+        a.cv = cache_v->data();
+        a.out = out.data();
+        a.table = static_cast<const int32_t*>(page_table->data());
+        a.lens = static_cast<const int32_t*>(kv_lens->data());
+        a.qstarts = query_starts ? static_cast<const int32_t*>(query_starts->data()) : nullptr;
+        a.gstarts = group_starts ? static_cast<const int32_t*>(group_starts->data()) : nullptr;
+        a.prefix = prefix_lens ? static_cast<const int32_t*>(prefix_lens->data()) : nullptr;
+        a.pages = cache_k->shape[0];
+        a.T = (int)T;
+        a.B = (int)B;
+        a.H = (int)H;
+        a.Hkv = (int)Hkv;
+        a.G = (int)(H / Hkv);
+        a.D = (int)D;
+        a.groups = (int)groups;
+        a.max_pages = (int)max_pages;
+        a.page_size = (int)cache_k->shape[1];
+        a.scale = scale;
+        a.err = stream_error_word(stream);
+        if (T > 0 && B > 0) {
+            const dim3 grid((unsigned)T, (unsigned)H);
+            if (tq == F32 && tk == F32) paged_attn_any_kernel<float, float><<<grid, kAnyWarps * 32, 0, stream->s>>>(a);
+            else if (tq == F32) paged_attn_any_kernel<float, __half><<<grid, kAnyWarps * 32, 0, stream->s>>>(a);
+            else if (tq == F16) paged_attn_any_kernel<__half, __half><<<grid, kAnyWarps * 32, 0, stream->s>>>(a);
+            else paged_attn_any_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, kAnyWarps * 32, 0, stream->s>>>(a);
+            BC_LAUNCHED("paged_attn_any_kernel");
+        }
+        out.release();
+        return BEACON_CUDA_OK;
+    });
+}

@@ -1,0 +1,638 @@
+// rotary.cu -- rotary positions of token-major rows (rope_scaled), head norms
+// with the rotation (qk_norm_rope) and the cache append with the rotation
+// (paged_append).
+//
+// All three are one pass over rows of `dim` values: read a head, optionally
+// scale it by w / sqrt(mean(x^2) + eps), turn its first rotary_dim values, and
+// write it to a dense row or to its cache page, so one kernel does them. It is
+// bound by memory: 16-byte loads, each value read and written once.
+//
+// A block takes whole tokens. It first computes the sine and cosine of every
+// pair for its tokens into shared memory (a 64-bit product position * f_i / 2pi
+// reduced to one turn, then sincospif in 32 bits, so the angle of position 10^6
+// is as good as that of position 1) and all heads of the token use them: the
+// 64-bit work is per token, not per head.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "common.cuh"
+#include "internal.h"
+#include "kernels.h"
+#include "rotary.h"
+
+namespace bc {
+
+OutTensor::OutTensor(BeaconCudaContext* ctx, BeaconCudaTensor** inout, const std::vector<int64_t>& shape,
+                     int32_t dtype, const char* what)
+    : inout_(inout), t_(*inout) {
+    if (t_) {
+        check_tensor(ctx, t_, what);
+        if (t_->shape != shape) shape_err(std::string(what) + ": the output tensor's shape is not the result's");
+        if (t_->dtype != dtype)
+            fail(BEACON_CUDA_ERR_UNSUPPORTED_DTYPE, std::string(what) + ": the output tensor's dtype is not the result's");
+    } else {
+        made_.reset(new_tensor(ctx, shape, dtype));
+        t_ = made_.get();
+    }
+}
+
+void OutTensor::check_overlap(const BeaconCudaTensor* x, bool in_place, const char* what) const {
+    if (!x) return;
+    const char *a = static_cast<const char*>(t_->data()), *b = static_cast<const char*>(x->data());
+    const size_t an = t_->nbytes(), bn = x->nbytes();
+    if (!an || !bn || a + an <= b || b + bn <= a) return;
+    if (in_place && a == b && an == bn) return;
+    invalid(std::string(what) + ": the output overlaps an input");
+}
+
+void check_tensor(const BeaconCudaContext* ctx, const BeaconCudaTensor* t, const char* what) {
+    if (t->ctx != ctx) invalid(std::string(what) + ": a tensor belongs to another context");
+}
+
+void check_stream(const BeaconCudaContext* ctx, const BeaconCudaStream* stream, const char* what) {
+    if (stream->ctx != ctx) invalid(std::string(what) + ": the stream belongs to another context");
+}
+
+namespace {
+
+constexpr int kRowThreads = 256;
+constexpr int kMaxTokens = 32;     // tokens of one block
+constexpr int kMaxHeadDim = 512;
+
+struct RowSegment {                // heads of one input tensor
+    const void* src = nullptr;     // [T][heads][dim]
+    void* dst = nullptr;           // the same, or cache pages when RowArgs.table
+    const void* weight = nullptr;  // norm weight [dim]; null: no norm
+    int32_t weight_dtype = 0;
+    int heads = 0;
+    bool turn = false;
+};
+
+struct RowArgs {
+    RowSegment seg[2];
+    int64_t tokens = 0;
+    int heads = 0;  // of both segments
+    int dim = 0, rotary = 0;
+    float eps = 0.0f, amplitude = 1.0f;
+    const int32_t* positions = nullptr;
+    const double* turns = nullptr;  // [rotary / 2]
+    // cache pages
+    const int32_t* table = nullptr;  // [seqs][max_pages]; null: dense rows
+    const int32_t* seq_ids = nullptr;
+    int64_t seqs = 0, max_pages = 0, pages = 0, page_size = 0;
+    int* err = nullptr;
+    // launch shape
+    int block_tokens = 1;  // tokens of one block
+    int lanes = 1;         // threads of one head (power of two)
+    int parts = 1;         // blocks that share a block's heads (grid.y)
+};
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+    T v[N];
+};
+
+__device__ __forceinline__ float load_weight(const void* w, int32_t dtype, int i) {
+    return dtype == BEACON_CUDA_DTYPE_F16 ? __half2float(static_cast<const __half*>(w)[i])
+                                          : static_cast<const float*>(w)[i];
+}
+
+// Row of the pages that token t's key and value go to; -1: skip.
+__device__ __forceinline__ int64_t cache_row(const RowArgs& a, int64_t t) {
+    const int64_t p = a.positions[t];
+    if (p < 0) return -1;
+    const int64_t b = a.seq_ids ? (int64_t)a.seq_ids[t] : t;
+    if (b >= 0 && b < a.seqs && p < a.max_pages * a.page_size) {
+        const int64_t page = a.table[b * a.max_pages + p / a.page_size];
+        if (page >= 0 && page < a.pages) return page * a.page_size + p % a.page_size;
+    }
+    *a.err = kErrIndex;
+    return -1;
+}
+
+// Sine and cosine of the block's tokens into shared memory, and their cache rows.
+__device__ __forceinline__ void fill_tables(const RowArgs& a, int64_t t0, int nt, float2* cs, int64_t* rows) {
+    const int half = a.rotary / 2;
+    for (int i = threadIdx.x; i < nt * half; i += blockDim.x) {
+        const int t = i / half, j = i - t * half;
+        double turn = (double)a.positions[t0 + t] * a.turns[j];
+        turn -= rint(turn);
+        float s, c;
+        sincospif(2.0f * (float)turn, &s, &c);
+        cs[i] = make_float2(c * a.amplitude, s * a.amplitude);
+    }
+    if (a.table)
+        for (int t = threadIdx.x; t < nt; t += blockDim.x) rows[t] = cache_row(a, t0 + t);
+}
+
+// Each head is handled by `lanes` threads, each with two slots of V values.
+// HALF: slot 0 holds values of the first half of the rotated part and slot 1
+// their partners; the threads after those take the unrotated rest, two slots
+// each. Interleaved: slots 2l and 2l + 1, whose pairs lie inside a slot.
+template <typename TI, typename TO, bool HALF>
+__global__ void __launch_bounds__(kRowThreads) row_kernel(const RowArgs a) {
+    constexpr int V = 16 / sizeof(TI);
+    extern __shared__ float2 cs_s[];
+    __shared__ int64_t rows_s[kMaxTokens];
+    const int64_t t0 = (int64_t)blockIdx.x * a.block_tokens;
+    const int nt = (int)min((int64_t)a.block_tokens, a.tokens - t0);
+    const int half = a.rotary / 2;
+    const int lane = threadIdx.x & (a.lanes - 1);
+    // this thread's slots of every head
+    int at0, at1;
+    bool turn;
+    if (HALF) {
+        const int turning = half / V;
+        turn = lane < turning;
+        at0 = turn ? lane * V : a.rotary + (lane - turning) * 2 * V;
+        at1 = turn ? at0 + half : at0 + V;
+    } else {
+        at0 = lane * 2 * V;
+        at1 = at0 + V;
+        turn = true;
+    }
+    const bool has0 = at0 < a.dim, has1 = at1 < a.dim;
+    const int per = kRowThreads / a.lanes;  // heads of one step
+    const int total = nt * a.heads;
+    const int step = per * (int)gridDim.y;
+    int r = (int)blockIdx.y * per + threadIdx.x / a.lanes;
+
+    Pack<TI, V> x0{}, x1{};
+    auto load = [&](int i) {
+        const int t = i / a.heads, h = i - t * a.heads;
+        const bool second = h >= a.seg[0].heads;
+        const RowSegment& sg = a.seg[second ? 1 : 0];
+        const TI* src = static_cast<const TI*>(sg.src) +
+                        ((t0 + t) * sg.heads + (second ? h - a.seg[0].heads : h)) * a.dim;
+        if (has0) x0 = *reinterpret_cast<const Pack<TI, V>*>(src + at0);
+        if (has1) x1 = *reinterpret_cast<const Pack<TI, V>*>(src + at1);
+    };
+    // the first heads are on their way while the angles are computed
+    if (r < total) load(r);
+    fill_tables(a, t0, nt, cs_s, rows_s);
+    __syncthreads();
+    for (int base = r - (int)(threadIdx.x / a.lanes); base < total; base += step, r += step) {
+        const bool live = r < total;  // a head's lanes agree, so shuffles among them are whole
+        const int i = live ? r : 0;
+        const int t = i / a.heads, h = i - t * a.heads;
+        const bool second = h >= a.seg[0].heads;
+        const RowSegment& sg = a.seg[second ? 1 : 0];
+        float f0[V], f1[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            f0[j] = to_f32(x0.v[j]);
+            f1[j] = to_f32(x1.v[j]);
+        }
+        if (r + step < total) load(r + step);
+        if (sg.weight) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (has0) ss = fmaf(f0[j], f0[j], ss);
+                if (has1) ss = fmaf(f1[j], f1[j], ss);
+            }
+            for (int o = a.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float inv = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (has0) f0[j] = f0[j] * inv * load_weight(sg.weight, sg.weight_dtype, at0 + j);
+                if (has1) f1[j] = f1[j] * inv * load_weight(sg.weight, sg.weight_dtype, at1 + j);
+            }
+        }
+        if (sg.turn && half) {
+            const float2* cs = cs_s + t * half;
+            if (HALF) {
+                if (turn) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const float2 c = cs[at0 + j];
+                        const float u = f0[j], w = f1[j];
+                        f0[j] = u * c.x - w * c.y;
+                        f1[j] = w * c.x + u * c.y;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; j += 2) {
+                    if (at0 + j < a.rotary) {
+                        const float2 c = cs[(at0 + j) / 2];
+                        const float u = f0[j], w = f0[j + 1];
+                        f0[j] = u * c.x - w * c.y;
+                        f0[j + 1] = u * c.y + w * c.x;
+                    }
+                    if (at1 + j < a.rotary) {
+                        const float2 c = cs[(at1 + j) / 2];
+                        const float u = f1[j], w = f1[j + 1];
+                        f1[j] = u * c.x - w * c.y;
+                        f1[j + 1] = u * c.y + w * c.x;
+                    }
+                }
+            }
+        }
+        int64_t row = t0 + t;
+        if (a.table) row = rows_s[t];
+        if (live && row >= 0) {
+            Pack<TO, V> y0, y1;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                y0.v[j] = from_f32<TO>(f0[j]);
+                y1.v[j] = from_f32<TO>(f1[j]);
+            }
+            TO* dst = static_cast<TO*>(sg.dst) + (row * sg.heads + (second ? h - a.seg[0].heads : h)) * a.dim;
+            if (has0) *reinterpret_cast<Pack<TO, V>*>(dst + at0) = y0;
+            if (has1) *reinterpret_cast<Pack<TO, V>*>(dst + at1) = y1;
+        }
+    }
+}
+
+__device__ __forceinline__ float ld_value(const void* p, int32_t dtype, int64_t i) {
+    switch (dtype) {
+        case BEACON_CUDA_DTYPE_F16: return __half2float(static_cast<const __half*>(p)[i]);
+        case BEACON_CUDA_DTYPE_BF16: return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+        default: return static_cast<const float*>(p)[i];
+    }
+}
+__device__ __forceinline__ void st_value(void* p, int32_t dtype, int64_t i, float v) {
+    switch (dtype) {
+        case BEACON_CUDA_DTYPE_F16: static_cast<__half*>(p)[i] = __float2half_rn(v); break;
+        case BEACON_CUDA_DTYPE_BF16: static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v); break;
+        default: static_cast<float*>(p)[i] = v;
+    }
+}
+
+// The same for dims and addresses that 16-byte slots do not fit: one warp per
+// head, a pair of values at a time (rotated pairs, then the rest two by two).
+__global__ void __launch_bounds__(kRowThreads) row_scalar_kernel(const RowArgs a, int32_t ti, int32_t to, bool half_layout) {
+    extern __shared__ float2 cs_s[];
+    __shared__ int64_t rows_s[kMaxTokens];
+    const int64_t t0 = (int64_t)blockIdx.x * a.block_tokens;
+    const int nt = (int)min((int64_t)a.block_tokens, a.tokens - t0);
+    const int half = a.rotary / 2, lane = threadIdx.x & 31;
+    fill_tables(a, t0, nt, cs_s, rows_s);
+    __syncthreads();
+    const int pairs = half + (a.dim - a.rotary + 1) / 2;
+    for (int r = (int)(blockIdx.y * (kRowThreads / 32) + threadIdx.x / 32); r < nt * a.heads;
+         r += (kRowThreads / 32) * (int)gridDim.y) {
+        const int t = r / a.heads, h = r - t * a.heads;
+        const bool second = h >= a.seg[0].heads;
+        const RowSegment& sg = a.seg[second ? 1 : 0];
+        const int hh = second ? h - a.seg[0].heads : h;
+        const int64_t src = ((t0 + t) * sg.heads + hh) * a.dim;
+        const int64_t row = a.table ? rows_s[t] : t0 + t;
+        float u[kMaxHeadDim / 64], w[kMaxHeadDim / 64];
+        float ss = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kMaxHeadDim / 64; ++k) {
+            const int j = lane + 32 * k;
+            if (j >= pairs) break;
+            const int i0 = j < half ? (half_layout ? j : 2 * j) : a.rotary + 2 * (j - half);
+            const int i1 = j < half && half_layout ? j + half : i0 + 1;
+            u[k] = ld_value(sg.src, ti, src + i0);
+            w[k] = i1 < a.dim ? ld_value(sg.src, ti, src + i1) : 0.0f;
+            ss = fmaf(u[k], u[k], fmaf(w[k], w[k], ss));
+        }
+        float inv = 1.0f;
+        if (sg.weight) inv = 1.0f / sqrtf(warp_sum(ss) / (float)a.dim + a.eps);
+        if (row < 0) continue;
+        const int64_t dst = (row * sg.heads + hh) * a.dim;
+#pragma unroll
+        for (int k = 0; k < kMaxHeadDim / 64; ++k) {
+            const int j = lane + 32 * k;
+            if (j >= pairs) break;
+            const int i0 = j < half ? (half_layout ? j : 2 * j) : a.rotary + 2 * (j - half);
+            const int i1 = j < half && half_layout ? j + half : i0 + 1;
+            float x = u[k], y = w[k];
+            if (sg.weight) {
+                x = x * inv * load_weight(sg.weight, sg.weight_dtype, i0);
+                if (i1 < a.dim) y = y * inv * load_weight(sg.weight, sg.weight_dtype, i1);
+            }
+            if (sg.turn && j < half) {
+                const float2 c = cs_s[t * half + j];
+                const float x2 = x * c.x - y * c.y;
+                y = y * c.x + x * c.y;
+                x = x2;
+            }
+            st_value(sg.dst, to, dst + i0, x);
+            if (i1 < a.dim) st_value(sg.dst, to, dst + i1, y);
+        }
+    }
+}
+
+template <typename TI, typename TO>
+void launch_rows_t(const RowArgs& a, bool half_layout, dim3 grid, size_t smem, cudaStream_t s) {
+    if (half_layout)
+        row_kernel<TI, TO, true><<<grid, kRowThreads, smem, s>>>(a);
+    else
+        row_kernel<TI, TO, false><<<grid, kRowThreads, smem, s>>>(a);
+}
+
+void launch_rows(BeaconCudaContext* ctx, RowArgs a, int32_t ti, int32_t to, const BeaconCudaRope* rope, cudaStream_t s) {
+    a.heads = a.seg[0].heads + a.seg[1].heads;
+    if (a.tokens == 0 || a.heads == 0 || a.dim == 0) return;
+    const bool half_layout = rope && rope->layout == BEACON_CUDA_ROPE_HALF;
+    if (rope) {
+        a.rotary = rope->rotary_dim;
+        a.amplitude = rope->amplitude;
+        a.turns = static_cast<const double*>(rope->turns->ptr);
+    }
+    const int esize = (int)plain_elem_bytes(ti), V = 16 / esize;
+    const int slots = half_layout ? a.rotary / 2 / V + (a.dim - a.rotary + 2 * V - 1) / (2 * V) : (a.dim + 2 * V - 1) / (2 * V);
+    bool vec = a.dim % V == 0 && a.rotary % (half_layout ? 2 * V : V) == 0 && slots <= 32;
+    for (const RowSegment& sg : a.seg)
+        vec = vec && aligned16(sg.src) &&
+              reinterpret_cast<uintptr_t>(sg.dst) % (V * plain_elem_bytes(to)) == 0;
+    int per = kRowThreads / 32;  // heads of a block's step
+    if (vec) {
+        a.lanes = 1;
+        while (a.lanes < slots) a.lanes *= 2;
+        per = kRowThreads / a.lanes;
+    }
+    // one step of the block's threads covers a block's heads, and more blocks
+    // than that share them while the device is not full (small batches)
+    a.block_tokens = std::min(kMaxTokens, std::max(1, per / a.heads));
+    const int64_t blocks = (a.tokens + a.block_tokens - 1) / a.block_tokens;
+    if (blocks > 0x7FFFFFFF) shape_err("too many tokens");
+    const int steps = (a.block_tokens * a.heads + per - 1) / per;
+    a.parts = (int)std::min<int64_t>(steps, std::max<int64_t>(1, 4 * ctx->sm_count / blocks));
+    const dim3 grid((unsigned)blocks, (unsigned)std::min(a.parts, 65535));
+    // at most 16 KB: the angles of the values that one step of the threads holds
+    const size_t smem = (size_t)a.block_tokens * (a.rotary / 2) * sizeof(float2);
+    if (!vec) {
+        row_scalar_kernel<<<grid, kRowThreads, smem, s>>>(a, ti, to, half_layout);
+        BC_LAUNCHED("row_scalar_kernel");
+        return;
+    }
+    const int32_t F32 = BEACON_CUDA_DTYPE_F32, F16 = BEACON_CUDA_DTYPE_F16, BF16 = BEACON_CUDA_DTYPE_BF16;
+    if (ti == F32 && to == F32) launch_rows_t<float, float>(a, half_layout, grid, smem, s);
+    else if (ti == F32 && to == F16) launch_rows_t<float, __half>(a, half_layout, grid, smem, s);
+    else if (ti == F32 && to == BF16) launch_rows_t<float, __nv_bfloat16>(a, half_layout, grid, smem, s);
+    else if (ti == F16 && to == F16) launch_rows_t<__half, __half>(a, half_layout, grid, smem, s);
+    else if (ti == F16 && to == F32) launch_rows_t<__half, float>(a, half_layout, grid, smem, s);
+    else if (ti == F16 && to == BF16) launch_rows_t<__half, __nv_bfloat16>(a, half_layout, grid, smem, s);
+    else if (ti == BF16 && to == BF16) launch_rows_t<__nv_bfloat16, __nv_bfloat16>(a, half_layout, grid, smem, s);
+    else if (ti == BF16 && to == F16) launch_rows_t<__nv_bfloat16, __half>(a, half_layout, grid, smem, s);
+    else launch_rows_t<__nv_bfloat16, float>(a, half_layout, grid, smem, s);
+    BC_LAUNCHED("row_kernel");
+}
+
+void check_rows(const BeaconCudaContext* ctx, const BeaconCudaTensor* x, const char* what) {
+    check_tensor(ctx, x, what);
+    if (x->dtype != BEACON_CUDA_DTYPE_F32 && x->dtype != BEACON_CUDA_DTYPE_F16 && x->dtype != BEACON_CUDA_DTYPE_BF16)
+        fail(BEACON_CUDA_ERR_UNSUPPORTED_DTYPE, std::string(what) + ": rows must be F32, F16 or BF16");
+    if (x->shape.size() != 3) shape_err(std::string(what) + ": rows must be [T, heads, dim]");
+    if (x->shape[2] < 1 || x->shape[2] > kMaxHeadDim || x->shape[1] < 1 || x->shape[1] > 65535)
+        shape_err(std::string(what) + ": 1 to 65535 heads of 1 to 512 values");
+}
+
+void check_ids(const BeaconCudaContext* ctx, const BeaconCudaTensor* t, int64_t n, const char* what) {
+    check_tensor(ctx, t, what);
+    if (t->dtype != BEACON_CUDA_DTYPE_I32) fail(BEACON_CUDA_ERR_UNSUPPORTED_DTYPE, std::string(what) + ": must be I32");
+    if (t->numel() != n) shape_err(std::string(what) + ": one entry per row is needed");
+}
+
+void check_rope(const BeaconCudaContext* ctx, const BeaconCudaRope* rope, int64_t dim, const char* what) {
+    if (!rope) return;
+    if (rope->ctx != ctx) invalid(std::string(what) + ": the rotation belongs to another context");
+    if (rope->rotary_dim > dim) shape_err(std::string(what) + ": the rotation is wider than the head");
+}
+
+}  // namespace
+}  // namespace bc
+
+using namespace bc;
+
+extern "C" {
+
+int32_t beacon_cuda_rope_create(BeaconCudaContext* ctx, const BeaconCudaRopeParams* params, const float* freq_factors,
+                                BeaconCudaRope** out_rope) {
+    return guard([&]() -> int32_t {
+        require(ctx && params && out_rope, "rope_create: null argument");
+        const BeaconCudaRopeParams& p = *params;
+        if (p.rotary_dim < 2 || p.rotary_dim % 2 || p.rotary_dim > kMaxHeadDim)
+            invalid("rope_create: rotary_dim must be even, 2 to 512");
+        if (p.layout != BEACON_CUDA_ROPE_INTERLEAVED && p.layout != BEACON_CUDA_ROPE_HALF)
+            invalid("rope_create: unknown layout");
+        if (!(p.theta > 1.0f) || !std::isfinite(p.theta)) invalid("rope_create: theta must be above 1");
+        if (p.scaling < BEACON_CUDA_ROPE_SCALING_NONE || p.scaling > BEACON_CUDA_ROPE_SCALING_BANDS)
+            invalid("rope_create: unknown scaling");
+        const bool scaled = p.scaling != BEACON_CUDA_ROPE_SCALING_NONE;
+        if (scaled && (!(p.factor >= 1.0f) || !std::isfinite(p.factor))) invalid("rope_create: factor must be at least 1");
+        if (!scaled && p.factor != 1.0f) invalid("rope_create: a factor needs a scaling");
+        if (p.scaling >= BEACON_CUDA_ROPE_SCALING_YARN && p.original_context < 1)
+            invalid("rope_create: the scaling needs the original context");
+        if (!(p.attention_factor >= 0.0f) || !std::isfinite(p.attention_factor))
+            invalid("rope_create: attention_factor must be finite and not negative");
+        if (p.scaling == BEACON_CUDA_ROPE_SCALING_YARN &&
+            (!(p.beta_slow > 0.0f) || !(p.beta_fast >= p.beta_slow) || !std::isfinite(p.beta_fast)))
+            invalid("rope_create: yarn needs beta_fast >= beta_slow > 0");
+        if (p.scaling == BEACON_CUDA_ROPE_SCALING_BANDS &&
+            (!(p.low_freq_factor > 0.0f) || !(p.high_freq_factor > p.low_freq_factor) || !std::isfinite(p.high_freq_factor)))
+            invalid("rope_create: bands need high_freq_factor > low_freq_factor > 0");
+        const int half = p.rotary_dim / 2;
+        const double pi2 = 6.283185307179586476925286766559, d = p.rotary_dim, c = p.original_context, s = p.factor;
+        double lo = 0.0, hi = 0.0;
+        if (p.scaling == BEACON_CUDA_ROPE_SCALING_YARN) {
+            auto at = [&](double turns) { return d * std::log(c / (turns * pi2)) / (2.0 * std::log((double)p.theta)); };
+            lo = std::max(0.0, std::floor(at(p.beta_fast)));
+            hi = std::min(d - 1.0, std::ceil(at(p.beta_slow)));
+        }
+        std::vector<double> turns((size_t)half);
+        for (int i = 0; i < half; ++i) {
+            double f = std::pow((double)p.theta, -2.0 * i / d);
+            if (p.scaling == BEACON_CUDA_ROPE_SCALING_LINEAR) {
+                f /= s;
+            } else if (p.scaling == BEACON_CUDA_ROPE_SCALING_YARN) {
+                const double r = std::clamp((i - lo) / std::max(hi - lo, 0.001), 0.0, 1.0);
+                f *= (1.0 - r) + r / s;
+            } else if (p.scaling == BEACON_CUDA_ROPE_SCALING_BANDS) {
+                const double m = std::clamp((c * f / pi2 - p.low_freq_factor) /
+                                                ((double)p.high_freq_factor - p.low_freq_factor), 0.0, 1.0);
+                f *= m + (1.0 - m) / s;
+            }
+            if (freq_factors) {
+                if (!(freq_factors[i] > 0.0f) || !std::isfinite(freq_factors[i]))
+                    invalid("rope_create: frequency factors must be positive");
+                f /= freq_factors[i];
+            }
+            turns[(size_t)i] = f / pi2;
+        }
+        DeviceScope dev(ctx);
+        auto r = std::make_unique<BeaconCudaRope>();
+        r->ctx = ctx;
+        r->rotary_dim = p.rotary_dim;
+        r->layout = p.layout;
+        r->amplitude = p.attention_factor != 0.0f ? p.attention_factor
+                       : p.scaling == BEACON_CUDA_ROPE_SCALING_YARN ? (float)(0.1 * std::log(s) + 1.0) : 1.0f;
+        r->turns = std::make_unique<DeviceBuffer>((size_t)half * sizeof(double));
+        BC_CUDA(cudaMemcpy(r->turns->ptr, turns.data(), (size_t)half * sizeof(double), cudaMemcpyHostToDevice));
+        *out_rope = r.release();
+        return BEACON_CUDA_OK;
+    });
+}
+
+void beacon_cuda_rope_destroy(BeaconCudaRope* rope) { delete rope; }
+
+int32_t beacon_cuda_op_rope_scaled(BeaconCudaContext* ctx, BeaconCudaStream* stream, const BeaconCudaTensor* x,
+                                   const BeaconCudaTensor* positions, const BeaconCudaRope* rope,
+                                   BeaconCudaTensor** inout_out) {
+    return guard([&]() -> int32_t {
+        require(ctx && stream && x && positions && rope && inout_out, "rope_scaled: null argument");
+        check_stream(ctx, stream, "rope_scaled");
+        check_rows(ctx, x, "rope_scaled");
+        check_ids(ctx, positions, x->shape[0], "rope_scaled: positions");
+        check_rope(ctx, rope, x->shape[2], "rope_scaled");
+        DeviceScope dev(ctx);
+        OutTensor out(ctx, inout_out, x->shape, x->dtype, "rope_scaled");
+        out.check_overlap(x, true, "rope_scaled");
+        out.check_overlap(positions, false, "rope_scaled");
+        RowArgs a;
+        a.seg[0].src = x->data();
+        a.seg[0].dst = out.data();
+        a.seg[0].heads = (int)x->shape[1];
+        a.seg[0].turn = true;
+        a.tokens = x->shape[0];
+        a.dim = (int)x->shape[2];
+        a.positions = static_cast<const int32_t*>(positions->data());
+        launch_rows(ctx, a, x->dtype, x->dtype, rope, stream->s);
+        out.release();
+        return BEACON_CUDA_OK;
+    });
+}
+
+int32_t beacon_cuda_op_qk_norm_rope(BeaconCudaContext* ctx, BeaconCudaStream* stream, const BeaconCudaTensor* q,
+                                    const BeaconCudaTensor* k, const BeaconCudaTensor* q_weight,
+                                    const BeaconCudaTensor* k_weight, float eps, const BeaconCudaTensor* positions,
+                                    const BeaconCudaRope* rope, BeaconCudaTensor** inout_q, BeaconCudaTensor** inout_k) {
+    return guard([&]() -> int32_t {
+        require(ctx && stream && q && k && q_weight && k_weight && inout_q && inout_k, "qk_norm_rope: null argument");
+        require(positions || !rope, "qk_norm_rope: a rotation needs positions");
+        check_stream(ctx, stream, "qk_norm_rope");
+        check_rows(ctx, q, "qk_norm_rope");
+        check_rows(ctx, k, "qk_norm_rope");
+        if (q->dtype != k->dtype) fail(BEACON_CUDA_ERR_UNSUPPORTED_DTYPE, "qk_norm_rope: q and k must have one dtype");
+        if (q->shape[0] != k->shape[0] || q->shape[2] != k->shape[2])
+            shape_err("qk_norm_rope: q and k must have the same rows and head size");
+        for (const BeaconCudaTensor* w : {q_weight, k_weight}) {
+            check_tensor(ctx, w, "qk_norm_rope");
+            if (w->dtype != BEACON_CUDA_DTYPE_F32 && w->dtype != BEACON_CUDA_DTYPE_F16)
+                fail(BEACON_CUDA_ERR_UNSUPPORTED_DTYPE, "qk_norm_rope: weights must be F32 or F16");
+            if (w->numel() != q->shape[2]) shape_err("qk_norm_rope: a weight needs one value per head value");
+        }
+        if (!(eps >= 0.0f)) invalid("qk_norm_rope: eps must not be negative");
+        if (positions) check_ids(ctx, positions, q->shape[0], "qk_norm_rope: positions");
+        check_rope(ctx, rope, q->shape[2], "qk_norm_rope");
+        DeviceScope dev(ctx);
+        OutTensor oq(ctx, inout_q, q->shape, q->dtype, "qk_norm_rope"), ok(ctx, inout_k, k->shape, k->dtype, "qk_norm_rope");
+        for (const BeaconCudaTensor* other : {q_weight, k_weight, positions}) {
+            oq.check_overlap(other, false, "qk_norm_rope");
+            ok.check_overlap(other, false, "qk_norm_rope");
+        }
+        oq.check_overlap(q, true, "qk_norm_rope");
+        oq.check_overlap(k, false, "qk_norm_rope");
+        ok.check_overlap(k, true, "qk_norm_rope");
+        ok.check_overlap(q, false, "qk_norm_rope");
+        ok.check_overlap(oq.get(), false, "qk_norm_rope");
+        RowArgs a;
+        const BeaconCudaTensor* in[2] = {q, k};
+        const BeaconCudaTensor* w[2] = {q_weight, k_weight};
+        void* dst[2] = {oq.data(), ok.data()};
+        for (int i = 0; i < 2; ++i) {
+            a.seg[i].src = in[i]->data();
+            a.seg[i].dst = dst[i];
+            a.seg[i].heads = (int)in[i]->shape[1];
+            a.seg[i].weight = w[i]->data();
+            a.seg[i].weight_dtype = w[i]->dtype;
+            a.seg[i].turn = rope != nullptr;
+        }
+        a.tokens = q->shape[0];
+        a.dim = (int)q->shape[2];
+        a.eps = eps;
+        a.positions = positions ? static_cast<const int32_t*>(positions->data()) : nullptr;
+        launch_rows(ctx, a, q->dtype, q->dtype, rope, stream->s);
+        oq.release();
+        ok.release();
+        return BEACON_CUDA_OK;
+    });
+}
+
+int32_t beacon_cuda_op_paged_append(BeaconCudaContext* ctx, BeaconCudaStream* stream, BeaconCudaTensor* cache_k,
+                                    BeaconCudaTensor* cache_v, const BeaconCudaTensor* new_k,
+                                    const BeaconCudaTensor* new_v, const BeaconCudaTensor* page_table,
+                                    const BeaconCudaTensor* seq_ids, const BeaconCudaTensor* positions,
+                                    const BeaconCudaRope* rope) {
+    return guard([&]() -> int32_t {
+        require(ctx && stream && cache_k && cache_v && new_k && new_v && page_table && positions,
+                "paged_append: null argument");
+        check_stream(ctx, stream, "paged_append");
+        check_rows(ctx, new_k, "paged_append");
+        check_rows(ctx, new_v, "paged_append");
+        if (new_k->shape != new_v->shape) shape_err("paged_append: new_k and new_v must have one shape");
+        if (new_k->dtype != new_v->dtype) fail(BEACON_CUDA_ERR_UNSUPPORTED_DTYPE, "paged_append: new_k and new_v must have one dtype");
+        for (const BeaconCudaTensor* c : {static_cast<const BeaconCudaTensor*>(cache_k), static_cast<const BeaconCudaTensor*>(cache_v)}) {
+            check_tensor(ctx, c, "paged_append");
+            if (c->dtype != BEACON_CUDA_DTYPE_F32 && c->dtype != BEACON_CUDA_DTYPE_F16 && c->dtype != BEACON_CUDA_DTYPE_BF16)
+                fail(BEACON_CUDA_ERR_UNSUPPORTED_DTYPE, "paged_append: caches must be F32, F16 or BF16");
+            if (c->shape.size() != 4 || c->shape[2] != new_k->shape[1] || c->shape[3] != new_k->shape[2] || c->shape[1] < 1)
+                shape_err("paged_append: caches must be [pages, page_size, heads, dim]");
+        }
+        if (cache_k->shape != cache_v->shape || cache_k->dtype != cache_v->dtype)
+            shape_err("paged_append: both caches must be alike");
+        check_tensor(ctx, page_table, "paged_append");
+        if (page_table->dtype != BEACON_CUDA_DTYPE_I32) fail(BEACON_CUDA_ERR_UNSUPPORTED_DTYPE, "paged_append: page_table must be I32");
+        if (page_table->shape.size() != 2) shape_err("paged_append: page_table must be [B, max_pages]");
+        const int64_t T = new_k->shape[0];
+        check_ids(ctx, positions, T, "paged_append: positions");
+        if (seq_ids) check_ids(ctx, seq_ids, T, "paged_append: seq_ids");
+        else if (page_table->shape[0] != T) shape_err("paged_append: without seq_ids every row is a sequence of page_table");
+        check_rope(ctx, rope, new_k->shape[2], "paged_append");
+        DeviceScope dev(ctx);
+        BeaconCudaTensor *pk = cache_k, *pv = cache_v;
+        OutTensor ok(ctx, &pk, cache_k->shape, cache_k->dtype, "paged_append"), ov(ctx, &pv, cache_v->shape, cache_v->dtype, "paged_append");
+        ok.check_overlap(cache_v, false, "paged_append");
+        for (const BeaconCudaTensor* t : {new_k, new_v, page_table, seq_ids, positions}) {
+            ok.check_overlap(t, false, "paged_append");
+            ov.check_overlap(t, false, "paged_append");
+        }
+        RowArgs a;
+        a.seg[0].src = new_k->data();
+        a.seg[1].src = new_v->data();
+        a.seg[0].dst = cache_k->data();
+        a.seg[1].dst = cache_v->data();
+        a.seg[0].heads = a.seg[1].heads = (int)new_k->shape[1];
+        a.seg[0].turn = rope != nullptr;
+        a.tokens = T;
+        a.dim = (int)new_k->shape[2];
+        a.positions = static_cast<const int32_t*>(positions->data());
+        a.table = static_cast<const int32_t*>(page_table->data());
+        a.seq_ids = seq_ids ? static_cast<const int32_t*>(seq_ids->data()) : nullptr;
+        a.seqs = page_table->shape[0];
+        a.max_pages = page_table->shape[1];
+        a.pages = cache_k->shape[0];
+        a.page_size = cache_k->shape[1];
+        a.err = stream_error_word(stream);
+        launch_rows(ctx, a, new_k->dtype, cache_k->dtype, rope, stream->s);
+        return BEACON_CUDA_OK;
+    });
+}
+
+}  // extern "C"

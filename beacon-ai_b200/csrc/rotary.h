@@ -1,0 +1,59 @@
+// rotary.h -- rotation tables and the row kernel shared by the rotary, norm
+// and cache-append operations (rotary.cu).
+#pragma once
+
+#include <memory>
+
+#include "internal.h"
+
+struct BeaconCudaRope {
+    BeaconCudaContext* ctx = nullptr;
+    int rotary_dim = 0;
+    int layout = BEACON_CUDA_ROPE_INTERLEAVED;
+    float amplitude = 1.0f;                   // factor on sine and cosine
+    std::unique_ptr<bc::DeviceBuffer> turns;  // f64 [rotary_dim / 2]: f_i / 2 pi
+};
+
+namespace bc {
+
+// Makes the context's device current for a call and puts back the caller's.
+struct DeviceScope {
+    int before = -1;
+    explicit DeviceScope(const BeaconCudaContext* ctx) {
+        BC_CUDA(cudaGetDevice(&before));
+        if (before == ctx->device)
+            before = -1;
+        else
+            BC_CUDA(cudaSetDevice(ctx->device));
+    }
+    ~DeviceScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+// The output of an operation: the caller's tensor, checked against the
+// result's shape, dtype and inputs, or a new one that is handed over last.
+class OutTensor {
+   public:
+    OutTensor(BeaconCudaContext* ctx, BeaconCudaTensor** inout, const std::vector<int64_t>& shape, int32_t dtype,
+              const char* what);
+    void* data() const { return t_->data(); }
+    BeaconCudaTensor* get() const { return t_; }
+    // The output may be `x` itself (same bytes) when in_place, else must not touch it.
+    void check_overlap(const BeaconCudaTensor* x, bool in_place, const char* what) const;
+    void release() {
+        made_.release();
+        *inout_ = t_;
+    }
+
+   private:
+    BeaconCudaTensor** inout_;
+    BeaconCudaTensor* t_;
+    std::unique_ptr<BeaconCudaTensor> made_;  // freed if the call throws
+};
+
+// Tensors of an operation must live on its context.
+void check_tensor(const BeaconCudaContext* ctx, const BeaconCudaTensor* t, const char* what);
+void check_stream(const BeaconCudaContext* ctx, const BeaconCudaStream* stream, const char* what);
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+}  // namespace bc

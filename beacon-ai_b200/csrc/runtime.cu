@@ -144,7 +144,43 @@ static std::vector<cudaError_t (*)(long long)>& wait_limit_setters() {
 }
 void register_wait_limit_setter(cudaError_t (*setter)(long long)) { wait_limit_setters().push_back(setter); }
 
+int* stream_error_word(BeaconCudaStream* stream) {
+    constexpr int kSlabWords = 1024;
+    if (stream->err_word) return stream->err_word;
+    BeaconCudaContext* ctx = stream->ctx;
+    std::lock_guard<std::mutex> lk(ctx->streams_mu);
+    if (stream->err_word) return stream->err_word;
+    if (ctx->err_slabs.empty() || ctx->err_used == kSlabWords) {
+        // a capture on this thread forbids allocating unless the thread's
+        // capture mode is relaxed; no stream work is enqueued here
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        BC_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        void* p = nullptr;
+        const cudaError_t e = cudaHostAlloc(&p, kSlabWords * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        cuda_check(e, "cudaHostAlloc");
+        std::memset(p, 0, kSlabWords * sizeof(int));
+        try {
+            ctx->err_slabs.push_back(static_cast<int*>(p));
+        } catch (...) {
+            cudaFreeHost(p);
+            throw;
+        }
+        ctx->err_used = 0;
+    }
+    stream->err_word = ctx->err_slabs.back() + ctx->err_used++;
+    return stream->err_word;
+}
+
 void check_stream_timeout(BeaconCudaStream* stream) {
+    if (stream && stream->ctx && stream->err_word) {
+        volatile int* w = stream->err_word;  // the stream's work is done: no kernel is writing it
+        if (*w) {
+            *w = 0;
+            shape_err("a sequence number, position, length or page id held in a device tensor is out of range; "
+                      "the rows it names were left out");
+        }
+    }
     if (!stream || !stream->ws.buf) return;
     if (stream->ctx) set_device(stream->ctx);
     int flag = 0;
@@ -288,10 +324,14 @@ void beacon_cuda_context_destroy(BeaconCudaContext* ctx) {
     {
         // streams outliving their context keep their handles but lose the link
         std::lock_guard<std::mutex> lk(ctx->streams_mu);
-        for (BeaconCudaStream* st : ctx->streams) st->ctx = nullptr;
+        for (BeaconCudaStream* st : ctx->streams) {
+            st->ctx = nullptr;
+            st->err_word = nullptr;
+        }
         ctx->streams.clear();
     }
     if (ctx->internal) cudaStreamDestroy(ctx->internal);
+    for (int* p : ctx->err_slabs) cudaFreeHost(p);
     comm_destroy(ctx);
     delete ctx;
 }

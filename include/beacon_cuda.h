@@ -283,6 +283,109 @@ int32_t beacon_cuda_quantize_blocks(BeaconCudaContext* ctx, BeaconCudaStream* st
                                     int64_t n_rows, int64_t k, int32_t dtype, int32_t nibble_order,
                                     void* d_out);
 
+/* === Rotary positions and paged key/value caches ===
+ * The attention block over caches whose rows live in pages, so that many
+ * sequences of different lengths, and several continuations of one prompt,
+ * share device memory. Tensors are token-major: row t of a [T, heads, dim]
+ * tensor is one token, whatever sequence it belongs to. No counterpart in the
+ * reference, whose cache is one contiguous [max_ctx, Hkv, D] array per
+ * sequence (kv_cache.rs:13-21) and whose RoPE is the interleaved unscaled one
+ * (ops.rs:124-142).
+ *
+ * `inout_out` of these operations: *inout_out == NULL on entry makes a new
+ * tensor; otherwise it must be a tensor of the result's shape and dtype, which
+ * is written in place and stays the caller's (no device memory is allocated
+ * for the result then, so the call can be captured in a CUDA graph). An
+ * output may be the input it is computed from elementwise (the same tensor or
+ * the same address); any other overlap is refused.
+ *
+ * Positions, sequence numbers, lengths and page tables are device tensors, so
+ * the kernels check them: an entry that is out of range is never used as an
+ * address, and the next synchronising call on the stream (stream_synchronize,
+ * tensor_eval; tensor_read_*) returns SHAPE_MISMATCH. */
+typedef struct BeaconCudaRope BeaconCudaRope;
+/* Which values of a head form pair i of rotary_dim/2: (2i, 2i+1), or
+ * (i, i + rotary_dim/2). */
+typedef enum { BEACON_CUDA_ROPE_INTERLEAVED = 0, BEACON_CUDA_ROPE_HALF = 1 } BeaconCudaRopeLayout;
+/* Frequencies f_i = theta^(-2i/rotary_dim) for contexts longer than trained
+ * (factor s, original context c):
+ *  LINEAR: f_i / s.
+ *  YARN:   f_i ((1 - r) + r/s), r = clamp((i - lo) / (hi - lo), 0, 1), where lo
+ *          (hi) is the pair that turns beta_fast (beta_slow) times in c,
+ *          rounded down (up) and kept in [0, rotary_dim - 1].
+ *  BANDS:  f_i (m + (1 - m)/s), m = clamp((c f_i / 2 pi - low_freq_factor) /
+ *          (high_freq_factor - low_freq_factor), 0, 1). */
+typedef enum {
+    BEACON_CUDA_ROPE_SCALING_NONE = 0,
+    BEACON_CUDA_ROPE_SCALING_LINEAR = 1,
+    BEACON_CUDA_ROPE_SCALING_YARN = 2,
+    BEACON_CUDA_ROPE_SCALING_BANDS = 3
+} BeaconCudaRopeScaling;
+typedef struct {
+    float theta;
+    int32_t rotary_dim;       /* leading values of a head that turn (even, <= 512) */
+    int32_t layout, scaling;
+    float factor;             /* >= 1; 1 with NONE */
+    int32_t original_context; /* YARN, BANDS */
+    float beta_fast, beta_slow;                 /* YARN */
+    float low_freq_factor, high_freq_factor;    /* BANDS */
+    float attention_factor;   /* on sine and cosine; 0: 0.1 ln(factor) + 1 for YARN, 1 otherwise */
+} BeaconCudaRopeParams;
+/* The table of a rotation, made once and kept by the caller: angles are
+ * position * f_i in 64 bits reduced to one turn, so far positions lose
+ * nothing. freq_factors (host, rotary_dim/2 values, NULL = none) divide the
+ * frequencies (GGUF rope_freqs). */
+int32_t beacon_cuda_rope_create(BeaconCudaContext* ctx, const BeaconCudaRopeParams* params,
+                                const float* freq_factors, BeaconCudaRope** out_rope);
+void    beacon_cuda_rope_destroy(BeaconCudaRope* rope);
+/* x [T, heads, dim] (F32, F16, BF16) with the first rotary_dim values of
+ * every head turned to positions[t] (I32 [T], any value); out: x's dtype,
+ * rounded once. */
+int32_t beacon_cuda_op_rope_scaled(BeaconCudaContext* ctx, BeaconCudaStream* stream, const BeaconCudaTensor* x,
+                                   const BeaconCudaTensor* positions, const BeaconCudaRope* rope,
+                                   BeaconCudaTensor** inout_out);
+/* Every head of q [T, H, dim] and k [T, Hkv, dim] normalised, x w /
+ * sqrt(mean(x^2) + eps) with w [dim] (F32 or F16) of its own kind, and turned
+ * as rope_scaled does (rope NULL: normalised only), in one pass. */
+int32_t beacon_cuda_op_qk_norm_rope(BeaconCudaContext* ctx, BeaconCudaStream* stream, const BeaconCudaTensor* q,
+                                    const BeaconCudaTensor* k, const BeaconCudaTensor* q_weight,
+                                    const BeaconCudaTensor* k_weight, float eps, const BeaconCudaTensor* positions,
+                                    const BeaconCudaRope* rope, BeaconCudaTensor** inout_q, BeaconCudaTensor** inout_k);
+/* Writes rows new_k (turned to their positions; rope NULL: as they are) and
+ * new_v, both [T, Hkv, D], into the pages of cache_k/cache_v [pages,
+ * page_size, Hkv, D] (F32, F16, BF16; rounded once). Row t goes to position p =
+ * positions[t] of sequence b = seq_ids[t] (NULL: b = t): page
+ * page_table[b][p / page_size], row p % page_size. page_table I32 [B,
+ * max_pages]. A row with a negative position is skipped (padding). Of two rows
+ * of one call at the same place either may win, value by value. */
+int32_t beacon_cuda_op_paged_append(BeaconCudaContext* ctx, BeaconCudaStream* stream, BeaconCudaTensor* cache_k,
+                                    BeaconCudaTensor* cache_v, const BeaconCudaTensor* new_k,
+                                    const BeaconCudaTensor* new_v, const BeaconCudaTensor* page_table,
+                                    const BeaconCudaTensor* seq_ids, const BeaconCudaTensor* positions,
+                                    const BeaconCudaRope* rope);
+/* Causal attention of q [T, H, D] over the paged caches, H a multiple of Hkv
+ * (query head h reads KV head h / (H/Hkv)). Sequence b's kv_lens[b] (I32 [B])
+ * rows include its new ones. Its queries are rows query_starts[b] ..
+ * query_starts[b+1] of q (I32 [B+1], from 0 upwards; NULL: T == B, one row
+ * each), the last n = query_starts[b+1] - query_starts[b] positions: query j
+ * sees the keys at positions 0 .. kv_lens[b] - n + j.
+ *   Shared prefixes: sequences group_starts[g] .. group_starts[g+1] (I32 [G+1],
+ * 0 upwards to B; NULL: none) hold the same keys below position prefix_lens[g]
+ * (I32 [G]); those are read through the page table row of the group's first
+ * sequence, once for all queries of the group.
+ *   scale multiplies the scores. A query that sees no key gives zeros. Rows of
+ * q behind the last sequence are not written. Cache rows at positions >=
+ * kv_lens[b] are never read. Dtypes (q, caches): (F32, F16), (F16, F16), (BF16,
+ * BF16) and (F32, F32); D a multiple of 8 up to 256, tensors 16-byte aligned.
+ * out: q's shape and dtype. Split partial results use the stream's scratch, or
+ * memory that belongs to the graph while the stream is being captured. */
+int32_t beacon_cuda_op_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream, const BeaconCudaTensor* q,
+                                       const BeaconCudaTensor* cache_k, const BeaconCudaTensor* cache_v,
+                                       const BeaconCudaTensor* page_table, const BeaconCudaTensor* kv_lens,
+                                       const BeaconCudaTensor* query_starts, const BeaconCudaTensor* group_starts,
+                                       const BeaconCudaTensor* prefix_lens, float scale,
+                                       BeaconCudaTensor** inout_out);
+
 /* === Fused decoder runtime (Engine<B>::forward, engine.rs:190-456) === */
 typedef struct {
     int32_t vocab_size, hidden_size, num_layers, num_heads, num_kv_heads, head_dim;
