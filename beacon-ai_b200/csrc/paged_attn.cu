@@ -101,6 +101,88 @@ __global__ void __launch_bounds__(kAnyWarps * 32) paged_attn_any_kernel(const Pa
     }
 }
 
+// Scratch of one call: the stream's workspace, which later calls on the stream
+// use again in stream order. A captured call gets memory of its graph instead,
+// so graphs captured on one stream can replay at the same time.
+class CallScratch {
+   public:
+    CallScratch(BeaconCudaContext* ctx, BeaconCudaStream* stream, size_t bytes) : s_(stream->s) {
+        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+        BC_CUDA(cudaStreamIsCapturing(s_, &st));
+        if (st == cudaStreamCaptureStatusNone) {
+            std::lock_guard<std::mutex> lk(ctx->streams_mu);
+            p_ = stream->ws.get(bytes, s_);
+        } else {
+            BC_CUDA(cudaMallocAsync(&p_, bytes, s_));
+            graph_ = true;
+        }
+    }
+    ~CallScratch() {
+        if (graph_) cudaFreeAsync(p_, s_);
+    }
+    CallScratch(const CallScratch&) = delete;
+    CallScratch& operator=(const CallScratch&) = delete;
+    uint8_t* data() const { return static_cast<uint8_t*>(p_); }
+    bool of_graph() const { return graph_; }
+
+   private:
+    cudaStream_t s_;
+    void* p_ = nullptr;
+    bool graph_ = false;
+};
+
+// Carves PartArgs out of one scratch region (base null: only counts the bytes).
+class Carve {
+   public:
+    explicit Carve(uint8_t* base) : base_(base) {}
+    template <typename T>
+    T* take(int64_t n) {
+        T* p = base_ ? reinterpret_cast<T*>(base_ + used_) : nullptr;
+        used_ += (size_t)((n * (int64_t)sizeof(T) + 255) / 256 * 256);
+        return p;
+    }
+    size_t used() const { return used_; }
+
+   private:
+    uint8_t* base_;
+    size_t used_ = 0;
+};
+
+PartArgs carve_part(Carve& c, const PagedArgs& a, int ctas, int slot_rows, bool by_row) {
+    PartArgs p;
+    const int64_t rows = (int64_t)a.T * a.H, slots = (int64_t)ctas * slot_rows;
+    p.stat = c.take<float4>(rows);
+    p.head = c.take<float>((by_row ? rows : slots) * a.D);
+    p.tail_stat = c.take<float2>(slots);
+    p.tail = c.take<float>(slots * a.D);
+    p.by_row = by_row;
+    p.slot_rows = slot_rows;
+    p.ctas = ctas;
+    return p;
+}
+
+void run_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream, const PagedArgs& a, int32_t tq, int32_t tk) {
+    const int32_t F32 = BEACON_CUDA_DTYPE_F32, F16 = BEACON_CUDA_DTYPE_F16;
+    if (tk != F32 && a.D <= 128 && !a.qstarts && a.G <= kDecodeMaxGroup && !a.gstarts) {
+        const int ctas = paged_decode_ctas(ctx, a, tq == F32);
+        Carve count(nullptr);
+        carve_part(count, a, ctas, a.G, false);
+        CallScratch scratch(ctx, stream, count.used());
+        Carve c(scratch.data());
+        const PartArgs rest = carve_part(c, a, ctas, a.G, false);
+        launch_paged_decode(a, rest, tq, tk, stream->s, !scratch.of_graph());
+        launch_paged_combine(a, PartArgs{}, rest, tq, stream->s);
+        return;
+    }
+    const dim3 grid((unsigned)a.T, (unsigned)a.H);
+    cudaStream_t s = stream->s;
+    if (tq == F32 && tk == F32) paged_attn_any_kernel<float, float><<<grid, kAnyWarps * 32, 0, s>>>(a);
+    else if (tq == F32) paged_attn_any_kernel<float, __half><<<grid, kAnyWarps * 32, 0, s>>>(a);
+    else if (tq == F16) paged_attn_any_kernel<__half, __half><<<grid, kAnyWarps * 32, 0, s>>>(a);
+    else paged_attn_any_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, kAnyWarps * 32, 0, s>>>(a);
+    BC_LAUNCHED("paged_attn_any_kernel");
+}
+
 void check_i32(const BeaconCudaContext* ctx, const BeaconCudaTensor* t, int64_t n, const char* what) {
     check_tensor(ctx, t, what);
     if (t->dtype != BEACON_CUDA_DTYPE_I32) fail(BEACON_CUDA_ERR_UNSUPPORTED_DTYPE, std::string(what) + " must be I32");
@@ -139,6 +221,7 @@ extern "C" int32_t beacon_cuda_op_paged_attention(BeaconCudaContext* ctx, Beacon
         if (D < 8 || D > kAnyMaxDim || D % 8) shape_err("paged_attention: the head size must be a multiple of 8, 8 to 256");
         if (Hkv < 1 || H < 1 || H % Hkv || H > 65535) shape_err("paged_attention: H must be a multiple of Hkv, at most 65535");
         if (cache_k->shape[1] < 1 || cache_k->shape[1] > 0x7FFFFFFF) shape_err("paged_attention: empty pages");
+        if (cache_k->shape[0] * cache_k->shape[1] > 0x7FFFFFFF) shape_err("paged_attention: more than 2^31 - 1 cache rows");
         check_i32(ctx, page_table, -1, "paged_attention: page_table");
         if (page_table->shape.size() != 2) shape_err("paged_attention: page_table must be [B, max_pages]");
         const int64_t B = page_table->shape[0], max_pages = page_table->shape[1];
@@ -183,14 +266,7 @@ extern "C" int32_t beacon_cuda_op_paged_attention(BeaconCudaContext* ctx, Beacon
         a.page_size = (int)cache_k->shape[1];
         a.scale = scale;
         a.err = stream_error_word(stream);
-        if (T > 0 && B > 0) {
-            const dim3 grid((unsigned)T, (unsigned)H);
-            if (tq == F32 && tk == F32) paged_attn_any_kernel<float, float><<<grid, kAnyWarps * 32, 0, stream->s>>>(a);
-            else if (tq == F32) paged_attn_any_kernel<float, __half><<<grid, kAnyWarps * 32, 0, stream->s>>>(a);
-            else if (tq == F16) paged_attn_any_kernel<__half, __half><<<grid, kAnyWarps * 32, 0, stream->s>>>(a);
-            else paged_attn_any_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, kAnyWarps * 32, 0, stream->s>>>(a);
-            BC_LAUNCHED("paged_attn_any_kernel");
-        }
+        if (T > 0 && B > 0) run_paged_attention(ctx, stream, a, tq, tk);
         out.release();
         return BEACON_CUDA_OK;
     });

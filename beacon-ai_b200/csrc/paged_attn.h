@@ -24,6 +24,40 @@ struct PagedArgs {
     int* err = nullptr;
 };
 
+// Partial results. The keys of a query row fall into two parts, its group's
+// prefix (kind 0) and its own sequence's rows behind it (kind 1). Each part is
+// cut into key tiles; the tiles of all rows form one line that the CTAs of a
+// launch share evenly, so a row's tiles may lie with several neighbouring
+// CTAs. The CTA that has the first of them leaves (m, l, first CTA, last CTA)
+// in `stat` and its sums in `head`; the CTAs after it, each of which has at
+// most one such row block, leave theirs under their own number in `tail`.
+// m is the largest score times log2(e), l the sum of 2^(score - m), and the
+// sums are of 2^(score - m) v.
+struct PartArgs {
+    float4* stat = nullptr;   // [T * H]: m, l and, as integers, the CTAs
+    float* head = nullptr;    // [T * H][D], or [ctas][slot_rows][D] when !by_row
+    float2* tail_stat = nullptr;  // [ctas][slot_rows]
+    float* tail = nullptr;        // [ctas][slot_rows][D]
+    int by_row = 0;    // heads are kept per row: a row has both kinds
+    int slot_rows = 0;  // rows of a row block
+    int ctas = 0;
+};
+
+// CTAs that take part (each then has a tile, so those between two that share a
+// row have a part of it), the share of CTA c of the line of `total` tiles, and
+// the CTA that holds tile u.
+__device__ __forceinline__ int sharers(long long total, int ctas) { return total < ctas ? (int)total : ctas; }
+__device__ __forceinline__ long long share_begin(long long total, int ctas, int c) { return total * c / ctas; }
+__device__ __forceinline__ int share_of(long long total, int ctas, long long u) {
+    return (int)(((u + 1) * ctas - 1) / total);
+}
+
+// Launchers. `prefix`/`rest`: kinds 0 and 1.
+constexpr int kDecodeMaxGroup = 16;  // query heads of one KV head that paged_decode_kernel holds
+int paged_decode_ctas(const BeaconCudaContext* ctx, const PagedArgs& a, bool split);
+void launch_paged_decode(const PagedArgs& a, const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s, bool pdl);
+void launch_paged_combine(const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, int32_t tq, cudaStream_t s);
+
 // A start array entry kept inside [0, n] (callers hold it in a device tensor).
 __device__ __forceinline__ int start_at(const int32_t* s, int i, int n, int* err) {
     const int v = s[i];
