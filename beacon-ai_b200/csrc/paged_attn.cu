@@ -163,15 +163,29 @@ PartArgs carve_part(Carve& c, const PagedArgs& a, int ctas, int slot_rows, bool 
 
 void run_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream, const PagedArgs& a, int32_t tq, int32_t tk) {
     const int32_t F32 = BEACON_CUDA_DTYPE_F32, F16 = BEACON_CUDA_DTYPE_F16;
-    if (tk != F32 && a.D <= 128 && !a.qstarts && a.G <= kDecodeMaxGroup && !a.gstarts) {
-        const int ctas = paged_decode_ctas(ctx, a, tq == F32);
-        Carve count(nullptr);
-        carve_part(count, a, ctas, a.G, false);
-        CallScratch scratch(ctx, stream, count.used());
-        Carve c(scratch.data());
-        const PartArgs rest = carve_part(c, a, ctas, a.G, false);
-        launch_paged_decode(a, rest, tq, tk, stream->s, !scratch.of_graph());
-        launch_paged_combine(a, PartArgs{}, rest, tq, stream->s);
+    if (tk != F32 && a.D <= 128) {
+        // single rows of few heads: paged_decode_kernel; prefixes, several rows
+        // of a sequence or many heads: the tensor-core kernel, whose row block is 128
+        const bool decode = !a.qstarts && a.G <= kDecodeMaxGroup, tc = a.gstarts || !decode;
+        const bool split = tq == F32, by_row = a.gstarts != nullptr;
+        const PagedTcPlan plan = tc ? plan_paged_tc(ctx, a, split, !decode) : PagedTcPlan{};
+        const int dctas = decode ? paged_decode_ctas(ctx, a, split) : 0;
+        PartArgs prefix, rest;
+        auto carve = [&](uint8_t* base) {
+            Carve c(base);
+            if (tc && a.gstarts) prefix = carve_part(c, a, plan.ctas, plan.slot_rows, by_row);
+            rest = decode ? carve_part(c, a, dctas, a.G, by_row) : carve_part(c, a, plan.ctas, plan.slot_rows, by_row);
+            return c.used();
+        };
+        CallScratch scratch(ctx, stream, carve(nullptr));
+        carve(scratch.data());
+        bool pdl = !scratch.of_graph();  // a graph's allocation comes first
+        if (tc) {
+            launch_paged_tc(plan, a, prefix, rest, tq, tk, stream->s, pdl);
+            pdl = true;
+        }
+        if (decode) launch_paged_decode(a, rest, tq, tk, stream->s, pdl);
+        launch_paged_combine(a, prefix, rest, tq, stream->s);
         return;
     }
     const dim3 grid((unsigned)a.T, (unsigned)a.H);
@@ -226,6 +240,7 @@ extern "C" int32_t beacon_cuda_op_paged_attention(BeaconCudaContext* ctx, Beacon
         if (page_table->shape.size() != 2) shape_err("paged_attention: page_table must be [B, max_pages]");
         const int64_t B = page_table->shape[0], max_pages = page_table->shape[1];
         if (T > 0x3FFFFFFF || B > 0x3FFFFFFF || max_pages > 0x7FFFFFFF) shape_err("paged_attention: too many rows or pages");
+        if (T * H > 0x7FFFFFFF) shape_err("paged_attention: more than 2^31 - 1 query heads");
         check_i32(ctx, kv_lens, B, "paged_attention: kv_lens");
         if (query_starts) check_i32(ctx, query_starts, B + 1, "paged_attention: query_starts");
         else if (T != B) shape_err("paged_attention: without query_starts every sequence has one query row");

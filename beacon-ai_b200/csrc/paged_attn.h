@@ -56,6 +56,17 @@ __device__ __forceinline__ int share_of(long long total, int ctas, long long u) 
 constexpr int kDecodeMaxGroup = 16;  // query heads of one KV head that paged_decode_kernel holds
 int paged_decode_ctas(const BeaconCudaContext* ctx, const PagedArgs& a, bool split);
 void launch_paged_decode(const PagedArgs& a, const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s, bool pdl);
+// Rows of a block and CTAs of the tensor-core kernel (paged_tc.cu), for the
+// prefixes and, when with_rest, the rest of every sequence.
+struct PagedTcPlan {
+    bool two = false;    // two row tiles of 128 share a CTA's keys
+    bool rest = false;
+    int slot_rows = 128;
+    int ctas = 0;
+};
+PagedTcPlan plan_paged_tc(const BeaconCudaContext* ctx, const PagedArgs& a, bool split, bool with_rest);
+void launch_paged_tc(const PagedTcPlan& plan, const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, int32_t tq,
+                     int32_t tk, cudaStream_t s, bool pdl);
 void launch_paged_combine(const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, int32_t tq, cudaStream_t s);
 
 // A start array entry kept inside [0, n] (callers hold it in a device tensor).
@@ -120,10 +131,10 @@ __device__ __forceinline__ SeqInfo seq_info(const PagedArgs& a, int b) {
     if (a.gstarts) {
         const int g = span_of(a.gstarts, a.groups, b);
         if (g >= 0) {
-            s.prefix = prefix_len(a, g);
             s.first = start_at(a.gstarts, g, a.B, a.err);
             start_at(a.gstarts, g + 1, a.B, a.err);
             if (s.first >= a.B) s.first = b;  // cannot hold b
+            s.prefix = min(prefix_len(a, g), kv_len(a, s.first));  // no row beyond what it holds is read
         }
     }
     return s;

@@ -393,12 +393,16 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedArgs a, c
         const PartArgs& p = kind ? rest : prefix;
         const float4 st = p.stat[row];
         const int c0 = __float_as_int(st.z), c1 = __float_as_int(st.w);
+        if (c0 < 0 || c1 < c0 || c1 >= p.ctas) {  // start arrays that contradict each other: no CTA had the row
+            *a.err = kErrIndex;
+            continue;
+        }
         if (kind == 1 && !on[0] && c0 == c1) return;  // written by the CTA that had all of it
         // row of the block that the CTAs share (its first token is the entry's)
         int q0 = s.q0;
         if (kind == 0 && a.qstarts) q0 = start_at(a.qstarts, s.first, a.T, a.err);
         else if (kind == 0) q0 = s.first;
-        const int r = (int)((((int64_t)(t - q0)) * a.G + h % a.G) % p.slot_rows);
+        const int r = (int)((((int64_t)max(0, t - q0)) * a.G + h % a.G) % p.slot_rows);
         const float* first = p.head + (p.by_row ? row : (int64_t)c0 * p.slot_rows + r) * a.D;
         for (int base = c0; base <= c1; base += 32) {
             const int c = base + lane;

@@ -1,0 +1,729 @@
+// paged_tc.cu -- paged attention of many query rows that share their keys
+// (prefixes of a group of sequences, prompts) on the 5th-generation tensor
+// cores.
+//
+// A row block is the query rows of one KV head that see the same keys: all
+// sequences of a group against its prefix, or the rows of one sequence against
+// its own keys (token-major, so row r is token r / G, head r % G). Per 128-key
+// tile S = Q K^T and O += P V are chains of tcgen05.mma (M 128, K 16) with
+// scores and sums in tensor memory. A CTA has two streams of them, each with
+// its own 128 score and DP sum columns and its own 128 softmax threads (one
+// row each), so that one stream's matrix products run under the other's
+// exponentials:
+//  * two row tiles (block of 256 rows) that share every key tile, or
+//  * one row tile (128 rows) whose streams take the even and the odd key tiles
+//    and are joined at the end. 32-bit queries come as two f16 parts (SPLIT):
+//    two products for the scores, and two for the sums, whose weights are
+//    split likewise.
+// P replaces S in place, 32 keys at a time: the 16 columns of packed weights
+// (then 16 of their remainders) lie where the 32 scores were, and are the A
+// operand of O += P V from tensor memory; V is read N-major.
+// Four producer warps copy key and value rows, page by page, with 16-byte
+// asynchronous copies into a ring of tiles in the 128-byte swizzle; one thread
+// issues the products. The key tiles of all blocks form one line that the CTAs
+// share evenly (PartArgs).
+// The running maximum moves only when a tile exceeds it by 2^8: the sums are
+// rescaled in tensor memory then, and the weights stay below 2^8.
+// Every wait is bounded; one that runs out marks the stream's error word, and
+// the CTA waits for what it issued and ends.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "internal.h"
+#include "kernels.h"
+#include "paged_attn.h"
+#include "paged_mma.cuh"
+
+namespace bc {
+namespace {
+
+constexpr int kTile = 128;              // rows of a row tile, keys of a key tile
+constexpr int kSoftWarps = 8;
+constexpr int kMmaWarp = kSoftWarps;
+constexpr int kLoadWarps = 4;
+constexpr int kTcThreads = 32 * (kSoftWarps + 1 + kLoadWarps);
+constexpr uint32_t kTmemCols = 512;     // S 2 x 128, O 2 x DP
+constexpr float kRescale = 8.0f;        // log2 of the largest weight
+
+template <int DP, bool SPLIT, bool TWO>
+struct TcSmem {
+    static constexpr int tile = kTile * DP * 2;
+    static constexpr int q_tiles = TWO || SPLIT ? 2 : 1;
+    static constexpr int stages = DP == 128 ? 6 - q_tiles : 8;
+    static constexpr size_t bytes = (size_t)(q_tiles + stages) * tile + 1024;
+};
+
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {  // 8-row atoms of 1024 bytes
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+           ((uint64_t)2 << 61);
+}
+// Values: 64 dims (128 bytes) of a key in a row, blocks of 64 dims 128 rows
+// apart (leading offset), 8-key atoms 1024 bytes apart (stride offset).
+__device__ __forceinline__ uint64_t desc_n_major(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)((kTile * 128) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+template <typename T>
+constexpr uint32_t idesc(int n, bool b_n_major) {
+    const uint32_t ty = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    return (1u << 4) | (ty << 7) | (ty << 10) | ((b_n_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(kTile >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(id), "r"((uint32_t)acc)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool acc) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+                 "r"(a), "l"(b), "r"(id), "r"((uint32_t)acc)
+                 : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+        "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+        "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// The rows that share keys: a group's queries against its prefix (kind 0), or a
+// sequence's queries against its own keys (kind 1).
+struct Block {
+    int kind = 0;
+    int b = 0;                   // page table row
+    int key0 = 0, key1 = 0;      // keys [key0, key1)
+    int tok0 = 0, rows = 0;      // query rows tok0 * G ..
+    int nq = 0, len = 0;         // kind 1: causal limits
+};
+__device__ __forceinline__ Block block_of(const PagedArgs& a, int e) {
+    Block k;
+    if (e < a.groups) {
+        const int lo = start_at(a.gstarts, e, a.B, a.err), hi = start_at(a.gstarts, e + 1, a.B, a.err);
+        if (hi < lo) *a.err = kErrIndex;
+        if (hi <= lo) return k;
+        k.b = lo;
+        k.key1 = min(prefix_len(a, e), kv_len(a, lo));
+        k.tok0 = a.qstarts ? start_at(a.qstarts, lo, a.T, a.err) : lo;
+        const int tok1 = a.qstarts ? start_at(a.qstarts, hi, a.T, a.err) : hi;
+        k.rows = max(0, tok1 - k.tok0) * a.G;
+        return k;
+    }
+    const SeqInfo s = seq_info(a, e - a.groups);
+    k.kind = 1;
+    k.b = e - a.groups;
+    k.key0 = s.prefix;
+    k.key1 = s.len;
+    k.tok0 = s.q0;
+    k.rows = s.nq * a.G;
+    k.nq = s.nq;
+    k.len = s.len;
+    return k;
+}
+// Key tiles that row tile rt of a block needs (its last row sees the most keys).
+__device__ __forceinline__ int tiles_of(const PagedArgs& a, const Block& k, int rt, int block_rows) {
+    int end = k.key1;
+    if (k.kind) end = min(end, k.len - k.nq + (min((rt + 1) * block_rows, k.rows) - 1) / a.G + 1);
+    return end > k.key0 ? (end - k.key0 + kTile - 1) / kTile : 0;
+}
+__device__ __forceinline__ int tiles_of_block(const PagedArgs& a, const Block& k, int block_rows) {
+    const int n = (k.rows + block_rows - 1) / block_rows;
+    if (k.kind == 0) return n * tiles_of(a, k, 0, block_rows);
+    int sum = 0;
+    for (int rt = 0; rt < n; ++rt) sum += tiles_of(a, k, rt, block_rows);
+    return sum;
+}
+
+// A CTA's next piece of the line: key tiles [tile, tile + n) of row tile rt.
+struct Piece {
+    Block k;
+    int e = 0, entries = 0, kvh = 0, rt = 0, tile = 0;
+    int tiles = 0;     // of the row tile
+    int n = 0;
+    long long u = 0;   // place of `tile` in the line
+    __device__ __forceinline__ void next(const PagedArgs& a, int block_rows, long long u1) {
+        u += n;
+        if (u >= u1) return;
+        tile = 0;
+        for (;;) {
+            ++rt;
+            if ((long long)rt * block_rows >= k.rows) {
+                rt = 0;
+                if (++kvh == a.Hkv) {
+                    kvh = 0;
+                    if (++e >= entries) return;  // not reached while u < u1
+                    k = block_of(a, e);
+                }
+                if (k.rows == 0) {
+                    kvh = a.Hkv - 1;
+                    rt = 0;
+                    tiles = 0;
+                    continue;
+                }
+            }
+            tiles = tiles_of(a, k, rt, block_rows);
+            if (tiles) break;
+        }
+        n = (int)min((long long)tiles, u1 - u);
+    }
+};
+
+template <typename TQ, typename T16, int DP, bool SPLIT, bool TWO>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    paged_tc_kernel(const PagedArgs a, const PartArgs prefix, const PartArgs rest, int entries, int line_ctas) {
+    using SM = TcSmem<DP, SPLIT, TWO>;
+    constexpr int NST = SM::stages;
+    constexpr int LA = TWO ? 1 : 2;              // key tiles ahead of the value tile
+    constexpr int BR = TWO ? 2 * kTile : kTile;  // rows of a block's row tile
+    constexpr int CH = DP / 8;                   // 16-byte chunks of a row
+    extern __shared__ uint8_t tc_smem_raw[];
+    __shared__ __align__(8) uint64_t full_bar[NST], empty_bar[NST], qfull_bar, qempty_bar, s_bar[2], p_bar[2], ofin_bar, join_bar,
+        done_bar;
+    __shared__ uint32_t tmem_s;
+    __shared__ volatile int failed_s;
+    __shared__ float qscale_s[2][kTile];   // SPLIT: what the scores are multiplied by
+    __shared__ float2 join_s[2][kTile];    // !TWO: (m, l) of both streams
+    __shared__ long long sums_s[kTcThreads / 32];
+    __shared__ long long before_s;
+    __shared__ int entry_s;
+    uint8_t* q_smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* ring = q_smem + SM::q_tiles * SM::tile;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < NST; ++i) {
+            mbar_init(&full_bar[i], kLoadWarps * 32);
+            mbar_init(&empty_bar[i], 1);
+        }
+        mbar_init(&qfull_bar, kLoadWarps * 32);
+        mbar_init(&qempty_bar, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_bar[i], 1);
+            mbar_init(&p_bar[i], kTile);
+        }
+        mbar_init(&ofin_bar, 1);
+        mbar_init(&join_bar, 2 * kTile);
+        mbar_init(&done_bar, 1);
+        failed_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pdl_wait();
+
+    // this CTA's share of the line
+    const int chunk = (entries + kTcThreads - 1) / kTcThreads;
+    const int e0 = min(entries, tid * chunk), e1 = min(entries, e0 + chunk);
+    long long mine = 0;
+    for (int e = e0; e < e1; ++e) mine += tiles_of_block(a, block_of(a, e), BR);
+    long long scan = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += v;
+    }
+    if (lane == 31) sums_s[warp] = scan;
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_s;
+    long long total = 0, before = scan - mine;
+#pragma unroll
+    for (int w = 0; w < kTcThreads / 32; ++w) {
+        if (w < warp) before += sums_s[w];
+        total += sums_s[w];
+    }
+    total *= a.Hkv;
+    pdl_trigger();
+    const int cta = blockIdx.x, ctas = sharers(total, line_ctas);
+    const long long u0 = cta < ctas ? share_begin(total, ctas, cta) : 0, u1 = cta < ctas ? share_begin(total, ctas, cta + 1) : 0;
+    if (u0 < u1 && before * a.Hkv <= u0 && u0 < (before + mine) * a.Hkv) {
+        int e = e0;
+        for (; e < e1; ++e) {
+            const int n = tiles_of_block(a, block_of(a, e), BR);
+            if (u0 < (before + n) * a.Hkv) break;
+            before += n;
+        }
+        entry_s = e;
+        before_s = before;
+    }
+    __syncthreads();
+
+    Piece pc;
+    if (u0 < u1) {
+        pc.e = entry_s;
+        pc.entries = entries;
+        pc.k = block_of(a, pc.e);
+        const long long per = tiles_of_block(a, pc.k, BR), off = u0 - before_s * a.Hkv;
+        pc.kvh = (int)(off / per);
+        int at = (int)(off - pc.kvh * per);
+        pc.tiles = tiles_of(a, pc.k, 0, BR);
+        while (at >= pc.tiles) {
+            at -= pc.tiles;
+            pc.tiles = tiles_of(a, pc.k, ++pc.rt, BR);
+        }
+        pc.tile = at;
+        pc.u = u0;
+        pc.n = (int)min((long long)(pc.tiles - at), u1 - u0);
+    }
+    auto give_up = [&]() {
+        *a.err = kErrAttnWait;
+        failed_s = 1;
+    };
+
+    if (warp > kMmaWarp) {
+        // --- producers: queries, then key and value tiles in the order of their use
+        const int ptid = tid - 32 * (kMmaWarp + 1), pw = ptid >> 5;
+        int it = 0, told = 0;  // tiles requested, tiles announced
+        bool ok = true;
+        auto announce = [&](int upto) {  // tiles [told, upto) have landed
+            if (told < upto) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            for (; told < upto; ++told) arrive(&full_bar[told % NST]);
+        };
+        auto load_tile = [&](const Piece& p, int tile, const void* cache) {
+            const int pos = p.k.key0 + tile * kTile + pw * 32 + lane;
+            const int row = pos < p.k.key1 ? (int)page_row(a, p.k.b, pos) : -1;
+            const int st = it % NST;
+            if (it >= NST) {
+                const uint32_t par = (uint32_t)((it / NST - 1) & 1);
+                if (!mbar_test_wait(&empty_bar[st], par)) {
+                    cp_async_wait<0>();  // hand over all that is on its way before waiting for room
+                    announce(it);
+                    if (!mbar_wait_bounded(&empty_bar[st], par) || failed_s) {
+                        give_up();
+                        ok = false;
+                    }
+                }
+                // the lanes copy for each other: they go on or give up together
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    return;
+                }
+            }
+            const uint32_t dst = smem_u32(ring + (size_t)st * SM::tile);
+            constexpr int RPI = 32 / CH;
+            const int c = lane % CH;
+            const bool chunk_live = c * 8 < a.D;
+#pragma unroll
+            for (int i = 0; i < 32 / RPI; ++i) {
+                const int rr = i * RPI + lane / CH;
+                const int cr = __shfl_sync(0xffffffffu, row, rr);
+                const bool live = cr >= 0 && chunk_live;
+                const int64_t src = live ? ((int64_t)cr * a.Hkv + p.kvh) * a.D + c * 8 : 0;
+                const int r = pw * 32 + rr;
+                cp_async16_zfill(dst + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                                 static_cast<const T16*>(cache) + src, live);
+            }
+            cp_async_commit();
+            ++it;
+            if (it - told > 2) {  // two tiles stay in flight
+                cp_async_wait<2>();
+                announce(it - 2);
+            }
+        };
+        int seg = 0;
+        for (Piece p = pc; ok && p.u < u1; p.next(a, BR, u1), ++seg) {
+            if (seg > 0) {
+                // the last products of the piece before need all of its tiles
+                cp_async_wait<0>();
+                announce(it);
+                if (!mbar_wait_bounded(&qempty_bar, (uint32_t)((seg - 1) & 1)) || failed_s) {
+                    give_up();
+                    ok = false;
+                }
+            }
+            if (!__all_sync(0xffffffffu, ok)) {
+                ok = false;
+                break;
+            }
+#pragma unroll 1
+            for (int i = 0; i < (TWO ? 2 : 1); ++i) {
+                const int row = p.rt * BR + i * kTile + ptid;
+                const bool live = row < p.k.rows;
+                const TQ* q = static_cast<const TQ*>(a.q) +
+                              ((int64_t)(p.k.tok0 + row / a.G) * a.H + p.kvh * a.G + row % a.G) * a.D;
+                const uint32_t dst = smem_u32(q_smem) + (TWO ? i * SM::tile : 0) + ptid * 128;
+                float sc = 1.0f;
+                if constexpr (SPLIT) {
+                    float mx = 0.0f;
+                    if (live)
+                        for (int d = 0; d < a.D; d += 4) {
+                            const float4 v = *reinterpret_cast<const float4*>(q + d);
+                            mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+                        }
+                    sc = query_scale(mx);
+                    qscale_s[seg & 1][ptid] = a.scale * 1.4426950408889634f / sc;
+                }
+#pragma unroll 4
+                for (int c = 0; c < CH; ++c) {
+                    const uint32_t at = dst + (c >> 3) * (kTile * 128) + (((c & 7) ^ (ptid & 7)) << 4);
+                    uint4 h = make_uint4(0, 0, 0, 0), l = h;
+                    if (live && c * 8 < a.D) {
+                        if constexpr (SPLIT) {
+                            const float4 x = *reinterpret_cast<const float4*>(q + c * 8), y = *reinterpret_cast<const float4*>(q + c * 8 + 4);
+                            split_f16(x.x * sc, x.y * sc, h.x, l.x);
+                            split_f16(x.z * sc, x.w * sc, h.y, l.y);
+                            split_f16(y.x * sc, y.y * sc, h.z, l.z);
+                            split_f16(y.z * sc, y.w * sc, h.w, l.w);
+                        } else {
+                            h = *reinterpret_cast<const uint4*>(q + c * 8);
+                        }
+                    }
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(h.x), "r"(h.y), "r"(h.z), "r"(h.w) : "memory");
+                    if constexpr (SPLIT)
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + SM::tile), "r"(l.x), "r"(l.y), "r"(l.z), "r"(l.w)
+                                     : "memory");
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            arrive(&qfull_bar);
+            for (int t = 0; ok && t < min(LA, p.n); ++t) load_tile(p, p.tile + t, a.ck);
+            for (int t = 0; ok && t < p.n; ++t) {
+                load_tile(p, p.tile + t, a.cv);
+                if (ok && t + LA < p.n) load_tile(p, p.tile + t + LA, a.ck);
+            }
+        }
+        cp_async_wait<0>();  // nothing may land after the CTA has ended
+        if (ok) announce(it);
+    } else if (warp == kMmaWarp) {
+        if (lane == 0) {
+            int it = 0, np[2] = {0, 0};
+            bool ok = true;
+            const uint32_t qa = smem_u32(q_smem), ra = smem_u32(ring);
+            auto wait = [&](uint64_t* bar, uint32_t par) {
+                if (ok && (!mbar_wait_bounded(bar, par) || failed_s)) {
+                    give_up();
+                    ok = false;
+                }
+                fence_after();
+            };
+            auto acquire = [&]() {
+                wait(&full_bar[it % NST], (uint32_t)((it / NST) & 1));
+                return it++ % NST;
+            };
+            constexpr uint32_t id_qk = idesc<T16>(kTile, false), id_pv = idesc<T16>(DP, true);
+            auto scores = [&](int s, int st) {
+#pragma unroll
+                for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {
+                        const uint32_t off = (k >> 2) * (kTile * 128) + (k & 3) * 32;
+                        mma_ss(tmem + s * kTile, desc_k_major(qa + (TWO ? s : part) * SM::tile + off),
+                               desc_k_major(ra + st * SM::tile + off), id_qk, part + k > 0);
+                    }
+                commit(&s_bar[s]);
+            };
+            auto sums = [&](int s, int st, bool first) {
+                wait(&p_bar[s], (uint32_t)(np[s]++ & 1));
+                if (!ok) return;
+                const uint32_t o = tmem + 2 * kTile + s * DP, pcol = tmem + s * kTile;
+#pragma unroll
+                for (int k = 0; k < kTile / 16; ++k)
+#pragma unroll
+                    for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+                        mma_ts(o, pcol + (k >> 1) * 32 + (k & 1) * 8 + part * 16, desc_n_major(ra + st * SM::tile + k * 2048), id_pv,
+                               !(first && k + part == 0));
+            };
+            int seg = 0;
+            for (Piece p = pc; ok && p.u < u1; p.next(a, BR, u1), ++seg) {
+                wait(&qfull_bar, (uint32_t)(seg & 1));
+                for (int t = 0; ok && t < min(LA, p.n); ++t) {
+                    const int st = acquire();
+                    if (!ok) break;
+                    scores(t, st);
+                    if (TWO) scores(1, st);
+                    commit(&empty_bar[st]);
+                }
+                for (int t = 0; ok && t < p.n; ++t) {
+                    const int sv = acquire();
+                    if (TWO) {
+                        sums(0, sv, t == 0);
+                        int sk = 0;
+                        if (ok && t + 1 < p.n) {
+                            sk = acquire();
+                            if (ok) scores(0, sk);
+                        }
+                        if (ok) sums(1, sv, t == 0);
+                        if (!ok) break;
+                        commit(&empty_bar[sv]);
+                        if (t + 1 < p.n) {
+                            scores(1, sk);
+                            commit(&empty_bar[sk]);
+                        }
+                    } else {
+                        sums(t & 1, sv, t < 2);
+                        if (!ok) break;
+                        commit(&empty_bar[sv]);
+                        if (t + 2 < p.n) {
+                            const int sk = acquire();
+                            if (!ok) break;
+                            scores(t & 1, sk);
+                            commit(&empty_bar[sk]);
+                        }
+                    }
+                }
+                if (!ok) break;
+                commit(&qempty_bar);
+                commit(&ofin_bar);
+            }
+            commit(&done_bar);  // completes once every product issued above has
+        }
+        __syncwarp();
+    } else {
+        // --- softmax: stream s, row r of its tile
+        const int s = warp >> 2, r = tid & (kTile - 1);
+        const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t s_col = tmem + lane_at + s * kTile;
+        int ns = 0, seg = 0, nj = 0;
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t par) {
+            if (ok && (!mbar_wait_bounded(bar, par) || failed_s)) {
+                give_up();
+                ok = false;
+            }
+            ok = __all_sync(0xffffffffu, ok);  // the warp's tensor memory accesses are collective
+            fence_after();
+        };
+        for (Piece p = pc; ok && p.u < u1; p.next(a, BR, u1), ++seg) {
+            const int row = p.rt * BR + (TWO ? s * kTile : 0) + r;  // of the block
+            const bool live = row < p.k.rows;
+            const int tok = p.k.tok0 + row / a.G;
+            int limit = 0;
+            if (live) {
+                if (p.k.kind) {
+                    limit = min(p.k.len, p.k.len - p.k.nq + row / a.G + 1);
+                } else {
+                    const int b = a.qstarts ? span_of(a.qstarts, a.B, tok) : tok;
+                    if (b >= 0) {
+                        const SeqInfo si = seq_info(a, b);
+                        limit = min(p.k.key1, min(si.len, si.len - si.nq + (tok - si.q0) + 1));
+                    }
+                }
+            }
+            wait(&qfull_bar, (uint32_t)(seg & 1));
+            if (!ok) break;
+            const float cs = SPLIT ? qscale_s[seg & 1][r] : a.scale * 1.4426950408889634f;
+            float m = -INFINITY, l = 0.0f;
+            for (int t = TWO ? 0 : s; t < p.n; t += TWO ? 1 : 2) {
+                wait(&s_bar[s], (uint32_t)(ns++ & 1));
+                if (!ok) break;
+                const int key = p.k.key0 + (p.tile + t) * kTile;
+                const int seen = limit - key;  // columns [0, seen) are visible
+                const bool whole = __all_sync(0xffffffffu, seen >= kTile);
+                float mx = m;
+                float v[32];
+#pragma unroll
+                for (int c = 0; c < kTile / 32; ++c) {
+                    tmem_ld32(s_col + c * 32, v);
+                    tmem_wait_ld();
+                    if (whole) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, v[i] * cs);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, c * 32 + i < seen ? v[i] * cs : -INFINITY);
+                    }
+                }
+                const bool move = m != -INFINITY && mx > m + kRescale;
+                if (t >= (TWO ? 1 : 2) && __any_sync(0xffffffffu, move)) {
+                    const float keep = move ? exp2_fast(m - mx) : 1.0f;
+                    l *= keep;
+#pragma unroll
+                    for (int c = 0; c < DP / 32; ++c) {
+                        const uint32_t o_at = tmem + lane_at + 2 * kTile + s * DP + c * 32;
+                        tmem_ld32(o_at, v);
+                        tmem_wait_ld();
+                        uint32_t w[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i] * keep);
+                        tmem_st32(o_at, w);
+                    }
+                }
+                if (move || m == -INFINITY) m = mx;
+                const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                for (int c = 0; c < kTile / 32; ++c) {
+                    tmem_ld32(s_col + c * 32, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        v[i] = exp2_fast(fmaf(v[i], cs, -ref));
+                        if (!whole && c * 32 + i >= seen) v[i] = 0.0f;
+                        l += v[i];
+                    }
+                    if constexpr (SPLIT) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) split_f16(v[2 * i], v[2 * i + 1], w[i], w[16 + i]);
+                        tmem_st32(s_col + c * 32, w);
+                    } else {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) w[i] = Half2Of<T16>::pack(v[2 * i], v[2 * i + 1]);
+                        tmem_st16(s_col + c * 32, w);
+                    }
+                }
+                tmem_wait_st();
+                fence_before();
+                arrive(&p_bar[s]);
+            }
+            if (!ok) break;
+            wait(&ofin_bar, (uint32_t)(seg & 1));
+            if (!ok) break;
+            // --- results of the piece
+            float w0 = 1.0f, w1 = 0.0f, M = m, L = l;
+            if (!TWO) {
+                join_s[s][r] = make_float2(m, l);
+                arrive(&join_bar);
+                wait(&join_bar, (uint32_t)(nj++ & 1));
+                if (!ok) break;
+                const float2 x = join_s[0][r], y = join_s[1][r];
+                M = fmaxf(x.x, y.x);
+                w0 = x.x == -INFINITY ? 0.0f : exp2_fast(x.x - M);
+                w1 = y.x == -INFINITY ? 0.0f : exp2_fast(y.x - M);
+                L = x.y * w0 + y.y * w1;
+            }
+            const PartArgs& part = p.k.kind ? rest : prefix;
+            const long long first = p.u - p.tile;
+            const int c0 = share_of(total, ctas, first), c1 = share_of(total, ctas, first + p.tiles - 1);
+            const bool done = c0 == c1 && p.k.kind && p.k.key0 == 0;  // no other part anywhere
+            const int64_t orow = (int64_t)tok * a.H + p.kvh * a.G + row % a.G;
+            const int slot_row = (TWO ? s * kTile : 0) + r;
+            const int64_t slot = (int64_t)cta * part.slot_rows + slot_row;
+            float* dst = c0 == cta ? part.head + (part.by_row ? orow : slot) * a.D : part.tail + slot * a.D;
+            TQ* fin = static_cast<TQ*>(a.out) + orow * a.D;
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            // one row tile: each stream's threads write half of the columns
+            constexpr int CW = TWO ? DP : DP / 2;
+            const bool both = !TWO && p.n > 1;  // the second stream had a tile
+#pragma unroll 1
+            for (int c = 0; c < CW; c += 32) {
+                const int col = (TWO ? 0 : s * CW) + c;
+                float v[32];
+                __syncwarp();  // the loads below are the whole warp's
+                tmem_ld32(tmem + lane_at + 2 * kTile + (TWO ? s * DP : 0) + col, v);
+                tmem_wait_ld();
+                if (!TWO) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] *= w0;
+                    if (both) {
+                        float y[32];
+                        tmem_ld32(tmem + lane_at + 2 * kTile + DP + col, y);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = fmaf(y[i], w1, v[i]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    if (!live || col + i >= a.D) break;
+                    if (!done) {
+                        *reinterpret_cast<float4*>(dst + col + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                        *reinterpret_cast<float4*>(dst + col + i + 4) = make_float4(v[i + 4], v[i + 5], v[i + 6], v[i + 7]);
+                    } else if constexpr (sizeof(TQ) == 4) {
+                        *reinterpret_cast<float4*>(fin + col + i) = make_float4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
+                        *reinterpret_cast<float4*>(fin + col + i + 4) =
+                            make_float4(v[i + 4] * inv, v[i + 5] * inv, v[i + 6] * inv, v[i + 7] * inv);
+                    } else {
+                        *reinterpret_cast<uint4*>(fin + col + i) =
+                            make_uint4(Half2Of<T16>::pack(v[i] * inv, v[i + 1] * inv), Half2Of<T16>::pack(v[i + 2] * inv, v[i + 3] * inv),
+                                       Half2Of<T16>::pack(v[i + 4] * inv, v[i + 5] * inv), Half2Of<T16>::pack(v[i + 6] * inv, v[i + 7] * inv));
+                    }
+                }
+            }
+            if (live && (TWO || s == 0)) {
+                if (c0 == cta) part.stat[orow] = make_float4(M, L, __int_as_float(c0), __int_as_float(c1));
+                else part.tail_stat[slot] = make_float2(M, L);
+            }
+            if (!TWO) {
+                // the next piece's products overwrite sums that the other threads read
+                fence_before();
+                arrive(&join_bar);
+                wait(&join_bar, (uint32_t)(nj++ & 1));
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        mbar_drain(&done_bar, 0);  // products still running use the memory that is freed here
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    }
+    pdl_wait();
+}
+
+template <typename TQ, typename T16, int DP, bool SPLIT, bool TWO>
+void launch_tc_t(const PagedTcPlan& plan, const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, cudaStream_t s, bool pdl) {
+    auto kern = paged_tc_kernel<TQ, T16, DP, SPLIT, TWO>;
+    allow_max_dynamic_smem(kern);
+    const int entries = a.groups + (plan.rest ? a.B : 0);
+    launch_kernel(kern, dim3((unsigned)plan.ctas), dim3(kTcThreads), TcSmem<DP, SPLIT, TWO>::bytes, s, pdl, a, prefix, rest, entries,
+                  plan.ctas);
+}
+
+template <int DP>
+void launch_tc_d(const PagedTcPlan& plan, const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, int32_t tq, int32_t tk,
+                 cudaStream_t s, bool pdl) {
+    using H = __half;
+    using B = __nv_bfloat16;
+    if (tq == BEACON_CUDA_DTYPE_F32) launch_tc_t<float, H, DP, true, false>(plan, a, prefix, rest, s, pdl);
+    else if (tk == BEACON_CUDA_DTYPE_F16 && plan.two) launch_tc_t<H, H, DP, false, true>(plan, a, prefix, rest, s, pdl);
+    else if (tk == BEACON_CUDA_DTYPE_F16) launch_tc_t<H, H, DP, false, false>(plan, a, prefix, rest, s, pdl);
+    else if (plan.two) launch_tc_t<B, B, DP, false, true>(plan, a, prefix, rest, s, pdl);
+    else launch_tc_t<B, B, DP, false, false>(plan, a, prefix, rest, s, pdl);
+}
+
+}  // namespace
+
+PagedTcPlan plan_paged_tc(const BeaconCudaContext* ctx, const PagedArgs& a, bool split, bool with_rest) {
+    PagedTcPlan p;
+    // blocks of more than 128 rows on average share each key tile between two row tiles
+    p.two = !split && (int64_t)a.T * a.G > 128LL * (a.groups ? a.groups : a.B);
+    p.rest = with_rest;
+    p.slot_rows = p.two ? 2 * kTile : kTile;
+    p.ctas = ctx->sm_count;
+    return p;
+}
+
+void launch_paged_tc(const PagedTcPlan& plan, const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, int32_t tq,
+                     int32_t tk, cudaStream_t s, bool pdl) {
+    if (a.D <= 64) launch_tc_d<64>(plan, a, prefix, rest, tq, tk, s, pdl);
+    else launch_tc_d<128>(plan, a, prefix, rest, tq, tk, s, pdl);
+}
+
+}  // namespace bc

@@ -79,20 +79,20 @@ def attention(q, ck, cv, table, lens, scale, starts=None, group_starts=None, pre
                 if group_starts[k] <= b < group_starts[k + 1]:
                     prefix, first = int(prefix_lens[k]), int(group_starts[k])
         rows = [(table[first if p < prefix else b][p // ps], p % ps) for p in range(int(lens[b]))]
-        K = np.array([ck[r] for r in rows], dtype=np.float64).reshape(-1, Hkv, D)
-        V = np.array([cv[r] for r in rows], dtype=np.float64).reshape(-1, Hkv, D)
+        at = np.array(rows, dtype=np.int64).reshape(-1, 2)
+        K, V = ck[at[:, 0], at[:, 1]], cv[at[:, 0], at[:, 1]]
         for j in range(n):
             t = starts[b] + j
             see = max(0, int(lens[b]) - n + j + 1)
             out[t] = 0.0
             if see == 0:
                 continue
-            for h in range(H):
-                k, v = K[:see, h // g], V[:see, h // g]
-                s = k @ q[t, h].astype(np.float64) * scale
-                p = np.exp(s - s.max())
-                out[t, h] = (p / p.sum()) @ v
-                info[t, 0] = max(info[t, 0], (np.abs(k) @ np.abs(q[t, h].astype(np.float64))).max() * abs(scale))
+            for h in range(Hkv):
+                k, v, x = K[:see, h], V[:see, h], q[t, h * g:(h + 1) * g]
+                s = x @ k.T * scale
+                p = np.exp(s - s.max(-1, keepdims=True))
+                out[t, h * g:(h + 1) * g] = (p / p.sum(-1, keepdims=True)) @ v
+                info[t, 0] = max(info[t, 0], (np.abs(x) @ np.abs(k).T).max() * abs(scale))
             info[t, 1], info[t, 2] = see, np.abs(V[:see]).max()
     return out, info
 

@@ -343,6 +343,25 @@ def test_attention_many_rows(be, s, dtype, cache, H, Hkv, D, ps, lens, new, grou
 
 
 @pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("B,H,Hkv,D,ps,most,new,shared", [
+    (150, 8, 8, 64, 16, 200, 3, False),     # far more row blocks than multiprocessors
+    (40, 16, 8, 128, 32, 700, 40, True),    # more than one row tile a block, several blocks a CTA
+    (330, 4, 2, 64, 16, 300, 1, True),      # one row each, in groups of eleven
+])
+def test_attention_many_blocks(be, s, dtype, cache, B, H, Hkv, D, ps, most, new, shared):
+    rng = np.random.default_rng(B + H)
+    per = 11 if new == 1 else 20
+    prefix = 130 if shared else 0
+    lens = [int(prefix + max(n, rng.integers(1, most))) for n in [new] * B]
+    news = [int(rng.integers(1, new + 1)) for _ in range(B)]
+    groups, pre = (list(range(0, B + 1, per)), [prefix] * (B // per)) if shared else (None, None)
+    ck, cv, table = make_cache(be, rng, -(-max(lens) // ps), lens, ps, Hkv, D, cache, groups, pre)
+    starts = None if new == 1 else np.concatenate([[0], np.cumsum(news)])
+    q = Dev(be, rng.standard_normal((B if new == 1 else starts[-1], H, D)) * 2, dtype)
+    check_attention(be, s, rng, q, ck, cv, table, lens, dtype, cache, starts, groups, pre)
+
+
+@pytest.mark.parametrize("dtype,cache", PAIRS)
 def test_attention_extreme_scores(be, s, dtype, cache):
     """Scores of several thousand (one key takes the whole weight), large
     32-bit queries outside the 16-bit range, and equal scores."""
