@@ -161,19 +161,21 @@ PartArgs carve_part(Carve& c, const PagedArgs& a, int ctas, int slot_rows, bool 
     return p;
 }
 
-void run_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream, const PagedArgs& a, int32_t tq, int32_t tk) {
+void run_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream, PagedArgs a, int32_t tq, int32_t tk) {
     const int32_t F32 = BEACON_CUDA_DTYPE_F32, F16 = BEACON_CUDA_DTYPE_F16;
     if (tk != F32 && a.D <= 128) {
         // single rows of few heads: paged_decode_kernel; prefixes, several rows
         // of a sequence or many heads: the tensor-core kernel, whose row block is 128
         const bool decode = !a.qstarts && a.G <= kDecodeMaxGroup, tc = a.gstarts || !decode;
-        const bool split = tq == F32, by_row = a.gstarts != nullptr;
+        const bool split = tq == F32;
+        a.merged = a.qstarts && (int64_t)a.T * a.G >= 128LL * a.B;
+        const bool by_row = a.gstarts && !a.merged;
         const PagedTcPlan plan = tc ? plan_paged_tc(ctx, a, split, !decode) : PagedTcPlan{};
         const int dctas = decode ? paged_decode_ctas(ctx, a, split) : 0;
         PartArgs prefix, rest;
         auto carve = [&](uint8_t* base) {
             Carve c(base);
-            if (tc && a.gstarts) prefix = carve_part(c, a, plan.ctas, plan.slot_rows, by_row);
+            if (tc && by_row) prefix = carve_part(c, a, plan.ctas, plan.slot_rows, by_row);
             rest = decode ? carve_part(c, a, dctas, a.G, by_row) : carve_part(c, a, plan.ctas, plan.slot_rows, by_row);
             return c.used();
         };

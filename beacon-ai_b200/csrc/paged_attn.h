@@ -20,6 +20,9 @@ struct PagedArgs {
     int64_t pages = 0;
     int T = 0, B = 0, H = 0, Hkv = 0, G = 0, D = 0, groups = 0;  // G = H / Hkv
     int max_pages = 0, page_size = 0;
+    // 1: a sequence's queries take its prefix and its own keys together (they
+    // fill row blocks by themselves); 0: prefixes are done for whole groups
+    int merged = 0;
     float scale = 0.0f;
     int* err = nullptr;
 };

@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedArgs a, c
     if (b < 0) return;
     const SeqInfo s = seq_info(a, b);
     const int limit = min(s.len, s.len - s.nq + (t - s.q0) + 1);
-    const bool on[2] = {min(s.prefix, limit) > 0, limit > s.prefix};
+    const bool on[2] = {!a.merged && min(s.prefix, limit) > 0, limit > (a.merged ? 0 : s.prefix)};
     float M = -INFINITY, L = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const bool live = lane * 4 < a.D;

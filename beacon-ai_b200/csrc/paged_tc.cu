@@ -15,9 +15,9 @@
 //    and are joined at the end. 32-bit queries come as two f16 parts (SPLIT):
 //    two products for the scores, and two for the sums, whose weights are
 //    split likewise.
-// P replaces S in place, 32 keys at a time: the 16 columns of packed weights
-// (then 16 of their remainders) lie where the 32 scores were, and are the A
-// operand of O += P V from tensor memory; V is read N-major.
+// P replaces S: the packed weights (64 columns, then 64 of their remainders)
+// lie where the scores were, and are the A operand of O += P V from tensor
+// memory; V is read N-major.
 // Four producer warps copy key and value rows, page by page, with 16-byte
 // asynchronous copies into a ring of tiles in the 128-byte swizzle; one thread
 // issues the products. The key tiles of all blocks form one line that the CTAs
@@ -40,9 +40,11 @@ namespace {
 
 constexpr int kTile = 128;              // rows of a row tile, keys of a key tile
 constexpr int kSoftWarps = 8;
-constexpr int kMmaWarp = kSoftWarps;
-constexpr int kLoadWarps = 4;
-constexpr int kTcThreads = 32 * (kSoftWarps + 1 + kLoadWarps);
+constexpr int kLoadWarp = 8, kLoadWarps = 4;
+constexpr int kMmaWarp = 12;            // with three idle warps: registers move by groups of four warps
+constexpr int kTcThreads = 512;
+// registers: 128 a thread at launch; 2 x 184 + 80 + 64 = 4 x 128
+constexpr int kSoftRegs = 184, kLoadRegs = 80, kMmaRegs = 64;
 constexpr uint32_t kTmemCols = 512;     // S 2 x 128, O 2 x DP
 constexpr float kRescale = 8.0f;        // log2 of the largest weight
 
@@ -51,7 +53,8 @@ struct TcSmem {
     static constexpr int tile = kTile * DP * 2;
     static constexpr int q_tiles = TWO || SPLIT ? 2 : 1;
     static constexpr int stages = DP == 128 ? 6 - q_tiles : 8;
-    static constexpr size_t bytes = (size_t)(q_tiles + stages) * tile + 1024;
+    static constexpr int stage_out = 32 * 64;  // per softmax warp: 64 bytes of each of its rows
+    static constexpr size_t bytes = (size_t)(q_tiles + stages) * tile + kSoftWarps * stage_out + 1024;
 };
 
 __device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {  // 8-row atoms of 1024 bytes
@@ -110,7 +113,15 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
         "r"(r[31])
         : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const float (&v)[16]) {
+    const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(addr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
@@ -119,18 +130,41 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two 32-bit operations in one instruction.
+__device__ __forceinline__ unsigned long long as_u64(float2 v) { return *reinterpret_cast<unsigned long long*>(&v); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(as_u64(a)), "l"(as_u64(b)), "l"(as_u64(c)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(as_u64(a)), "l"(as_u64(b)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ void st_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
 // The rows that share keys: a group's queries against its prefix (kind 0), or a
 // sequence's queries against its own keys (kind 1).
 struct Block {
     int kind = 0;
     int b = 0;                   // page table row
+    int cut = 0, first = 0;      // keys below cut are read through table row `first`
     int key0 = 0, key1 = 0;      // keys [key0, key1)
     int tok0 = 0, rows = 0;      // query rows tok0 * G ..
     int nq = 0, len = 0;         // kind 1: causal limits
 };
 __device__ __forceinline__ Block block_of(const PagedArgs& a, int e) {
     Block k;
-    if (e < a.groups) {
+    const int groups = a.merged ? 0 : a.groups;
+    if (e < groups) {
         const int lo = start_at(a.gstarts, e, a.B, a.err), hi = start_at(a.gstarts, e + 1, a.B, a.err);
         if (hi < lo) *a.err = kErrIndex;
         if (hi <= lo) return k;
@@ -141,10 +175,15 @@ __device__ __forceinline__ Block block_of(const PagedArgs& a, int e) {
         k.rows = max(0, tok1 - k.tok0) * a.G;
         return k;
     }
-    const SeqInfo s = seq_info(a, e - a.groups);
+    const SeqInfo s = seq_info(a, e - groups);
     k.kind = 1;
-    k.b = e - a.groups;
-    k.key0 = s.prefix;
+    k.b = e - groups;
+    if (a.merged) {
+        k.cut = s.prefix;
+        k.first = s.first;
+    } else {
+        k.key0 = s.prefix;
+    }
     k.key1 = s.len;
     k.tok0 = s.q0;
     k.rows = s.nq * a.G;
@@ -305,18 +344,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         failed_s = 1;
     };
 
-    if (warp > kMmaWarp) {
+    if (warp >= kLoadWarp && warp < kLoadWarp + kLoadWarps) {
         // --- producers: queries, then key and value tiles in the order of their use
-        const int ptid = tid - 32 * (kMmaWarp + 1), pw = ptid >> 5;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
+        const int pw = warp - kLoadWarp;
+        const int64_t stride = (int64_t)a.Hkv * a.D * 2;  // bytes from one cache row to the next
+        const int c = lane % CH;                          // this lane's chunk of the rows it copies
+        const bool chunk_live = c * 8 < a.D;
         int it = 0, told = 0;  // tiles requested, tiles announced
         bool ok = true;
         auto announce = [&](int upto) {  // tiles [told, upto) have landed
             if (told < upto) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             for (; told < upto; ++told) arrive(&full_bar[told % NST]);
         };
+        constexpr int RPI = 32 / CH;  // rows that one copy instruction of a warp covers
         auto load_tile = [&](const Piece& p, int tile, const void* cache) {
             const int pos = p.k.key0 + tile * kTile + pw * 32 + lane;
-            const int row = pos < p.k.key1 ? (int)page_row(a, p.k.b, pos) : -1;
+            const int row = pos < p.k.key1 ? (int)page_row(a, pos < p.k.cut ? p.k.first : p.k.b, pos) : -1;
             const int st = it % NST;
             if (it >= NST) {
                 const uint32_t par = (uint32_t)((it / NST - 1) & 1);
@@ -329,24 +373,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
                 // the lanes copy for each other: they go on or give up together
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    return;
-                }
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
             }
-            const uint32_t dst = smem_u32(ring + (size_t)st * SM::tile);
-            constexpr int RPI = 32 / CH;
-            const int c = lane % CH;
-            const bool chunk_live = c * 8 < a.D;
-#pragma unroll
+            const uint32_t dst = smem_u32(ring + (size_t)st * SM::tile) + (c >> 3) * (kTile * 128);
+            const uint8_t* src = static_cast<const uint8_t*>(cache) + (p.kvh * a.D + c * 8) * 2;
+#pragma unroll 8
             for (int i = 0; i < 32 / RPI; ++i) {
                 const int rr = i * RPI + lane / CH;
                 const int cr = __shfl_sync(0xffffffffu, row, rr);
                 const bool live = cr >= 0 && chunk_live;
-                const int64_t src = live ? ((int64_t)cr * a.Hkv + p.kvh) * a.D + c * 8 : 0;
                 const int r = pw * 32 + rr;
-                cp_async16_zfill(dst + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4),
-                                 static_cast<const T16*>(cache) + src, live);
+                cp_async16_zfill(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), live ? src + cr * stride : static_cast<const uint8_t*>(cache), live);
             }
             cp_async_commit();
             ++it;
@@ -365,49 +403,60 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     give_up();
                     ok = false;
                 }
-            }
-            if (!__all_sync(0xffffffffu, ok)) {
-                ok = false;
-                break;
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
             }
 #pragma unroll 1
             for (int i = 0; i < (TWO ? 2 : 1); ++i) {
-                const int row = p.rt * BR + i * kTile + ptid;
-                const bool live = row < p.k.rows;
-                const TQ* q = static_cast<const TQ*>(a.q) +
-                              ((int64_t)(p.k.tok0 + row / a.G) * a.H + p.kvh * a.G + row % a.G) * a.D;
-                const uint32_t dst = smem_u32(q_smem) + (TWO ? i * SM::tile : 0) + ptid * 128;
-                float sc = 1.0f;
+                // this lane's query row, as a row of [T * H][D]; -1: behind the block
+                const int br = p.rt * BR + i * kTile + pw * 32 + lane;
+                const int qrow = br < p.k.rows ? (p.k.tok0 + br / a.G) * a.H + p.kvh * a.G + br % a.G : -1;
+                const uint32_t dst = smem_u32(q_smem) + (TWO ? i * SM::tile : 0);
                 if constexpr (SPLIT) {
-                    float mx = 0.0f;
-                    if (live)
-                        for (int d = 0; d < a.D; d += 4) {
-                            const float4 v = *reinterpret_cast<const float4*>(q + d);
-                            mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+                    // a warp takes a row at a time, eight on their way: each lane four values
+#pragma unroll 1
+                    for (int r0 = 0; r0 < 32; r0 += 8) {
+                        float4 x[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const int qr = __shfl_sync(0xffffffffu, qrow, r0 + k);
+                            x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (qr >= 0 && lane * 4 < a.D)
+                                x[k] = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (int64_t)qr * a.D + lane * 4);
                         }
-                    sc = query_scale(mx);
-                    qscale_s[seg & 1][ptid] = a.scale * 1.4426950408889634f / sc;
-                }
-#pragma unroll 4
-                for (int c = 0; c < CH; ++c) {
-                    const uint32_t at = dst + (c >> 3) * (kTile * 128) + (((c & 7) ^ (ptid & 7)) << 4);
-                    uint4 h = make_uint4(0, 0, 0, 0), l = h;
-                    if (live && c * 8 < a.D) {
-                        if constexpr (SPLIT) {
-                            const float4 x = *reinterpret_cast<const float4*>(q + c * 8), y = *reinterpret_cast<const float4*>(q + c * 8 + 4);
-                            split_f16(x.x * sc, x.y * sc, h.x, l.x);
-                            split_f16(x.z * sc, x.w * sc, h.y, l.y);
-                            split_f16(y.x * sc, y.y * sc, h.z, l.z);
-                            split_f16(y.z * sc, y.w * sc, h.w, l.w);
-                        } else {
-                            h = *reinterpret_cast<const uint4*>(q + c * 8);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const int r = pw * 32 + r0 + k;
+                            float mx = fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w)));
+                            mx = warp_max(mx);
+                            const float sc = query_scale(mx);
+                            if (lane == 0) qscale_s[seg & 1][r] = fabsf(a.scale) * 1.4426950408889634f / sc;
+                            if (lane * 4 < DP) {
+                                uint2 h, l;
+                                split_f16(x[k].x * sc, x[k].y * sc, h.x, l.x);
+                                split_f16(x[k].z * sc, x[k].w * sc, h.y, l.y);
+                                const int cc = lane >> 1;
+                                const uint32_t at = dst + (cc >> 3) * (kTile * 128) + r * 128 + (((cc & 7) ^ (r & 7)) << 4) + (lane & 1) * 8;
+                                asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(at), "r"(h.x), "r"(h.y) : "memory");
+                                asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(at + SM::tile), "r"(l.x), "r"(l.y) : "memory");
+                            }
                         }
                     }
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(h.x), "r"(h.y), "r"(h.z), "r"(h.w) : "memory");
-                    if constexpr (SPLIT)
-                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + SM::tile), "r"(l.x), "r"(l.y), "r"(l.z), "r"(l.w)
-                                     : "memory");
+                } else {
+#pragma unroll 8
+                    for (int k = 0; k < 32 / RPI; ++k) {
+                        const int rr = k * RPI + lane / CH;
+                        const int qr = __shfl_sync(0xffffffffu, qrow, rr);
+                        const bool live = qr >= 0 && chunk_live;
+                        const int r = pw * 32 + rr;
+                        cp_async16_zfill(dst + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                                         static_cast<const TQ*>(a.q) + (live ? (int64_t)qr * a.D + c * 8 : 0), live);
+                    }
                 }
+            }
+            if (!SPLIT) {
+                cp_async_commit();
+                cp_async_wait<0>();
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             arrive(&qfull_bar);
@@ -419,8 +468,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         cp_async_wait<0>();  // nothing may land after the CTA has ended
         if (ok) announce(it);
-    } else if (warp == kMmaWarp) {
-        if (lane == 0) {
+    } else if (warp >= kMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+        if (warp == kMmaWarp && lane == 0) {
             int it = 0, np[2] = {0, 0};
             bool ok = true;
             const uint32_t qa = smem_u32(q_smem), ra = smem_u32(ring);
@@ -455,7 +505,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int k = 0; k < kTile / 16; ++k)
 #pragma unroll
                     for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
-                        mma_ts(o, pcol + (k >> 1) * 32 + (k & 1) * 8 + part * 16, desc_n_major(ra + st * SM::tile + k * 2048), id_pv,
+                        mma_ts(o, pcol + part * 64 + k * 8, desc_n_major(ra + st * SM::tile + k * 2048), id_pv,
                                !(first && k + part == 0));
             };
             int seg = 0;
@@ -505,6 +555,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         __syncwarp();
     } else {
         // --- softmax: stream s, row r of its tile
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         const int s = warp >> 2, r = tid & (kTile - 1);
         const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_col = tmem + lane_at + s * kTile;
@@ -536,7 +587,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             wait(&qfull_bar, (uint32_t)(seg & 1));
             if (!ok) break;
-            const float cs = SPLIT ? qscale_s[seg & 1][r] : a.scale * 1.4426950408889634f;
+            const float cs = SPLIT ? qscale_s[seg & 1][r] : fabsf(a.scale) * 1.4426950408889634f;
             float m = -INFINITY, l = 0.0f;
             for (int t = TWO ? 0 : s; t < p.n; t += TWO ? 1 : 2) {
                 wait(&s_bar[s], (uint32_t)(ns++ & 1));
@@ -544,59 +595,68 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const int key = p.k.key0 + (p.tile + t) * kTile;
                 const int seen = limit - key;  // columns [0, seen) are visible
                 const bool whole = __all_sync(0xffffffffu, seen >= kTile);
-                float mx = m;
-                float v[32];
+                float v[kTile];
 #pragma unroll
-                for (int c = 0; c < kTile / 32; ++c) {
-                    tmem_ld32(s_col + c * 32, v);
-                    tmem_wait_ld();
-                    if (whole) {
+                for (int c = 0; c < kTile; c += 32) tmem_ld32(s_col + c, *reinterpret_cast<float(*)[32]>(v + c));
+                tmem_wait_ld();
+                if (a.scale < 0.0f) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, v[i] * cs);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, c * 32 + i < seen ? v[i] * cs : -INFINITY);
-                    }
+                    for (int i = 0; i < kTile; ++i) v[i] = -v[i];
                 }
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < kTile; ++i)
+                        if (i >= seen) v[i] = -INFINITY;
+                }
+                float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+                for (int i = 4; i < kTile; i += 4)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], v[i + j]);
+                top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                const float mx = top[0] == -INFINITY ? m : fmaxf(m, top[0] * cs);
                 const bool move = m != -INFINITY && mx > m + kRescale;
                 if (t >= (TWO ? 1 : 2) && __any_sync(0xffffffffu, move)) {
                     const float keep = move ? exp2_fast(m - mx) : 1.0f;
                     l *= keep;
-#pragma unroll
-                    for (int c = 0; c < DP / 32; ++c) {
-                        const uint32_t o_at = tmem + lane_at + 2 * kTile + s * DP + c * 32;
-                        tmem_ld32(o_at, v);
+#pragma unroll 1
+                    for (int c = 0; c < DP; c += 16) {
+                        float w[16];
+                        const uint32_t o_at = tmem + lane_at + 2 * kTile + s * DP + c;
+                        tmem_ld16(o_at, w);
                         tmem_wait_ld();
-                        uint32_t w[32];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i] * keep);
-                        tmem_st32(o_at, w);
+                        for (int i = 0; i < 16; ++i) w[i] *= keep;
+                        tmem_st16(o_at, w);
                     }
                 }
                 if (move || m == -INFINITY) m = mx;
                 const float ref = m == -INFINITY ? 0.0f : m;
+                const float2 cs2 = make_float2(cs, cs), ref2 = make_float2(-ref, -ref);
+                float2 sum[2] = {make_float2(l, 0.0f), make_float2(0.0f, 0.0f)};
+                // the weights, 64 at a time so that the matrix unit's columns are written early
 #pragma unroll
-                for (int c = 0; c < kTile / 32; ++c) {
-                    tmem_ld32(s_col + c * 32, v);
-                    tmem_wait_ld();
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t w[32], w2[SPLIT ? 32 : 1];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        v[i] = exp2_fast(fmaf(v[i], cs, -ref));
-                        if (!whole && c * 32 + i >= seen) v[i] = 0.0f;
-                        l += v[i];
+                        const int k = h * 64 + 2 * i;
+                        float2 x = fma2(make_float2(v[k], v[k + 1]), cs2, ref2);
+                        x.x = exp2_fast(x.x);
+                        x.y = exp2_fast(x.y);
+                        if (!whole) {  // also where a zero scale times the mask is no number
+                            if (k >= seen) x.x = 0.0f;
+                            if (k + 1 >= seen) x.y = 0.0f;
+                        }
+                        sum[i & 1] = add2(sum[i & 1], x);
+                        if constexpr (SPLIT) split_f16(x.x, x.y, w[i], w2[i]);
+                        else w[i] = Half2Of<T16>::pack(x.x, x.y);
                     }
-                    if constexpr (SPLIT) {
-                        uint32_t w[32];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) split_f16(v[2 * i], v[2 * i + 1], w[i], w[16 + i]);
-                        tmem_st32(s_col + c * 32, w);
-                    } else {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) w[i] = Half2Of<T16>::pack(v[2 * i], v[2 * i + 1]);
-                        tmem_st16(s_col + c * 32, w);
-                    }
+                    tmem_st32(s_col + h * 32, w);
+                    if constexpr (SPLIT) tmem_st32(s_col + 64 + h * 32, w2);
                 }
+                sum[0] = add2(sum[0], sum[1]);
+                l = sum[0].x + sum[0].y;
                 tmem_wait_st();
                 fence_before();
                 arrive(&p_bar[s]);
@@ -624,45 +684,84 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int64_t orow = (int64_t)tok * a.H + p.kvh * a.G + row % a.G;
             const int slot_row = (TWO ? s * kTile : 0) + r;
             const int64_t slot = (int64_t)cta * part.slot_rows + slot_row;
-            float* dst = c0 == cta ? part.head + (part.by_row ? orow : slot) * a.D : part.tail + slot * a.D;
-            TQ* fin = static_cast<TQ*>(a.out) + orow * a.D;
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            // Each thread has a row; through 64 bytes of each row at a time in
+            // shared memory the warp writes 8 rows by 64 bytes per instruction
+            // (a thread writing its own row touches 32 lines at once: 14,000
+            // cycles for 256 rows of 128 sums).
+            const int64_t own = !live ? -1 : (done || (c0 == cta && part.by_row) ? orow : slot) * a.D;
+            int64_t to[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[i] = __shfl_sync(0xffffffffu, own, i * 8 + lane / 4);
+            const uint32_t st = smem_u32(ring + (size_t)NST * SM::tile) + warp * SM::stage_out;
+            const uint32_t put = st + lane * 64, get = st + (lane / 4) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
             // one row tile: each stream's threads write half of the columns
             constexpr int CW = TWO ? DP : DP / 2;
             const bool both = !TWO && p.n > 1;  // the second stream had a tile
-#pragma unroll 1
-            for (int c = 0; c < CW; c += 32) {
-                const int col = (TWO ? 0 : s * CW) + c;
-                float v[32];
-                __syncwarp();  // the loads below are the whole warp's
-                tmem_ld32(tmem + lane_at + 2 * kTile + (TWO ? s * DP : 0) + col, v);
+            auto sums_of = [&](int col, float (&v)[16]) {
+                const uint32_t o_at = tmem + lane_at + 2 * kTile + col;
+                tmem_ld16(o_at + (TWO ? s * DP : 0), v);
                 tmem_wait_ld();
                 if (!TWO) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] *= w0;
+                    for (int i = 0; i < 16; ++i) v[i] *= w0;
                     if (both) {
-                        float y[32];
-                        tmem_ld32(tmem + lane_at + 2 * kTile + DP + col, y);
+                        float y[16];
+                        tmem_ld16(o_at + DP, y);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = fmaf(y[i], w1, v[i]);
+                        for (int i = 0; i < 16; ++i) v[i] = fmaf(y[i], w1, v[i]);
                     }
                 }
+                if (done) {
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    if (!live || col + i >= a.D) break;
-                    if (!done) {
-                        *reinterpret_cast<float4*>(dst + col + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                        *reinterpret_cast<float4*>(dst + col + i + 4) = make_float4(v[i + 4], v[i + 5], v[i + 6], v[i + 7]);
-                    } else if constexpr (sizeof(TQ) == 4) {
-                        *reinterpret_cast<float4*>(fin + col + i) = make_float4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
-                        *reinterpret_cast<float4*>(fin + col + i + 4) =
-                            make_float4(v[i + 4] * inv, v[i + 5] * inv, v[i + 6] * inv, v[i + 7] * inv);
-                    } else {
-                        *reinterpret_cast<uint4*>(fin + col + i) =
-                            make_uint4(Half2Of<T16>::pack(v[i] * inv, v[i + 1] * inv), Half2Of<T16>::pack(v[i + 2] * inv, v[i + 3] * inv),
-                                       Half2Of<T16>::pack(v[i + 4] * inv, v[i + 5] * inv), Half2Of<T16>::pack(v[i + 6] * inv, v[i + 7] * inv));
+                    for (int i = 0; i < 16; ++i) v[i] *= inv;
+                }
+            };
+            if (!done || sizeof(TQ) == 4) {
+                float* base = done ? static_cast<float*>(a.out) : c0 == cta ? part.head : part.tail;
+#pragma unroll 1
+                for (int c = 0; c < CW; c += 16) {
+                    const int col = (TWO ? 0 : s * CW) + c;
+                    float v[16];
+                    sums_of(col, v);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        st_shared16(put + ((i ^ ((lane >> 1) & 3)) << 4), __float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
+                                    __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+                    __syncwarp();
+                    const int d = col + (lane & 3) * 4;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint4 x = ld_shared16(get + i * 512);
+                        if (to[i] >= 0 && d < a.D) *reinterpret_cast<uint4*>(base + to[i] + d) = x;
                     }
+                    __syncwarp();
+                }
+            } else if constexpr (sizeof(TQ) == 2) {
+                TQ* base = static_cast<TQ*>(a.out);
+#pragma unroll 1
+                for (int c = 0; c < CW; c += 32) {
+                    const int col = (TWO ? 0 : s * CW) + c;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float v[16];
+                        sums_of(col + 16 * h, v);
+                        uint32_t w[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) w[i] = Half2Of<T16>::pack(v[2 * i], v[2 * i + 1]);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            st_shared16(put + (((2 * h + i) ^ ((lane >> 1) & 3)) << 4), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                    }
+                    __syncwarp();
+                    const int d = col + (lane & 3) * 8;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint4 x = ld_shared16(get + i * 512);
+                        if (to[i] >= 0 && d < a.D) *reinterpret_cast<uint4*>(base + to[i] + d) = x;
+                    }
+                    __syncwarp();
                 }
             }
             if (live && (TWO || s == 0)) {
@@ -691,7 +790,7 @@ template <typename TQ, typename T16, int DP, bool SPLIT, bool TWO>
 void launch_tc_t(const PagedTcPlan& plan, const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, cudaStream_t s, bool pdl) {
     auto kern = paged_tc_kernel<TQ, T16, DP, SPLIT, TWO>;
     allow_max_dynamic_smem(kern);
-    const int entries = a.groups + (plan.rest ? a.B : 0);
+    const int entries = (a.merged ? 0 : a.groups) + (plan.rest ? a.B : 0);
     launch_kernel(kern, dim3((unsigned)plan.ctas), dim3(kTcThreads), TcSmem<DP, SPLIT, TWO>::bytes, s, pdl, a, prefix, rest, entries,
                   plan.ctas);
 }
@@ -713,7 +812,7 @@ void launch_tc_d(const PagedTcPlan& plan, const PagedArgs& a, const PartArgs& pr
 PagedTcPlan plan_paged_tc(const BeaconCudaContext* ctx, const PagedArgs& a, bool split, bool with_rest) {
     PagedTcPlan p;
     // blocks of more than 128 rows on average share each key tile between two row tiles
-    p.two = !split && (int64_t)a.T * a.G > 128LL * (a.groups ? a.groups : a.B);
+    p.two = !split && (int64_t)a.T * a.G > 128LL * (a.groups && !a.merged ? a.groups : a.B);
     p.rest = with_rest;
     p.slot_rows = p.two ? 2 * kTile : kTile;
     p.ctas = ctx->sm_count;
