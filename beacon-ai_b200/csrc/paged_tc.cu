@@ -57,31 +57,39 @@ struct TcSmem {
     static constexpr size_t bytes = (size_t)(q_tiles + stages) * tile + kSoftWarps * stage_out + 1024;
 };
 
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {  // 8-row atoms of 1024 bytes
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-           ((uint64_t)2 << 61);
-}
-// Values: 64 dims (128 bytes) of a key in a row, blocks of 64 dims 128 rows
-// apart (leading offset), 8-key atoms 1024 bytes apart (stride offset).
-__device__ __forceinline__ uint64_t desc_n_major(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)((kTile * 128) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
+// Shared-memory descriptors, 128-byte swizzle. K-major (queries, keys): 8-row
+// atoms of 1024 bytes. N-major (values): 64 dims (128 bytes) of a key in a row,
+// blocks of 64 dims 128 rows apart (leading offset), 8-key atoms 1024 bytes
+// apart (stride offset).
+__device__ __forceinline__ uint32_t desc_lo_k(uint32_t addr) { return ((addr >> 4) & 0x3FFF) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_lo_n(uint32_t addr) { return ((addr >> 4) & 0x3FFF) | ((uint32_t)((kTile * 128) >> 4) << 16); }
+constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
 template <typename T>
 constexpr uint32_t idesc(int n, bool b_n_major) {
     const uint32_t ty = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     return (1u << 4) | (ty << 7) | (ty << 10) | ((b_n_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
            ((uint32_t)(kTile >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-                 "l"(a), "l"(b), "r"(id), "r"((uint32_t)acc)
-                 : "memory");
+// Products issued by the elected thread of a converged warp. The descriptors'
+// upper halves are constants; only the address field (lower half) moves.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 a, b;\n mov.b64 a, {%1, %2};\n mov.b64 b, {%3, %4};\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n}\n" ::"r"(d),
+        "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(id), "r"(acc)
+        : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool acc) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-                 "r"(a), "l"(b), "r"(id), "r"((uint32_t)acc)
-                 : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 b;\n mov.b64 b, {%2, %3};\n setp.ne.b32 p, %5, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b_lo), "r"(b_hi), "r"(id), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t on;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(on));
+    return on != 0;
 }
 __device__ __forceinline__ void commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -149,6 +157,21 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t at) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
     return v;
+}
+
+// Bounded wait (mbar_wait_bounded) whose limit is already in a register and
+// that reads the clock only when the barrier is not there yet.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, long long limit) {
+    if (mbar_test_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    if (limit >= kBoundedWaitLimit) {
+        while (!mbar_try_wait(bar, parity))
+            if (clock64() - t0 > limit) return false;
+        return true;
+    }
+    while (!mbar_test_wait(bar, parity))
+        if (clock64() - t0 > limit) return false;
+    return true;
 }
 
 // The rows that share keys: a group's queries against its prefix (kind 0), or a
@@ -339,6 +362,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         pc.u = u0;
         pc.n = (int)min((long long)(pc.tiles - at), u1 - u0);
     }
+    const long long limit_cycles = g_wait_limit;
     auto give_up = [&]() {
         *a.err = kErrAttnWait;
         failed_s = 1;
@@ -367,7 +391,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (!mbar_test_wait(&empty_bar[st], par)) {
                     cp_async_wait<0>();  // hand over all that is on its way before waiting for room
                     announce(it);
-                    if (!mbar_wait_bounded(&empty_bar[st], par) || failed_s) {
+                    if (!wait_bar(&empty_bar[st], par, limit_cycles) || failed_s) {
                         give_up();
                         ok = false;
                     }
@@ -399,7 +423,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 // the last products of the piece before need all of its tiles
                 cp_async_wait<0>();
                 announce(it);
-                if (!mbar_wait_bounded(&qempty_bar, (uint32_t)((seg - 1) & 1)) || failed_s) {
+                if (!wait_bar(&qempty_bar, (uint32_t)((seg - 1) & 1), limit_cycles) || failed_s) {
                     give_up();
                     ok = false;
                 }
@@ -470,15 +494,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (ok) announce(it);
     } else if (warp >= kMmaWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
-        if (warp == kMmaWarp && lane == 0) {
+        if (warp == kMmaWarp) {
+            // the whole warp waits; its elected thread issues
             int it = 0, np[2] = {0, 0};
             bool ok = true;
             const uint32_t qa = smem_u32(q_smem), ra = smem_u32(ring);
             auto wait = [&](uint64_t* bar, uint32_t par) {
-                if (ok && (!mbar_wait_bounded(bar, par) || failed_s)) {
+                if (ok && (!wait_bar(bar, par, limit_cycles) || failed_s)) {
                     give_up();
                     ok = false;
                 }
+                ok = __all_sync(0xffffffffu, ok);
                 fence_after();
             };
             auto acquire = [&]() {
@@ -486,27 +512,38 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 return it++ % NST;
             };
             constexpr uint32_t id_qk = idesc<T16>(kTile, false), id_pv = idesc<T16>(DP, true);
-            auto scores = [&](int s, int st) {
+            // S_s = Q K^T; then announces it and, if it was the tile's last use, frees the tile
+            auto scores = [&](int s, int st, bool last) {
+                if (elect_one()) {
+                    const uint32_t d = tmem + s * kTile, b = desc_lo_k(ra + st * SM::tile);
 #pragma unroll
-                for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+                    for (int part = 0; part < (SPLIT ? 2 : 1); ++part) {
+                        const uint32_t q = desc_lo_k(qa + (TWO ? s : part) * SM::tile);
 #pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) {
-                        const uint32_t off = (k >> 2) * (kTile * 128) + (k & 3) * 32;
-                        mma_ss(tmem + s * kTile, desc_k_major(qa + (TWO ? s : part) * SM::tile + off),
-                               desc_k_major(ra + st * SM::tile + off), id_qk, part + k > 0);
+                        for (int k = 0; k < DP / 16; ++k) {
+                            const uint32_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
+                            mma_ss(d, q + off, kDescHi, b + off, kDescHi, id_qk, part + k > 0);
+                        }
                     }
-                commit(&s_bar[s]);
+                    commit(&s_bar[s]);
+                    if (last) commit(&empty_bar[st]);
+                }
+                __syncwarp();
             };
-            auto sums = [&](int s, int st, bool first) {
+            // O_s += P V
+            auto sums = [&](int s, int st, bool first, bool last) {
                 wait(&p_bar[s], (uint32_t)(np[s]++ & 1));
                 if (!ok) return;
-                const uint32_t o = tmem + 2 * kTile + s * DP, pcol = tmem + s * kTile;
+                if (elect_one()) {
+                    const uint32_t o = tmem + 2 * kTile + s * DP, p = tmem + s * kTile, b = desc_lo_n(ra + st * SM::tile);
 #pragma unroll
-                for (int k = 0; k < kTile / 16; ++k)
+                    for (int k = 0; k < kTile / 16; ++k)
 #pragma unroll
-                    for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
-                        mma_ts(o, pcol + part * 64 + k * 8, desc_n_major(ra + st * SM::tile + k * 2048), id_pv,
-                               !(first && k + part == 0));
+                        for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+                            mma_ts(o, p + part * 64 + k * 8, b + k * (2048 >> 4), kDescHi, id_pv, k + part > 0 || !first);
+                    if (last) commit(&empty_bar[st]);
+                }
+                __syncwarp();
             };
             int seg = 0;
             for (Piece p = pc; ok && p.u < u1; p.next(a, BR, u1), ++seg) {
@@ -514,45 +551,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int t = 0; ok && t < min(LA, p.n); ++t) {
                     const int st = acquire();
                     if (!ok) break;
-                    scores(t, st);
-                    if (TWO) scores(1, st);
-                    commit(&empty_bar[st]);
+                    scores(t, st, !TWO);
+                    if (TWO) scores(1, st, true);
                 }
                 for (int t = 0; ok && t < p.n; ++t) {
                     const int sv = acquire();
+                    if (!ok) break;
                     if (TWO) {
-                        sums(0, sv, t == 0);
+                        sums(0, sv, t == 0, false);
                         int sk = 0;
                         if (ok && t + 1 < p.n) {
                             sk = acquire();
-                            if (ok) scores(0, sk);
+                            if (ok) scores(0, sk, false);
                         }
-                        if (ok) sums(1, sv, t == 0);
-                        if (!ok) break;
-                        commit(&empty_bar[sv]);
-                        if (t + 1 < p.n) {
-                            scores(1, sk);
-                            commit(&empty_bar[sk]);
-                        }
+                        if (ok) sums(1, sv, t == 0, true);
+                        if (ok && t + 1 < p.n) scores(1, sk, true);
                     } else {
-                        sums(t & 1, sv, t < 2);
-                        if (!ok) break;
-                        commit(&empty_bar[sv]);
-                        if (t + 2 < p.n) {
+                        sums(t & 1, sv, t < 2, true);
+                        if (ok && t + 2 < p.n) {
                             const int sk = acquire();
-                            if (!ok) break;
-                            scores(t & 1, sk);
-                            commit(&empty_bar[sk]);
+                            if (ok) scores(t & 1, sk, true);
                         }
                     }
                 }
                 if (!ok) break;
-                commit(&qempty_bar);
-                commit(&ofin_bar);
+                if (elect_one()) {
+                    commit(&qempty_bar);
+                    commit(&ofin_bar);
+                }
+                __syncwarp();
             }
-            commit(&done_bar);  // completes once every product issued above has
+            if (elect_one()) commit(&done_bar);  // completes once every product issued above has
+            __syncwarp();
         }
-        __syncwarp();
     } else {
         // --- softmax: stream s, row r of its tile
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
@@ -562,7 +593,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         int ns = 0, seg = 0, nj = 0;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t par) {
-            if (ok && (!mbar_wait_bounded(bar, par) || failed_s)) {
+            if (ok && (!wait_bar(bar, par, limit_cycles) || failed_s)) {
                 give_up();
                 ok = false;
             }
