@@ -1,6 +1,8 @@
 // paged_attn.cu -- causal attention over paged key/value caches with prefixes
 // shared by groups of sequences (beacon_cuda_op_paged_attention): the argument
 // checks and the kernel of any dtype and head size.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 
 #include <cmath>
@@ -53,7 +55,7 @@ __global__ void __launch_bounds__(kAnyWarps * 32) paged_attn_any_kernel(const Pa
     }
     float m = -INFINITY, l = 0.0f;
     for (int p = warp; p < limit; p += kAnyWarps) {
-        const int64_t row = page_row(a, p < s.prefix ? s.first : b, p);
+        const int64_t row = page_row(a, page_id(a, p < s.prefix ? s.first : b, p), p);
         if (row < 0) continue;
         const int64_t at = (row * a.Hkv + kvh) * a.D;
         const TK* k = static_cast<const TK*>(a.ck) + at;
@@ -161,6 +163,28 @@ PartArgs carve_part(Carve& c, const PagedArgs& a, int ctas, int slot_rows, bool 
     return p;
 }
 
+// [pages * page_size][Hkv][D] in boxes of `box` rows by 64 values of one head,
+// 128-byte swizzle; values past D and rows past the end arrive as zeros.
+CUtensorMap cache_map(const PagedArgs& a, const void* cache, int32_t tk) {
+    static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+        BC_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
+        if (q != cudaDriverEntryPointSuccess || !fn) fail(BEACON_CUDA_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    }();
+    CUtensorMap map;
+    const cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)a.Hkv, (cuuint64_t)a.pages * (cuuint64_t)a.page_size};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.D * 2, (cuuint64_t)a.Hkv * (cuuint64_t)a.D * 2};
+    const cuuint32_t box[3] = {64, 1, (cuuint32_t)a.box};
+    const cuuint32_t es[3] = {1, 1, 1};
+    const CUresult r = encode(&map, tk == BEACON_CUDA_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                              const_cast<void*>(cache), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) fail(BEACON_CUDA_ERR_CUDA, "cuTensorMapEncodeTiled failed for a paged cache");
+    return map;
+}
+
 void run_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream, PagedArgs a, int32_t tq, int32_t tk) {
     const int32_t F32 = BEACON_CUDA_DTYPE_F32, F16 = BEACON_CUDA_DTYPE_F16;
     if (tk != F32 && a.D <= 128) {
@@ -181,9 +205,16 @@ void run_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream, Paged
         };
         CallScratch scratch(ctx, stream, carve(nullptr));
         carve(scratch.data());
+        CacheMaps maps{};
+        if (a.pages > 0 && a.page_size % 8 == 0) {
+            a.box = 8;
+            while (a.box < 128 && a.page_size % (2 * a.box) == 0) a.box *= 2;
+            maps.k = cache_map(a, a.ck, tk);
+            maps.v = cache_map(a, a.cv, tk);
+        }
         bool pdl = !scratch.of_graph();  // a graph's allocation comes first
         if (tc) {
-            launch_paged_tc(plan, a, prefix, rest, tq, tk, stream->s, pdl);
+            launch_paged_tc(plan, a, maps, prefix, rest, tq, tk, stream->s, pdl);
             pdl = true;
         }
         if (decode) launch_paged_decode(a, rest, tq, tk, stream->s, pdl);
@@ -253,7 +284,7 @@ extern "C" int32_t beacon_cuda_op_paged_attention(BeaconCudaContext* ctx, Beacon
             check_i32(ctx, prefix_lens, groups, "paged_attention: prefix_lens");
             check_i32(ctx, group_starts, groups + 1, "paged_attention: group_starts");
         }
-        if (!std::isfinite(scale)) invalid("paged_attention: scale must be finite");
+        if (!std::isfinite(scale) || scale < 0.0f) invalid("paged_attention: scale must be finite and not negative");
         for (const BeaconCudaTensor* t : {q, cache_k, cache_v})
             if (!aligned16(t->data())) invalid("paged_attention: tensors must be 16-byte aligned");
         DeviceScope dev(ctx);
@@ -281,6 +312,8 @@ extern "C" int32_t beacon_cuda_op_paged_attention(BeaconCudaContext* ctx, Beacon
         a.groups = (int)groups;
         a.max_pages = (int)max_pages;
         a.page_size = (int)cache_k->shape[1];
+        for (int i = 0; i < 31; ++i)
+            if (a.page_size == 1 << i) a.page_shift = i;
         a.scale = scale;
         a.err = stream_error_word(stream);
         if (T > 0 && B > 0) run_paged_attention(ctx, stream, a, tq, tk);

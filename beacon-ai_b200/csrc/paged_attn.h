@@ -2,6 +2,8 @@
 // shared by its kernels (paged_attn*.cu).
 #pragma once
 
+#include <cuda.h>
+
 #include "common.cuh"
 #include "internal.h"
 
@@ -19,10 +21,13 @@ struct PagedArgs {
     const int32_t* prefix = nullptr;   // [groups]
     int64_t pages = 0;
     int T = 0, B = 0, H = 0, Hkv = 0, G = 0, D = 0, groups = 0;  // G = H / Hkv
-    int max_pages = 0, page_size = 0;
+    int max_pages = 0, page_size = 0, page_shift = -1;  // page_shift: log2 of a power of two, else -1
     // 1: a sequence's queries take its prefix and its own keys together (they
     // fill row blocks by themselves); 0: prefixes are done for whole groups
     int merged = 0;
+    // rows of one tensor copy of cache rows: the largest power of two, 8 to 128,
+    // that divides the page size; 0: rows are copied one by one
+    int box = 0;
     float scale = 0.0f;
     int* err = nullptr;
 };
@@ -68,8 +73,11 @@ struct PagedTcPlan {
     int ctas = 0;
 };
 PagedTcPlan plan_paged_tc(const BeaconCudaContext* ctx, const PagedArgs& a, bool split, bool with_rest);
-void launch_paged_tc(const PagedTcPlan& plan, const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, int32_t tq,
-                     int32_t tk, cudaStream_t s, bool pdl);
+struct CacheMaps {  // tensor maps of the caches (PagedArgs::box rows by 64 values of one head)
+    CUtensorMap k, v;
+};
+void launch_paged_tc(const PagedTcPlan& plan, const PagedArgs& a, const CacheMaps& maps, const PartArgs& prefix,
+                     const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s, bool pdl);
 void launch_paged_combine(const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, int32_t tq, cudaStream_t s);
 
 // A start array entry kept inside [0, n] (callers hold it in a device tensor).
@@ -143,10 +151,16 @@ __device__ __forceinline__ SeqInfo seq_info(const PagedArgs& a, int b) {
     return s;
 }
 
-// Cache row of position p < capacity through table row b; -1: bad page id.
-__device__ __forceinline__ int64_t page_row(const PagedArgs& a, int b, int p) {
-    const int64_t page = a.table[(int64_t)b * a.max_pages + p / a.page_size];
-    if (page >= 0 && page < a.pages) return page * a.page_size + p % a.page_size;
+// Cache row of position p < capacity through table row b, in two steps so that
+// the table entry can be fetched ahead of its use; -1: bad page id.
+__device__ __forceinline__ int page_index(const PagedArgs& a, int p) {
+    return a.page_shift >= 0 ? p >> a.page_shift : p / a.page_size;
+}
+__device__ __forceinline__ int page_id(const PagedArgs& a, int b, int p) {
+    return __ldg(a.table + (int64_t)b * a.max_pages + page_index(a, p));
+}
+__device__ __forceinline__ int64_t page_row(const PagedArgs& a, int page, int p) {
+    if (page >= 0 && page < a.pages) return (int64_t)page * a.page_size + (p - page_index(a, p) * a.page_size);
     *a.err = kErrIndex;
     return -1;
 }

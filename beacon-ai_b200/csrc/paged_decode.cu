@@ -132,12 +132,18 @@ __global__ void __launch_bounds__(kDecThreads) paged_decode_kernel(const PagedAr
         const int rl = lane / CH, chunk16 = lane % CH;
         const bool chunk_live = chunk16 * 8 < a.D;
 
-        // cache row of this lane's key of a tile; -1: none
-        auto row_of = [&](const Walk& w) -> int {
-            const int p = w.cur.from + w.tile * kDecKeys + warp * 16 + (lane & 15);
-            return p < w.cur.to ? (int)page_row(a, w.b, p) : -1;
+        // this lane's key of a tile and its page (fetched a tile ahead)
+        struct Key {
+            int pos, page;  // pos -1: no key
         };
-        auto copy_tile = [&](int stage, int kvh, int row) {
+        auto key_of = [&](const Walk& w) {
+            const int p = w.cur.from + w.tile * kDecKeys + warp * 16 + (lane & 15);
+            Key k{-1, 0};
+            if (p < w.cur.to) k = Key{p, page_id(a, w.b, p)};
+            return k;
+        };
+        auto copy_tile = [&](int stage, int kvh, Key k) {
+            const int row = k.pos >= 0 ? (int)page_row(a, k.page, k.pos) : -1;
             const uint32_t dst = smem_u32(ring + stage * 2 * S::sub);
 #pragma unroll
             for (int i = 0; i < 16 / RPI; ++i) {
@@ -150,13 +156,13 @@ __global__ void __launch_bounds__(kDecThreads) paged_decode_kernel(const PagedAr
                 cp_async16_zfill(d + S::sub, static_cast<const TK*>(a.cv) + src, live);
             }
         };
-        int row_next = row_of(load);
+        Key key_next = key_of(load);
 #pragma unroll
         for (int i = 0; i < NS - 1; ++i) {
             if (i < count) {
-                copy_tile(i, load.kvh, row_next);
+                copy_tile(i, load.kvh, key_next);
                 load.step(a);
-                if (i + 1 < count) row_next = row_of(load);
+                if (i + 1 < count) key_next = key_of(load);
             }
             cp_async_commit();
         }
@@ -193,8 +199,9 @@ __global__ void __launch_bounds__(kDecThreads) paged_decode_kernel(const PagedAr
                     if constexpr (SPLIT) {
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                        const float sc = query_scale(mx);
-                        cs[r] /= sc;
+                        float inv;
+                        const float sc = query_scale(mx, inv);
+                        cs[r] *= inv;
 #pragma unroll
                         for (int k = 0; k < KSTEPS; ++k)
 #pragma unroll
@@ -211,9 +218,9 @@ __global__ void __launch_bounds__(kDecThreads) paged_decode_kernel(const PagedAr
             cp_async_wait<NS - 2>();
             __syncwarp();  // the tile has landed for every lane, and all have read the stage refilled next
             if (j + NS - 1 < count) {
-                copy_tile((j + NS - 1) % NS, load.kvh, row_next);
+                copy_tile((j + NS - 1) % NS, load.kvh, key_next);
                 load.step(a);
-                if (j + NS < count) row_next = row_of(load);
+                if (j + NS < count) key_next = key_of(load);
             }
             cp_async_commit();
 

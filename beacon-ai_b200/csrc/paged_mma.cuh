@@ -72,12 +72,14 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uin
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The power of two that brings the largest magnitude of a 32-bit query row
-// into [2^14, 2^15), so that its f16 parts neither overflow nor lose bits; 1
-// for rows that are zero or not finite.
-__device__ __forceinline__ float query_scale(float mx) {
-    if (!(mx > 0.0f) || mx == INFINITY) return 1.0f;
-    return exp2f((float)min(126, 14 - ilogbf(mx)));
+// The power of two that brings the largest magnitude mx of a 32-bit query row
+// to [2^14, 2^15), so that its f16 parts neither overflow nor lose bits, and its
+// reciprocal (exponent arithmetic; exponents below 2^-112 stay smaller). Rows
+// that are not finite come out as such.
+__device__ __forceinline__ float query_scale(float mx, float& inverse) {
+    const int e = min(254, max(15, (int)(__float_as_uint(mx) >> 23)));  // mx >= 0
+    inverse = __uint_as_float((uint32_t)(e - 14) << 23);
+    return __uint_as_float((uint32_t)(268 - e) << 23);
 }
 
 // x as a sum of two f16 values (hi: rounded, lo: what that left, rounded).

@@ -18,9 +18,14 @@
 // P replaces S: the packed weights (64 columns, then 64 of their remainders)
 // lie where the scores were, and are the A operand of O += P V from tensor
 // memory; V is read N-major.
-// Four producer warps copy key and value rows, page by page, with 16-byte
-// asynchronous copies into a ring of tiles in the 128-byte swizzle; one thread
-// issues the products. The key tiles of all blocks form one line that the CTAs
+// Key and value rows come in page by page by tensor copies (TMA) of up to 128
+// rows into a ring of tiles in the 128-byte swizzle, requested by one warp;
+// rows of a value tile that are no keys of the block are zeroed there (their
+// weights are zero, but what a page holds behind its last row may be no
+// number). 16-byte asynchronous copies by four warps, which zero-fill, serve
+// page sizes that are no multiple of 8 (they reach 8 bytes a cycle and
+// multiprocessor: the tensor copies are what feeds the matrix unit). One
+// thread issues the products. The key tiles of all blocks form one line that the CTAs
 // share evenly (PartArgs).
 // The running maximum moves only when a tile exceeds it by 2^8: the sums are
 // rescaled in tensor memory then, and the weights stay below 2^8.
@@ -43,8 +48,8 @@ constexpr int kSoftWarps = 8;
 constexpr int kLoadWarp = 8, kLoadWarps = 4;
 constexpr int kMmaWarp = 12;            // with three idle warps: registers move by groups of four warps
 constexpr int kTcThreads = 512;
-// registers: 128 a thread at launch; 2 x 184 + 80 + 64 = 4 x 128
-constexpr int kSoftRegs = 184, kLoadRegs = 80, kMmaRegs = 64;
+// registers: 128 a thread at launch; 2 x 176 + 104 + 56 = 4 x 128
+constexpr int kSoftRegs = 176, kLoadRegs = 104, kMmaRegs = 56;
 constexpr uint32_t kTmemCols = 512;     // S 2 x 128, O 2 x DP
 constexpr float kRescale = 8.0f;        // log2 of the largest weight
 
@@ -111,15 +116,10 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
         : "r"(addr));
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(addr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
-        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
-        "r"(r[31])
-        : "memory");
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -149,6 +149,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     unsigned long long d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(as_u64(a)), "l"(as_u64(b)));
     return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 __device__ __forceinline__ void st_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -181,6 +186,7 @@ struct Block {
     int b = 0;                   // page table row
     int cut = 0, first = 0;      // keys below cut are read through table row `first`
     int key0 = 0, key1 = 0;      // keys [key0, key1)
+    int base = 0;                // where the first tile begins: key0, or the copy box that holds it
     int tok0 = 0, rows = 0;      // query rows tok0 * G ..
     int nq = 0, len = 0;         // kind 1: causal limits
 };
@@ -207,6 +213,7 @@ __device__ __forceinline__ Block block_of(const PagedArgs& a, int e) {
     } else {
         k.key0 = s.prefix;
     }
+    k.base = a.box ? k.key0 & ~(a.box - 1) : k.key0;
     k.key1 = s.len;
     k.tok0 = s.q0;
     k.rows = s.nq * a.G;
@@ -218,7 +225,7 @@ __device__ __forceinline__ Block block_of(const PagedArgs& a, int e) {
 __device__ __forceinline__ int tiles_of(const PagedArgs& a, const Block& k, int rt, int block_rows) {
     int end = k.key1;
     if (k.kind) end = min(end, k.len - k.nq + (min((rt + 1) * block_rows, k.rows) - 1) / a.G + 1);
-    return end > k.key0 ? (end - k.key0 + kTile - 1) / kTile : 0;
+    return end > k.key0 ? (end - k.base + kTile - 1) / kTile : 0;
 }
 __device__ __forceinline__ int tiles_of_block(const PagedArgs& a, const Block& k, int block_rows) {
     const int n = (k.rows + block_rows - 1) / block_rows;
@@ -262,9 +269,17 @@ struct Piece {
     }
 };
 
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int head, int row, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(row), "r"(smem_u32(bar))
+        : "memory");
+}
+
 template <typename TQ, typename T16, int DP, bool SPLIT, bool TWO>
 __global__ void __launch_bounds__(kTcThreads, 1)
-    paged_tc_kernel(const PagedArgs a, const PartArgs prefix, const PartArgs rest, int entries, int line_ctas) {
+    paged_tc_kernel(const PagedArgs a, const __grid_constant__ CacheMaps maps, const PartArgs prefix, const PartArgs rest, int entries,
+                    int line_ctas) {
     using SM = TcSmem<DP, SPLIT, TWO>;
     constexpr int NST = SM::stages;
     constexpr int LA = TWO ? 1 : 2;              // key tiles ahead of the value tile
@@ -272,7 +287,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     constexpr int CH = DP / 8;                   // 16-byte chunks of a row
     extern __shared__ uint8_t tc_smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[NST], empty_bar[NST], qfull_bar, qempty_bar, s_bar[2], p_bar[2], ofin_bar, join_bar,
-        done_bar;
+        fix_bar, done_bar;
     __shared__ uint32_t tmem_s;
     __shared__ volatile int failed_s;
     __shared__ float qscale_s[2][kTile];   // SPLIT: what the scores are multiplied by
@@ -285,7 +300,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < NST; ++i) {
-            mbar_init(&full_bar[i], kLoadWarps * 32);
+            mbar_init(&full_bar[i], a.box ? 1 : kLoadWarps * 32);
             mbar_init(&empty_bar[i], 1);
         }
         mbar_init(&qfull_bar, kLoadWarps * 32);
@@ -296,6 +311,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         mbar_init(&ofin_bar, 1);
         mbar_init(&join_bar, 2 * kTile);
+        mbar_init(&fix_bar, 1);
         mbar_init(&done_bar, 1);
         failed_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -375,61 +391,147 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int64_t stride = (int64_t)a.Hkv * a.D * 2;  // bytes from one cache row to the next
         const int c = lane % CH;                          // this lane's chunk of the rows it copies
         const bool chunk_live = c * 8 < a.D;
-        int it = 0, told = 0;  // tiles requested, tiles announced
+        int it = 0, told = 0, nfix = 0;  // tiles requested, tiles announced
         bool ok = true;
         auto announce = [&](int upto) {  // tiles [told, upto) have landed
             if (told < upto) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             for (; told < upto; ++told) arrive(&full_bar[told % NST]);
         };
         constexpr int RPI = 32 / CH;  // rows that one copy instruction of a warp covers
-        auto load_tile = [&](const Piece& p, int tile, const void* cache) {
-            const int pos = p.k.key0 + tile * kTile + pw * 32 + lane;
-            const int row = pos < p.k.key1 ? (int)page_row(a, pos < p.k.cut ? p.k.first : p.k.b, pos) : -1;
-            const int st = it % NST;
-            if (it >= NST) {
-                const uint32_t par = (uint32_t)((it / NST - 1) & 1);
-                if (!mbar_test_wait(&empty_bar[st], par)) {
-                    cp_async_wait<0>();  // hand over all that is on its way before waiting for room
+        // The tiles of a piece in the order of their use: LA key tiles, then
+        // value tile t and key tile t + LA in turn, then the last value tiles.
+        auto key_tile = [&](const Piece& p, int f, bool& value) {
+            const int la = min(LA, p.n), j = f - la, pairs = 2 * (p.n - la);
+            value = j >= 0 && (j >= pairs || (j & 1) == 0);
+            return j < 0 ? f : j >= pairs ? p.n - la + (j - pairs) : value ? j / 2 : j / 2 + la;
+        };
+        // this lane's first row of a tile (copies row by row: 32 rows a warp;
+        // tensor copies: a box a lane) and its page
+        auto pos_of = [&](const Piece& p, int t) {
+            return p.k.base + (p.tile + t) * kTile + (a.box ? lane * a.box : pw * 32 + lane);
+        };
+        auto page_of = [&](const Piece& p, int f) {
+            bool value;
+            const int pos = f < 2 * p.n ? pos_of(p, key_tile(p, f, value)) : p.k.key1;
+            if (pos >= p.k.key1 || (a.box && lane * a.box >= kTile)) return 0;
+            return page_id(a, pos < p.k.cut ? p.k.first : p.k.b, pos);
+        };
+        auto room = [&]() {  // waits for the stage of tile `it`
+            const uint32_t par = (uint32_t)((it / NST - 1) & 1);
+            if (it >= NST && !mbar_test_wait(&empty_bar[it % NST], par)) {
+                if (!a.box) {
+                    cp_async_wait<0>();  // hand over all that is on its way before waiting
                     announce(it);
-                    if (!wait_bar(&empty_bar[st], par, limit_cycles) || failed_s) {
-                        give_up();
-                        ok = false;
-                    }
                 }
-                // the lanes copy for each other: they go on or give up together
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return;
+                if (!wait_bar(&empty_bar[it % NST], par, limit_cycles) || failed_s) {
+                    give_up();
+                    ok = false;
+                }
             }
-            const uint32_t dst = smem_u32(ring + (size_t)st * SM::tile) + (c >> 3) * (kTile * 128);
+            ok = __all_sync(0xffffffffu, ok);  // the lanes copy for each other: they go on or give up together
+            return ok;
+        };
+        // Rows pos0 + lane of a tile (of 32) one by one, 16 bytes a lane
+        auto copy_rows = [&](const Piece& p, const void* cache, int r0, int row) {
+            const uint32_t dst = smem_u32(ring + (size_t)(it % NST) * SM::tile) + (c >> 3) * (kTile * 128);
             const uint8_t* src = static_cast<const uint8_t*>(cache) + (p.kvh * a.D + c * 8) * 2;
 #pragma unroll 8
             for (int i = 0; i < 32 / RPI; ++i) {
                 const int rr = i * RPI + lane / CH;
                 const int cr = __shfl_sync(0xffffffffu, row, rr);
                 const bool live = cr >= 0 && chunk_live;
-                const int r = pw * 32 + rr;
+                const int r = r0 + rr;
                 cp_async16_zfill(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), live ? src + cr * stride : static_cast<const uint8_t*>(cache), live);
             }
-            cp_async_commit();
-            ++it;
-            if (it - told > 2) {  // two tiles stay in flight
-                cp_async_wait<2>();
-                announce(it - 2);
+        };
+        auto load_tile = [&](const Piece& p, int f, int page) {
+            bool value;
+            const int t = key_tile(p, f, value);
+            if (a.box && pw > 0) return;
+            if (!room()) return;
+            const int pos = pos_of(p, t);
+            if (!a.box) {
+                copy_rows(p, value ? a.cv : a.ck, pw * 32, pos < p.k.key1 ? (int)page_row(a, page, pos) : -1);
+                cp_async_commit();
+                ++it;
+                if (it - told > 2) {  // two tiles stay in flight
+                    cp_async_wait<2>();
+                    announce(it - 2);
+                }
+                return;
             }
+            const int st = it % NST;
+            const int pos0 = p.k.base + (p.tile + t) * kTile;
+            const uint32_t dst = smem_u32(ring + (size_t)st * SM::tile);
+            const bool mine = lane * a.box < kTile && pos < p.k.key1;
+            if (__any_sync(0xffffffffu, mine && pos < p.k.cut && pos + a.box > p.k.cut)) {
+                // a box whose rows lie in two tables: this tile row by row
+                for (int r0 = 0; r0 < kTile; r0 += 32) {
+                    const int q = pos0 + r0 + lane;
+                    copy_rows(p, value ? a.cv : a.ck, r0,
+                              q < p.k.key1 ? (int)page_row(a, page_id(a, q < p.k.cut ? p.k.first : p.k.b, q), q) : -1);
+                }
+                cp_async_commit();
+                cp_async_wait<0>();
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) arrive(&full_bar[st]);
+                ++it;
+                return;
+            }
+            // a value tile with rows that are no keys lands on fix_bar first
+            const bool part = value && (pos0 < p.k.key0 || pos0 + kTile > p.k.key1);
+            uint64_t* bar = part ? &fix_bar : &full_bar[st];
+            const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
+            if (lane == 0) mbar_expect_tx(bar, (uint32_t)(boxes * a.box * DP * 2));
+            __syncwarp();
+            if (mine) {
+                int64_t row = page_row(a, page, pos);
+                if (row < 0) row = a.pages * a.page_size;  // outside: zeros
+#pragma unroll
+                for (int h = 0; h < DP / 64; ++h)
+                    tma_rows(dst + h * (kTile * 128) + lane * a.box * 128, value ? &maps.v : &maps.k, h * 64, p.kvh, (int)row, bar);
+            }
+            if (part) {
+                if (!wait_bar(bar, (uint32_t)(nfix++ & 1), limit_cycles)) {
+                    mbar_drain(bar, (uint32_t)((nfix - 1) & 1));
+                    give_up();
+                    ok = false;
+                }
+                const int lo = max(0, p.k.key0 - pos0), hi = min(kTile, p.k.key1 - pos0);  // rows [lo, hi) are keys
+                for (int i = lane; i < (lo + kTile - hi) * CH; i += 32) {
+                    const int q = i / CH, r = q < lo ? q : hi + q - lo, cc = i % CH;
+                    st_shared16(dst + (cc >> 3) * (kTile * 128) + r * 128 + ((cc & 7) << 4), 0, 0, 0, 0);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                ok = __all_sync(0xffffffffu, ok);
+                if (lane == 0) arrive(&full_bar[st]);
+            }
+            ++it;
         };
         int seg = 0;
         for (Piece p = pc; ok && p.u < u1; p.next(a, BR, u1), ++seg) {
+            // the first tiles are on their way while the queries are brought in
+            int f = 0, page = page_of(p, 0);
+            auto load_next = [&]() {
+                const int ahead = page_of(p, f + 1);
+                load_tile(p, f++, page);
+                page = ahead;
+            };
+            while (ok && f < min(3, 2 * p.n)) load_next();
             if (seg > 0) {
-                // the last products of the piece before need all of its tiles
-                cp_async_wait<0>();
-                announce(it);
+                if (!a.box) {
+                    // the last products of the piece before need all of its tiles
+                    cp_async_wait<0>();
+                    announce(it);
+                }
                 if (!wait_bar(&qempty_bar, (uint32_t)((seg - 1) & 1), limit_cycles) || failed_s) {
                     give_up();
                     ok = false;
                 }
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
             }
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
 #pragma unroll 1
             for (int i = 0; i < (TWO ? 2 : 1); ++i) {
                 // this lane's query row, as a row of [T * H][D]; -1: behind the block
@@ -437,24 +539,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const int qrow = br < p.k.rows ? (p.k.tok0 + br / a.G) * a.H + p.kvh * a.G + br % a.G : -1;
                 const uint32_t dst = smem_u32(q_smem) + (TWO ? i * SM::tile : 0);
                 if constexpr (SPLIT) {
-                    // a warp takes a row at a time, eight on their way: each lane four values
+                    // a warp takes a row at a time, sixteen on their way: each lane four values
 #pragma unroll 1
-                    for (int r0 = 0; r0 < 32; r0 += 8) {
-                        float4 x[8];
+                    for (int r0 = 0; r0 < 32; r0 += 16) {
+                        float4 x[16];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
+                        for (int k = 0; k < 16; ++k) {
                             const int qr = __shfl_sync(0xffffffffu, qrow, r0 + k);
                             x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                             if (qr >= 0 && lane * 4 < a.D)
                                 x[k] = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (int64_t)qr * a.D + lane * 4);
                         }
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
+                        for (int k = 0; k < 16; ++k) {
                             const int r = pw * 32 + r0 + k;
                             float mx = fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w)));
                             mx = warp_max(mx);
-                            const float sc = query_scale(mx);
-                            if (lane == 0) qscale_s[seg & 1][r] = fabsf(a.scale) * 1.4426950408889634f / sc;
+                            float inv;
+                            const float sc = query_scale(mx, inv);
+                            if (lane == 0) qscale_s[seg & 1][r] = a.scale * 1.4426950408889634f * inv;
                             if (lane * 4 < DP) {
                                 uint2 h, l;
                                 split_f16(x[k].x * sc, x[k].y * sc, h.x, l.x);
@@ -484,14 +587,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             arrive(&qfull_bar);
-            for (int t = 0; ok && t < min(LA, p.n); ++t) load_tile(p, p.tile + t, a.ck);
-            for (int t = 0; ok && t < p.n; ++t) {
-                load_tile(p, p.tile + t, a.cv);
-                if (ok && t + LA < p.n) load_tile(p, p.tile + t + LA, a.ck);
-            }
+            while (ok && f < 2 * p.n) load_next();
         }
-        cp_async_wait<0>();  // nothing may land after the CTA has ended
-        if (ok) announce(it);
+        // nothing may land after the CTA has ended
+        cp_async_wait<0>();
+        if (!a.box && ok) announce(it);
+        if (a.box && pw == 0)
+            for (int i = max(0, it - NST); i < it; ++i) mbar_drain(&full_bar[i % NST], (uint32_t)((i / NST) & 1));
     } else if (warp >= kMmaWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
         if (warp == kMmaWarp) {
@@ -604,12 +706,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int row = p.rt * BR + (TWO ? s * kTile : 0) + r;  // of the block
             const bool live = row < p.k.rows;
             const int tok = p.k.tok0 + row / a.G;
-            int limit = 0;
+            int limit = 0x7FFFFFFF;  // rows behind the block: whatever comes out is not written
             if (live) {
                 if (p.k.kind) {
                     limit = min(p.k.len, p.k.len - p.k.nq + row / a.G + 1);
                 } else {
                     const int b = a.qstarts ? span_of(a.qstarts, a.B, tok) : tok;
+                    limit = 0;
                     if (b >= 0) {
                         const SeqInfo si = seq_info(a, b);
                         limit = min(p.k.key1, min(si.len, si.len - si.nq + (tok - si.q0) + 1));
@@ -618,34 +721,38 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             wait(&qfull_bar, (uint32_t)(seg & 1));
             if (!ok) break;
-            const float cs = SPLIT ? qscale_s[seg & 1][r] : fabsf(a.scale) * 1.4426950408889634f;
+            // above zero, so that a masked score (-inf) stays one
+            const float cs = fmaxf(SPLIT ? qscale_s[seg & 1][r] : a.scale * 1.4426950408889634f, 1e-37f);
+            const bool idle = __all_sync(0xffffffffu, !live);
             float m = -INFINITY, l = 0.0f;
             for (int t = TWO ? 0 : s; t < p.n; t += TWO ? 1 : 2) {
                 wait(&s_bar[s], (uint32_t)(ns++ & 1));
                 if (!ok) break;
-                const int key = p.k.key0 + (p.tile + t) * kTile;
-                const int seen = limit - key;  // columns [0, seen) are visible
-                const bool whole = __all_sync(0xffffffffu, seen >= kTile);
+                if (idle) {  // a warp without rows leaves its lanes as they are
+                    fence_before();
+                    arrive(&p_bar[s]);
+                    continue;
+                }
+                const int key = p.k.base + (p.tile + t) * kTile;
+                const int seen = limit - key, skip = p.k.key0 - key;  // columns [skip, seen) are visible
+                const bool whole = __all_sync(0xffffffffu, seen >= kTile && skip <= 0);
                 float v[kTile];
 #pragma unroll
                 for (int c = 0; c < kTile; c += 32) tmem_ld32(s_col + c, *reinterpret_cast<float(*)[32]>(v + c));
                 tmem_wait_ld();
-                if (a.scale < 0.0f) {
-#pragma unroll
-                    for (int i = 0; i < kTile; ++i) v[i] = -v[i];
-                }
                 if (!whole) {
 #pragma unroll
                     for (int i = 0; i < kTile; ++i)
-                        if (i >= seen) v[i] = -INFINITY;
+                        if (i >= seen || i < skip) v[i] = -INFINITY;
                 }
                 float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                for (int i = 4; i < kTile; i += 4)
+                for (int i = 4; i < kTile - 4; i += 8)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], v[i + j]);
-                top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                const float mx = top[0] == -INFINITY ? m : fmaxf(m, top[0] * cs);
+                    for (int j = 0; j < 4; ++j) top[j] = max3(top[j], v[i + j], v[i + 4 + j]);
+                top[0] = max3(top[0], top[1], fmaxf(top[2], top[3]));
+                top[0] = max3(max3(top[0], v[kTile - 4], v[kTile - 3]), v[kTile - 2], v[kTile - 1]);
+                const float mx = fmaxf(m, top[0] * cs);
                 const bool move = m != -INFINITY && mx > m + kRescale;
                 if (t >= (TWO ? 1 : 2) && __any_sync(0xffffffffu, move)) {
                     const float keep = move ? exp2_fast(m - mx) : 1.0f;
@@ -665,26 +772,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const float ref = m == -INFINITY ? 0.0f : m;
                 const float2 cs2 = make_float2(cs, cs), ref2 = make_float2(-ref, -ref);
                 float2 sum[2] = {make_float2(l, 0.0f), make_float2(0.0f, 0.0f)};
-                // the weights, 64 at a time so that the matrix unit's columns are written early
+                // the weights, 16 at a time: the packed ones take the registers of few scores
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t w[32], w2[SPLIT ? 32 : 1];
+                for (int c = 0; c < kTile / 16; ++c) {
+                    uint32_t w[8], w2[8];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int k = h * 64 + 2 * i;
+                    for (int i = 0; i < 8; ++i) {
+                        const int k = c * 16 + 2 * i;
                         float2 x = fma2(make_float2(v[k], v[k + 1]), cs2, ref2);
                         x.x = exp2_fast(x.x);
                         x.y = exp2_fast(x.y);
-                        if (!whole) {  // also where a zero scale times the mask is no number
-                            if (k >= seen) x.x = 0.0f;
-                            if (k + 1 >= seen) x.y = 0.0f;
-                        }
                         sum[i & 1] = add2(sum[i & 1], x);
                         if constexpr (SPLIT) split_f16(x.x, x.y, w[i], w2[i]);
                         else w[i] = Half2Of<T16>::pack(x.x, x.y);
                     }
-                    tmem_st32(s_col + h * 32, w);
-                    if constexpr (SPLIT) tmem_st32(s_col + 64 + h * 32, w2);
+                    tmem_st8(s_col + c * 8, w);
+                    if constexpr (SPLIT) tmem_st8(s_col + 64 + c * 8, w2);
                 }
                 sum[0] = add2(sum[0], sum[1]);
                 l = sum[0].x + sum[0].y;
@@ -818,24 +921,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 template <typename TQ, typename T16, int DP, bool SPLIT, bool TWO>
-void launch_tc_t(const PagedTcPlan& plan, const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, cudaStream_t s, bool pdl) {
+void launch_tc_t(const PagedTcPlan& plan, const PagedArgs& a, const CacheMaps& maps, const PartArgs& prefix, const PartArgs& rest, cudaStream_t s, bool pdl) {
     auto kern = paged_tc_kernel<TQ, T16, DP, SPLIT, TWO>;
     allow_max_dynamic_smem(kern);
     const int entries = (a.merged ? 0 : a.groups) + (plan.rest ? a.B : 0);
-    launch_kernel(kern, dim3((unsigned)plan.ctas), dim3(kTcThreads), TcSmem<DP, SPLIT, TWO>::bytes, s, pdl, a, prefix, rest, entries,
+    launch_kernel(kern, dim3((unsigned)plan.ctas), dim3(kTcThreads), TcSmem<DP, SPLIT, TWO>::bytes, s, pdl, a, maps, prefix, rest, entries,
                   plan.ctas);
 }
 
 template <int DP>
-void launch_tc_d(const PagedTcPlan& plan, const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, int32_t tq, int32_t tk,
+void launch_tc_d(const PagedTcPlan& plan, const PagedArgs& a, const CacheMaps& maps, const PartArgs& prefix, const PartArgs& rest, int32_t tq, int32_t tk,
                  cudaStream_t s, bool pdl) {
     using H = __half;
     using B = __nv_bfloat16;
-    if (tq == BEACON_CUDA_DTYPE_F32) launch_tc_t<float, H, DP, true, false>(plan, a, prefix, rest, s, pdl);
-    else if (tk == BEACON_CUDA_DTYPE_F16 && plan.two) launch_tc_t<H, H, DP, false, true>(plan, a, prefix, rest, s, pdl);
-    else if (tk == BEACON_CUDA_DTYPE_F16) launch_tc_t<H, H, DP, false, false>(plan, a, prefix, rest, s, pdl);
-    else if (plan.two) launch_tc_t<B, B, DP, false, true>(plan, a, prefix, rest, s, pdl);
-    else launch_tc_t<B, B, DP, false, false>(plan, a, prefix, rest, s, pdl);
+    if (tq == BEACON_CUDA_DTYPE_F32) launch_tc_t<float, H, DP, true, false>(plan, a, maps, prefix, rest, s, pdl);
+    else if (tk == BEACON_CUDA_DTYPE_F16 && plan.two) launch_tc_t<H, H, DP, false, true>(plan, a, maps, prefix, rest, s, pdl);
+    else if (tk == BEACON_CUDA_DTYPE_F16) launch_tc_t<H, H, DP, false, false>(plan, a, maps, prefix, rest, s, pdl);
+    else if (plan.two) launch_tc_t<B, B, DP, false, true>(plan, a, maps, prefix, rest, s, pdl);
+    else launch_tc_t<B, B, DP, false, false>(plan, a, maps, prefix, rest, s, pdl);
 }
 
 }  // namespace
@@ -850,10 +953,10 @@ PagedTcPlan plan_paged_tc(const BeaconCudaContext* ctx, const PagedArgs& a, bool
     return p;
 }
 
-void launch_paged_tc(const PagedTcPlan& plan, const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, int32_t tq,
-                     int32_t tk, cudaStream_t s, bool pdl) {
-    if (a.D <= 64) launch_tc_d<64>(plan, a, prefix, rest, tq, tk, s, pdl);
-    else launch_tc_d<128>(plan, a, prefix, rest, tq, tk, s, pdl);
+void launch_paged_tc(const PagedTcPlan& plan, const PagedArgs& a, const CacheMaps& maps, const PartArgs& prefix,
+                     const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s, bool pdl) {
+    if (a.D <= 64) launch_tc_d<64>(plan, a, maps, prefix, rest, tq, tk, s, pdl);
+    else launch_tc_d<128>(plan, a, maps, prefix, rest, tq, tk, s, pdl);
 }
 
 }  // namespace bc

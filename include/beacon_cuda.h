@@ -373,7 +373,7 @@ int32_t beacon_cuda_op_paged_append(BeaconCudaContext* ctx, BeaconCudaStream* st
  * 0 upwards to B; NULL: none) hold the same keys below position prefix_lens[g]
  * (I32 [G]); those are read through the page table row of the group's first
  * sequence, once for all queries of the group.
- *   scale multiplies the scores. A query that sees no key gives zeros. Rows of
+ *   scale (not negative) multiplies the scores. A query that sees no key gives zeros. Rows of
  * q behind the last sequence are not written. Cache rows at positions >=
  * kv_lens[b] are never read. Dtypes (q, caches): (F32, F16), (F16, F16), (BF16,
  * BF16) and (F32, F32); D a multiple of 8 up to 256, tensors 16-byte aligned.

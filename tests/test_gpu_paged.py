@@ -313,6 +313,8 @@ def test_attention_single_rows(be, s, dtype, cache, H, Hkv, D, ps, lens):
     (8, 2, 128, 16, [150, 131, 140, 70, 65, 64, 9], [0, 3, 6, 7], [130, 64, 0]),   # a prefix that ends inside a page
     (4, 4, 64, 8, [20, 10, 5, 30], [0, 3], [16]),      # sequences shorter than the prefix, one in no group
     (16, 1, 64, 32, [700] * 20, [0, 20], [650]),
+    (8, 2, 128, 5, [300, 280, 299], [0, 3], [270]),    # pages of no multiple of 8 rows
+    (40, 2, 128, 64, [300, 400, 500], [0, 2, 3], [250, 70]),   # many heads, prefixes that end inside a page
     (4, 2, 64, 16, [33, 20, 18], [0, 2, 2, 3], [16, 5, 16]),   # an empty group
 ])
 def test_attention_shared_prefix(be, s, dtype, cache, H, Hkv, D, ps, lens, groups, prefix):
@@ -332,6 +334,11 @@ def test_attention_shared_prefix(be, s, dtype, cache, H, Hkv, D, ps, lens, group
     (8, 1, 64, 8, [50, 45, 61, 20], [10, 5, 21, 20], [0, 2, 4], [40, 0]),
     (6, 2, 128, 32, [3, 2], [5, 2], None, None),      # more queries than keys: the first see nothing
     (4, 1, 64, 16, [30, 40], [20, 30], [0, 2], [25]),   # queries inside the prefix
+    (8, 1, 64, 16, [200, 260, 170], [60, 100, 33], [0, 3], [130]),   # prompts that fill row blocks, a prefix that ends inside a page
+    (8, 2, 128, 32, [400, 333], [300, 200], [0, 2], [128]),
+    (8, 2, 128, 8, [300, 290], [150, 140], [0, 2], [140]),
+    (8, 2, 80, 24, [300, 290], [150, 140], [0, 2], [144]),
+    (8, 2, 128, 10, [300, 290], [150, 140], [0, 2], [77]),    # pages of no multiple of 8 rows
 ])
 def test_attention_many_rows(be, s, dtype, cache, H, Hkv, D, ps, lens, new, groups, prefix):
     rng = np.random.default_rng(H + D + sum(lens) + sum(new))
@@ -497,6 +504,7 @@ def test_attention_refusals(be, s):
         refused(L.ERR_UNSUPPORTED_DTYPE, lambda: be.paged_attention(s, be.zeros((3, 4, 64), a), c, be.zeros((4, 8, 2, 64), b), tb, ln, 0.1))
     refused(L.ERR_UNSUPPORTED_DTYPE, lambda: be.paged_attention(s, q, ck, cv, tb, be.zeros((3,)), 0.1))
     refused(L.ERR_INVALID_ARGUMENT, lambda: be.paged_attention(s, q, ck, cv, tb, ln, math.inf))
+    refused(L.ERR_INVALID_ARGUMENT, lambda: be.paged_attention(s, q, ck, cv, tb, ln, -0.1))
     refused(L.ERR_INVALID_ARGUMENT, lambda: be.paged_attention(s, q, ck, cv, tb, ln, 0.1, out=q))
     refused(L.ERR_INVALID_ARGUMENT, lambda: be.paged_attention(s, q, ck, cv, tb, ln, 0.1, prefix_lens=be.zeros((1,), I)))
     refused(L.ERR_SHAPE_MISMATCH, lambda: be.paged_attention(s, q, ck, cv, tb, ln, 0.1, out=be.zeros((3, 4, 32))))
