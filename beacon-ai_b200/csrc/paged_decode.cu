@@ -377,85 +377,92 @@ __global__ void __launch_bounds__(kDecThreads) paged_decode_kernel(const PagedAr
     pdl_wait();
 }
 
-// The parts of one query row: both kinds, each a first part and those of the
-// CTAs after it. One warp per row.
+// The parts of the query rows of one token: both kinds, each a first part and
+// those of the CTAs after it. A warp takes a head at a time; the token's place
+// is worked out once for the block's heads.
 template <typename TQ, typename T16>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const PagedArgs a, const PartArgs prefix, const PartArgs rest) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(128) paged_combine_kernel(const PagedArgs a, const PartArgs prefix, const PartArgs rest, int heads) {
     const int lane = threadIdx.x & 31;
     pdl_wait();
-    if (row >= (int64_t)a.T * a.H) return;
-    const int t = (int)(row / a.H), h = (int)(row - (int64_t)t * a.H);
+    const int t = blockIdx.x;
     const int b = a.qstarts ? span_of(a.qstarts, a.B, t) : t;
     if (b < 0) return;
     const SeqInfo s = seq_info(a, b);
     const int limit = min(s.len, s.len - s.nq + (t - s.q0) + 1);
     const bool on[2] = {!a.merged && min(s.prefix, limit) > 0, limit > (a.merged ? 0 : s.prefix)};
-    float M = -INFINITY, L = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    // first token of the row block that the prefix's CTAs share
+    const int q0 = on[0] ? (a.qstarts ? start_at(a.qstarts, s.first, a.T, a.err) : s.first) : 0;
     const bool live = lane * 4 < a.D;
+    const int h1 = min(a.H, (int)(blockIdx.y + 1) * heads);
+    for (int h = blockIdx.y * heads + (threadIdx.x >> 5); h < h1; h += 4) {
+        const int64_t row = (int64_t)t * a.H + h;
+        float4 st[2];
+        if (on[0]) st[0] = prefix.stat[row];
+        if (on[1]) st[1] = rest.stat[row];
+        float M = -INFINITY, L = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        bool written = false;
 #pragma unroll
-    for (int kind = 0; kind < 2; ++kind) {
-        if (!on[kind]) continue;
-        const PartArgs& p = kind ? rest : prefix;
-        const float4 st = p.stat[row];
-        const int c0 = __float_as_int(st.z), c1 = __float_as_int(st.w);
-        if (c0 < 0 || c1 < c0 || c1 >= p.ctas) {  // start arrays that contradict each other: no CTA had the row
-            *a.err = kErrIndex;
-            continue;
-        }
-        if (kind == 1 && !on[0] && c0 == c1) return;  // written by the CTA that had all of it
-        // row of the block that the CTAs share (its first token is the entry's)
-        int q0 = s.q0;
-        if (kind == 0 && a.qstarts) q0 = start_at(a.qstarts, s.first, a.T, a.err);
-        else if (kind == 0) q0 = s.first;
-        const int r = (int)((((int64_t)max(0, t - q0)) * a.G + h % a.G) % p.slot_rows);
-        const float* first = p.head + (p.by_row ? row : (int64_t)c0 * p.slot_rows + r) * a.D;
-        for (int base = c0; base <= c1; base += 32) {
-            const int c = base + lane;
-            float m = -INFINITY, l = 0.0f;
-            if (c <= c1) {
-                if (c == c0) {
-                    m = st.x;
-                    l = st.y;
-                } else {
-                    const float2 v = p.tail_stat[(int64_t)c * p.slot_rows + r];
-                    m = v.x;
-                    l = v.y;
+        for (int kind = 0; kind < 2; ++kind) {
+            if (!on[kind]) continue;
+            const PartArgs& p = kind ? rest : prefix;
+            const int c0 = __float_as_int(st[kind].z), c1 = __float_as_int(st[kind].w);
+            if (c0 < 0 || c1 < c0 || c1 >= p.ctas) {  // start arrays that contradict each other: no CTA had the row
+                *a.err = kErrIndex;
+                continue;
+            }
+            if (kind == 1 && !on[0] && c0 == c1) {  // written by the CTA that had all of it
+                written = true;
+                continue;
+            }
+            const int r = (int)(((int64_t)max(0, t - (kind ? s.q0 : q0)) * a.G + h % a.G) % p.slot_rows);
+            const float* first = p.head + (p.by_row ? row : (int64_t)c0 * p.slot_rows + r) * a.D;
+            for (int base = c0; base <= c1; base += 32) {
+                const int c = base + lane;
+                float m = -INFINITY, l = 0.0f;
+                if (c <= c1) {
+                    if (c == c0) {
+                        m = st[kind].x;
+                        l = st[kind].y;
+                    } else {
+                        const float2 v = p.tail_stat[(int64_t)c * p.slot_rows + r];
+                        m = v.x;
+                        l = v.y;
+                    }
+                }
+                const float mx = fmaxf(M, warp_max(m));
+                if (mx == -INFINITY) continue;
+                const float keep = M == -INFINITY ? 0.0f : exp2_fast(M - mx);
+                const float w = m == -INFINITY ? 0.0f : exp2_fast(m - mx);
+                M = mx;
+                L = L * keep + warp_sum(l * w);
+                o.x *= keep;
+                o.y *= keep;
+                o.z *= keep;
+                o.w *= keep;
+                const int n = min(32, c1 - base + 1);
+#pragma unroll 8
+                for (int i = 0; i < n; ++i) {
+                    const float wi = __shfl_sync(0xffffffffu, w, i);
+                    const float* src = base + i == c0 ? first : p.tail + ((int64_t)(base + i) * p.slot_rows + r) * a.D;
+                    if (live) {
+                        const float4 v = *reinterpret_cast<const float4*>(src + lane * 4);
+                        o.x = fmaf(v.x, wi, o.x);
+                        o.y = fmaf(v.y, wi, o.y);
+                        o.z = fmaf(v.z, wi, o.z);
+                        o.w = fmaf(v.w, wi, o.w);
+                    }
                 }
             }
-            const float mx = fmaxf(M, warp_max(m));
-            if (mx == -INFINITY) continue;
-            const float keep = M == -INFINITY ? 0.0f : exp2_fast(M - mx);
-            const float w = m == -INFINITY ? 0.0f : exp2_fast(m - mx);
-            M = mx;
-            L = L * keep + warp_sum(l * w);
-            o.x *= keep;
-            o.y *= keep;
-            o.z *= keep;
-            o.w *= keep;
-            const int n = min(32, c1 - base + 1);
-#pragma unroll 4
-            for (int i = 0; i < n; ++i) {
-                const float wi = __shfl_sync(0xffffffffu, w, i);
-                const float* src = base + i == c0 ? first : p.tail + ((int64_t)(base + i) * p.slot_rows + r) * a.D;
-                if (live) {
-                    const float4 v = *reinterpret_cast<const float4*>(src + lane * 4);
-                    o.x = fmaf(v.x, wi, o.x);
-                    o.y = fmaf(v.y, wi, o.y);
-                    o.z = fmaf(v.z, wi, o.z);
-                    o.w = fmaf(v.w, wi, o.w);
-                }
-            }
         }
-    }
-    if (!live) return;
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    TQ* dst = static_cast<TQ*>(a.out) + row * a.D + lane * 4;
-    if constexpr (sizeof(TQ) == 4) {
-        *reinterpret_cast<float4*>(dst) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    } else {
-        *reinterpret_cast<uint2*>(dst) = make_uint2(Half2Of<T16>::pack(o.x * inv, o.y * inv), Half2Of<T16>::pack(o.z * inv, o.w * inv));
+        if (!live || written) continue;
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        TQ* dst = static_cast<TQ*>(a.out) + row * a.D + lane * 4;
+        if constexpr (sizeof(TQ) == 4) {
+            *reinterpret_cast<float4*>(dst) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        } else {
+            *reinterpret_cast<uint2*>(dst) = make_uint2(Half2Of<T16>::pack(o.x * inv, o.y * inv), Half2Of<T16>::pack(o.z * inv, o.w * inv));
+        }
     }
 }
 
@@ -486,10 +493,13 @@ void launch_paged_decode(const PagedArgs& a, const PartArgs& rest, int32_t tq, i
 }
 
 void launch_paged_combine(const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, int32_t tq, cudaStream_t s) {
-    const dim3 grid((unsigned)(((int64_t)a.T * a.H + 3) / 4));
-    if (tq == BEACON_CUDA_DTYPE_F32) launch_kernel(paged_combine_kernel<float, __half>, grid, dim3(128), 0, s, true, a, prefix, rest);
-    else if (tq == BEACON_CUDA_DTYPE_F16) launch_kernel(paged_combine_kernel<__half, __half>, grid, dim3(128), 0, s, true, a, prefix, rest);
-    else launch_kernel(paged_combine_kernel<__nv_bfloat16, __nv_bfloat16>, grid, dim3(128), 0, s, true, a, prefix, rest);
+    // four heads a block (one a warp) until the device is full, then more
+    const int64_t blocks = (int64_t)a.T * ((a.H + 3) / 4);
+    const int heads = (int)std::min<int64_t>((a.H + 3) / 4, std::max<int64_t>(1, blocks / 2048)) * 4;
+    const dim3 grid((unsigned)a.T, (unsigned)((a.H + heads - 1) / heads));
+    if (tq == BEACON_CUDA_DTYPE_F32) launch_kernel(paged_combine_kernel<float, __half>, grid, dim3(128), 0, s, true, a, prefix, rest, heads);
+    else if (tq == BEACON_CUDA_DTYPE_F16) launch_kernel(paged_combine_kernel<__half, __half>, grid, dim3(128), 0, s, true, a, prefix, rest, heads);
+    else launch_kernel(paged_combine_kernel<__nv_bfloat16, __nv_bfloat16>, grid, dim3(128), 0, s, true, a, prefix, rest, heads);
 }
 
 }  // namespace bc

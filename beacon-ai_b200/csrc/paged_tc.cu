@@ -19,7 +19,7 @@
 // lie where the scores were, and are the A operand of O += P V from tensor
 // memory; V is read N-major.
 // Key and value rows come in page by page by tensor copies (TMA) of up to 128
-// rows into a ring of tiles in the 128-byte swizzle, requested by one warp;
+// rows into a ring of tiles in the 128-byte swizzle, requested by four warps;
 // rows of a value tile that are no keys of the block are zeroed there (their
 // weights are zero, but what a page holds behind its last row may be no
 // number). 16-byte asynchronous copies by four warps, which zero-fill, serve
@@ -431,9 +431,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             ok = __all_sync(0xffffffffu, ok);  // the lanes copy for each other: they go on or give up together
             return ok;
         };
-        // Rows pos0 + lane of a tile (of 32) one by one, 16 bytes a lane
-        auto copy_rows = [&](const Piece& p, const void* cache, int r0, int row) {
-            const uint32_t dst = smem_u32(ring + (size_t)(it % NST) * SM::tile) + (c >> 3) * (kTile * 128);
+        // 32 rows of a tile one by one, 16 bytes a lane; each lane knows one cache row
+        auto copy_rows = [&](uint32_t dst, const Piece& p, const void* cache, int r0, int row) {
+            dst += (c >> 3) * (kTile * 128);
             const uint8_t* src = static_cast<const uint8_t*>(cache) + (p.kvh * a.D + c * 8) * 2;
 #pragma unroll 8
             for (int i = 0; i < 32 / RPI; ++i) {
@@ -447,11 +447,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         auto load_tile = [&](const Piece& p, int f, int page) {
             bool value;
             const int t = key_tile(p, f, value);
-            if (a.box && pw > 0) return;
             if (!room()) return;
             const int pos = pos_of(p, t);
             if (!a.box) {
-                copy_rows(p, value ? a.cv : a.ck, pw * 32, pos < p.k.key1 ? (int)page_row(a, page, pos) : -1);
+                copy_rows(smem_u32(ring + (size_t)(it % NST) * SM::tile), p, value ? a.cv : a.ck, pw * 32, pos < p.k.key1 ? (int)page_row(a, page, pos) : -1);
                 cp_async_commit();
                 ++it;
                 if (it - told > 2) {  // two tiles stay in flight
@@ -460,15 +459,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 return;
             }
-            const int st = it % NST;
+            const int st = it++ % NST;
             const int pos0 = p.k.base + (p.tile + t) * kTile;
             const uint32_t dst = smem_u32(ring + (size_t)st * SM::tile);
-            const bool mine = lane * a.box < kTile && pos < p.k.key1;
-            if (__any_sync(0xffffffffu, mine && pos < p.k.cut && pos + a.box > p.k.cut)) {
+            const bool live = lane * a.box < kTile && pos < p.k.key1;
+            if (__any_sync(0xffffffffu, live && pos < p.k.cut && pos + a.box > p.k.cut)) {
                 // a box whose rows lie in two tables: this tile row by row
+                if (pw > 0) return;
                 for (int r0 = 0; r0 < kTile; r0 += 32) {
                     const int q = pos0 + r0 + lane;
-                    copy_rows(p, value ? a.cv : a.ck, r0,
+                    copy_rows(dst, p, value ? a.cv : a.ck, r0,
                               q < p.k.key1 ? (int)page_row(a, page_id(a, q < p.k.cut ? p.k.first : p.k.b, q), q) : -1);
                 }
                 cp_async_commit();
@@ -476,16 +476,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) arrive(&full_bar[st]);
-                ++it;
                 return;
             }
             // a value tile with rows that are no keys lands on fix_bar first
             const bool part = value && (pos0 < p.k.key0 || pos0 + kTile > p.k.key1);
+            if (part && pw > 0) return;
             uint64_t* bar = part ? &fix_bar : &full_bar[st];
-            const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
-            if (lane == 0) mbar_expect_tx(bar, (uint32_t)(boxes * a.box * DP * 2));
-            __syncwarp();
-            if (mine) {
+            const int boxes = __popc(__ballot_sync(0xffffffffu, live));
+            // one arrival and all bytes from the first warp; the copies, whose
+            // requests take a hundred cycles each, from all four
+            if (pw == 0 && lane == 0) mbar_expect_tx(bar, (uint32_t)(boxes * a.box * DP * 2));
+            if (live && (part || lane % kLoadWarps == pw)) {
                 int64_t row = page_row(a, page, pos);
                 if (row < 0) row = a.pages * a.page_size;  // outside: zeros
 #pragma unroll
@@ -507,7 +508,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 ok = __all_sync(0xffffffffu, ok);
                 if (lane == 0) arrive(&full_bar[st]);
             }
-            ++it;
         };
         int seg = 0;
         for (Piece p = pc; ok && p.u < u1; p.next(a, BR, u1), ++seg) {
