@@ -5,6 +5,7 @@
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -163,9 +164,9 @@ PartArgs carve_part(Carve& c, const PagedArgs& a, int ctas, int slot_rows, bool 
     return p;
 }
 
-// [pages * page_size][Hkv][D] in boxes of `box` rows by 64 values of one head,
+// [pages * page_size][Hkv][D] in boxes of box_rows rows by 64 values of one head,
 // 128-byte swizzle; values past D and rows past the end arrive as zeros.
-CUtensorMap cache_map(const PagedArgs& a, const void* cache, int32_t tk) {
+CUtensorMap cache_map(const PagedArgs& a, const void* cache, int32_t tk, int box_rows) {
     static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
@@ -176,7 +177,7 @@ CUtensorMap cache_map(const PagedArgs& a, const void* cache, int32_t tk) {
     CUtensorMap map;
     const cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)a.Hkv, (cuuint64_t)a.pages * (cuuint64_t)a.page_size};
     const cuuint64_t strides[2] = {(cuuint64_t)a.D * 2, (cuuint64_t)a.Hkv * (cuuint64_t)a.D * 2};
-    const cuuint32_t box[3] = {64, 1, (cuuint32_t)a.box};
+    const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows};
     const cuuint32_t es[3] = {1, 1, 1};
     const CUresult r = encode(&map, tk == BEACON_CUDA_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
                               const_cast<void*>(cache), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -195,7 +196,7 @@ void run_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream, Paged
         a.merged = a.qstarts && (int64_t)a.T * a.G >= 128LL * a.B;
         const bool by_row = a.gstarts && !a.merged;
         const PagedTcPlan plan = tc ? plan_paged_tc(ctx, a, split, !decode) : PagedTcPlan{};
-        const int dctas = decode ? paged_decode_ctas(ctx, a, split) : 0;
+        const int dctas = decode ? paged_decode_ctas(ctx, a) : 0;
         PartArgs prefix, rest;
         auto carve = [&](uint8_t* base) {
             Carve c(base);
@@ -205,19 +206,20 @@ void run_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream, Paged
         };
         CallScratch scratch(ctx, stream, carve(nullptr));
         carve(scratch.data());
-        CacheMaps maps{};
+        CacheMaps maps{}, dmaps{};
         if (a.pages > 0 && a.page_size % 8 == 0) {
             a.box = 8;
             while (a.box < 128 && a.page_size % (2 * a.box) == 0) a.box *= 2;
-            maps.k = cache_map(a, a.ck, tk);
-            maps.v = cache_map(a, a.cv, tk);
+            if (tc) maps = {cache_map(a, a.ck, tk, a.box), cache_map(a, a.cv, tk, a.box)};
+            const int rows = std::min(a.box, kDecodeBox);
+            if (decode) dmaps = {cache_map(a, a.ck, tk, rows), cache_map(a, a.cv, tk, rows)};
         }
         bool pdl = !scratch.of_graph();  // a graph's allocation comes first
         if (tc) {
             launch_paged_tc(plan, a, maps, prefix, rest, tq, tk, stream->s, pdl);
             pdl = true;
         }
-        if (decode) launch_paged_decode(a, rest, tq, tk, stream->s, pdl);
+        if (decode) launch_paged_decode(a, dmaps, rest, tq, tk, stream->s, pdl, tc);
         launch_paged_combine(a, prefix, rest, tq, stream->s);
         return;
     }

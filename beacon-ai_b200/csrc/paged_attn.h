@@ -36,34 +36,66 @@ struct PagedArgs {
 // prefix (kind 0) and its own sequence's rows behind it (kind 1). Each part is
 // cut into key tiles; the tiles of all rows form one line that the CTAs of a
 // launch share evenly, so a row's tiles may lie with several neighbouring
-// CTAs. The CTA that has the first of them leaves (m, l, first CTA, last CTA)
+// CTAs. The CTA that has the first of them leaves m, l and where the parts are
 // in `stat` and its sums in `head`; the CTAs after it, each of which has at
 // most one such row block, leave theirs under their own number in `tail`.
 // m is the largest score times log2(e), l the sum of 2^(score - m), and the
-// sums are of 2^(score - m) v.
+// sums are of 2^(score - m) v. Every row has an entry of kind 1, also one that
+// sees no key.
 struct PartArgs {
-    float4* stat = nullptr;   // [T * H]: m, l and, as integers, the CTAs
+    float4* stat = nullptr;   // [T * H]: m, l, PartPlace
     float* head = nullptr;    // [T * H][D], or [ctas][slot_rows][D] when !by_row
     float2* tail_stat = nullptr;  // [ctas][slot_rows]
     float* tail = nullptr;        // [ctas][slot_rows][D]
     int by_row = 0;    // heads are kept per row: a row has both kinds
-    int slot_rows = 0;  // rows of a row block
-    int ctas = 0;
+    int slot_rows = 0;  // rows of a row block, at most 256
+    int ctas = 0;       // at most 4096
 };
-
-// CTAs that take part (each then has a tile, so those between two that share a
-// row have a part of it), the share of CTA c of the line of `total` tiles, and
-// the CTA that holds tile u.
-__device__ __forceinline__ int sharers(long long total, int ctas) { return total < ctas ? (int)total : ctas; }
-__device__ __forceinline__ long long share_begin(long long total, int ctas, int c) { return total * c / ctas; }
-__device__ __forceinline__ int share_of(long long total, int ctas, long long u) {
-    return (int)(((u + 1) * ctas - 1) / total);
+// The CTAs [c0, c1] that have a row's parts, its row in their slots, and
+// whether it has a part of kind 0 as well.
+struct PartPlace {
+    int c0, c1, row;
+    bool prefix;
+};
+__device__ __forceinline__ float4 pack_stat(float m, float l, const PartPlace& p) {
+    return make_float4(m, l, __int_as_float(p.c0 | p.row << 16), __int_as_float(p.c1 | (p.prefix ? 1 << 16 : 0)));
 }
+__device__ __forceinline__ PartPlace place_of(const float4& s) {
+    const int a = __float_as_int(s.z), b = __float_as_int(s.w);
+    return PartPlace{a & 0xFFFF, b & 0xFFFF, (a >> 16) & 0xFF, (b >> 16 & 1) != 0};
+}
+
+// Even shares of a line of `total` tiles: the first `more` CTAs have q + 1
+// tiles, the others q. At most one CTA per tile takes part, so that every CTA
+// between two that share a row has a part of it.
+struct Shares {
+    int ctas = 0, more = 0;
+    long long q = 0;
+    __device__ __forceinline__ Shares(long long total, int n) {
+        ctas = total < n ? (int)total : n;
+        if (ctas == 0) return;
+        q = total >> 31 ? total / ctas : (long long)((uint32_t)total / (uint32_t)ctas);
+        more = (int)(total - q * ctas);
+    }
+    __device__ __forceinline__ long long begin(int c) const { return q * c + min(c, more); }
+    __device__ __forceinline__ int of(long long u) const {  // the CTA that has tile u
+        const long long cut = (q + 1) * more;
+        if (u < cut) return (u >> 31) | ((q + 1) >> 31) ? (int)(u / (q + 1)) : (int)((uint32_t)u / (uint32_t)(q + 1));
+        u -= cut;
+        return more + ((u >> 31) | (q >> 31) ? (int)(u / q) : (int)((uint32_t)u / (uint32_t)q));
+    }
+};
 
 // Launchers. `prefix`/`rest`: kinds 0 and 1.
 constexpr int kDecodeMaxGroup = 16;  // query heads of one KV head that paged_decode_kernel holds
-int paged_decode_ctas(const BeaconCudaContext* ctx, const PagedArgs& a, bool split);
-void launch_paged_decode(const PagedArgs& a, const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s, bool pdl);
+struct CacheMaps {  // tensor maps of the caches: boxes of some rows by 64 values of one head
+    CUtensorMap k, v;
+};
+constexpr int kDecodeBox = 16;  // most rows of a copy box of paged_decode_kernel
+int paged_decode_ctas(const BeaconCudaContext* ctx, const PagedArgs& a);
+// after_tc: the launch before it is paged_tc_kernel of the same call.
+void launch_paged_decode(const PagedArgs& a, const CacheMaps& maps, const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s,
+                         bool pdl, bool after_tc);
 // Rows of a block and CTAs of the tensor-core kernel (paged_tc.cu), for the
 // prefixes and, when with_rest, the rest of every sequence.
 struct PagedTcPlan {
@@ -73,19 +105,35 @@ struct PagedTcPlan {
     int ctas = 0;
 };
 PagedTcPlan plan_paged_tc(const BeaconCudaContext* ctx, const PagedArgs& a, bool split, bool with_rest);
-struct CacheMaps {  // tensor maps of the caches (PagedArgs::box rows by 64 values of one head)
-    CUtensorMap k, v;
-};
 void launch_paged_tc(const PagedTcPlan& plan, const PagedArgs& a, const CacheMaps& maps, const PartArgs& prefix,
                      const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s, bool pdl);
 void launch_paged_combine(const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, int32_t tq, cudaStream_t s);
 
-// A start array entry kept inside [0, n] (callers hold it in a device tensor).
-__device__ __forceinline__ int start_at(const int32_t* s, int i, int n, int* err) {
-    const int v = s[i];
-    if (v >= 0 && v <= n) return v;
-    *err = kErrIndex;
-    return v < 0 ? 0 : n;
+// Values that callers hold in device tensors are kept inside their ranges; one
+// outside marks the stream's error word. Loads come before the checks so that
+// independent ones are in flight together.
+__device__ __forceinline__ int keep_in(int v, long long most, bool& bad) {
+    if (v >= 0 && v <= most) return v;
+    bad = true;
+    return v < 0 ? 0 : (int)most;
+}
+__device__ __forceinline__ long long capacity(const PagedArgs& a) { return (long long)a.max_pages * a.page_size; }
+
+// Asks for the index arrays before anything reads them, so that the first use
+// of each (one depends on another) does not wait for memory in turn. Requests
+// only: what an earlier kernel still writes is read after pdl_wait.
+__device__ __forceinline__ void prefetch_indices(const PagedArgs& a) {
+    auto ask = [](const int32_t* p, long long n) {
+        for (long long i = threadIdx.x * 32LL; i < n && i < 32LL * 2 * blockDim.x; i += 32LL * blockDim.x)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
+    };
+    ask(a.lens, a.B);
+    if (a.qstarts) ask(a.qstarts, a.B + 1);
+    if (a.gstarts) {
+        ask(a.gstarts, a.groups + 1);
+        ask(a.prefix, a.groups);
+    }
+    ask(a.table, (long long)a.B * a.max_pages);
 }
 
 // The i with starts[i] <= x < starts[i + 1] of an ascending array of n + 1
@@ -94,10 +142,10 @@ __device__ __forceinline__ int span_of(const int32_t* starts, int n, int x) {
     int lo = 0, hi = n;  // the last i with starts[i] <= x lies in [lo, hi)
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (starts[mid] <= x) lo = mid;
+        if (__ldg(starts + mid) <= x) lo = mid;
         else hi = mid;
     }
-    return n > 0 && starts[lo] <= x && x < starts[lo + 1] ? lo : -1;
+    return n > 0 && __ldg(starts + lo) <= x && x < __ldg(starts + lo + 1) ? lo : -1;
 }
 
 // Rows that sequence b holds, its queries and the prefix it shares.
@@ -108,46 +156,34 @@ struct SeqInfo {
     int first = 0;
 };
 
-__device__ __forceinline__ int kv_len(const PagedArgs& a, int b) {
-    const int len = a.lens[b];
-    const long long cap = (long long)a.max_pages * a.page_size;
-    if (len >= 0 && len <= cap) return len;
-    *a.err = kErrIndex;
-    return len < 0 ? 0 : (int)cap;
-}
-
-__device__ __forceinline__ int prefix_len(const PagedArgs& a, int g) {
-    const int p = a.prefix[g];
-    const long long cap = (long long)a.max_pages * a.page_size;
-    if (p >= 0 && p <= cap) return p;
-    *a.err = kErrIndex;
-    return p < 0 ? 0 : (int)cap;
-}
-
 __device__ __forceinline__ SeqInfo seq_info(const PagedArgs& a, int b) {
     SeqInfo s;
-    s.len = kv_len(a, b);
+    bool bad = false;
+    const int len = __ldg(a.lens + b);
+    int q0 = b, q1 = b + 1;
     if (a.qstarts) {
-        s.q0 = start_at(a.qstarts, b, a.T, a.err);
-        s.nq = start_at(a.qstarts, b + 1, a.T, a.err) - s.q0;
-        if (s.nq < 0) {
-            *a.err = kErrIndex;
-            s.nq = 0;
-        }
-    } else {
-        s.q0 = b;
-        s.nq = 1;
+        q0 = __ldg(a.qstarts + b);
+        q1 = __ldg(a.qstarts + b + 1);
     }
     s.first = b;
     if (a.gstarts) {
         const int g = span_of(a.gstarts, a.groups, b);
         if (g >= 0) {
-            s.first = start_at(a.gstarts, g, a.B, a.err);
-            start_at(a.gstarts, g + 1, a.B, a.err);
-            if (s.first >= a.B) s.first = b;  // cannot hold b
-            s.prefix = min(prefix_len(a, g), kv_len(a, s.first));  // no row beyond what it holds is read
+            const int lo = __ldg(a.gstarts + g), hi = __ldg(a.gstarts + g + 1), p = __ldg(a.prefix + g);
+            if (lo >= 0) s.first = lo;  // lo <= b
+            bad |= lo < 0 || hi > a.B;
+            // no row beyond what the first sequence holds is read
+            s.prefix = min(keep_in(p, capacity(a), bad), keep_in(__ldg(a.lens + s.first), capacity(a), bad));
         }
     }
+    s.len = keep_in(len, capacity(a), bad);
+    s.q0 = keep_in(q0, a.T, bad);
+    s.nq = keep_in(q1, a.T, bad) - s.q0;
+    if (s.nq < 0) {
+        bad = true;
+        s.nq = 0;
+    }
+    if (bad) *a.err = kErrIndex;
     return s;
 }
 

@@ -4,13 +4,17 @@
 // o = sum_p 2^(t_p - m) v_p / sum_p 2^(t_p - m), t_p = scale log2(e) q . k_p,
 // over the keys of a row behind its group's prefix. The G query heads of one
 // KV head share its keys, so the bound is reading the cache once. A tile is 64
-// keys, 16 for each of the 4 warps of a CTA, which brings them in with 16-byte
-// asynchronous copies through its own ring (no CTA barrier in the loop), forms
-// the scores and the value sums with m16n8k16 instructions (the G <= 16 heads
-// as rows) and keeps its own running maximum. The tiles of all sequences and
-// KV heads form one line that the CTAs share evenly (PartArgs): a batch of
-// uneven lengths loads every SM alike whatever the lengths are, and the lengths
-// may change between replays of a captured call.
+// keys, 16 for each of the 4 warps of a CTA: each brings its keys and values in
+// through its own ring (tensor copies of 8 or 16 rows, no CTA barrier in the
+// loop) and forms S^T = K Q^T (16 keys x 8 or 16 heads) and O^T += V^T P^T with
+// m16n8k16 instructions, so that few heads waste little of them. Each warp
+// keeps its own running maximum. The tiles of all sequences and KV heads form
+// one line that the CTAs share evenly (PartArgs): a batch of uneven lengths
+// loads every SM alike whatever the lengths are, and the lengths may change
+// between replays of a captured call.
+// 32-bit queries are two f16 parts (products for both), and so are the
+// weights; each tile's value sums are then added with rounding, because the
+// instruction's own sums truncate and a long chain of them would drift.
 #include <algorithm>
 #include <cmath>
 
@@ -26,17 +30,21 @@ constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kDecKeys = 16 * kDecWarps;  // keys of a tile
 
-template <int DP>
+template <int DP, int NT, bool SPLIT>
 struct DecodeSmem {
-    static constexpr int stages = DP == 128 ? 3 : 4;
-    static constexpr int sub = 16 * DP * 2;        // bytes of 16 key (or value) rows
-    static constexpr int ring = stages * 2 * sub;  // of one warp
-    // merge area: [warp][rows][DP] sums, then m and l
-    static constexpr size_t bytes(int rows) { return (size_t)kDecWarps * (ring + rows * DP * 4 + 2 * rows * 4); }
+    static constexpr int stages = DP == 128 ? 2 : 4;
+    static constexpr int part = 16 * DP * 2;        // 16 key (or value) rows: [64 values][row][128 bytes]
+    static constexpr int ring = stages * 2 * part;  // of one warp
+    static constexpr int rows = 8 * NT;             // heads, padded
+    static constexpr int q = rows * DP * 2;         // one part of the queries
+    // merge area: [warp][rows][DP] sums, then m and l [warp][rows], scales [rows]
+    static constexpr int merge = kDecWarps * rows * DP * 4;
+    static constexpr size_t bytes =
+        (size_t)kDecWarps * ring + (SPLIT ? 2 : 1) * q + merge + (2 * kDecWarps + 1) * rows * 4 + 1024;
 };
 
-struct Span {  // keys [from, to) of one sequence, in tiles
-    int from = 0, to = 0, tiles = 0;
+struct Span {  // keys [from, to) of one sequence, in tiles that begin at `base`
+    int from = 0, to = 0, base = 0, tiles = 0;
 };
 __device__ __forceinline__ Span rest_of(const PagedArgs& a, int b) {
     Span s;
@@ -44,45 +52,60 @@ __device__ __forceinline__ Span rest_of(const PagedArgs& a, int b) {
     const SeqInfo i = seq_info(a, b);
     s.from = i.prefix;
     s.to = i.len;
-    s.tiles = s.to > s.from ? (s.to - s.from + kDecKeys - 1) / kDecKeys : 0;
+    s.base = a.box ? s.from & ~(min(a.box, kDecodeBox) - 1) : s.from;
+    // a sequence without keys has a tile too: its rows are written by it
+    s.tiles = s.to > s.from ? (s.to - s.base + kDecKeys - 1) / kDecKeys : 1;
     return s;
 }
 
 // Place in the line of tiles: sequence, KV head, tile.
 struct Walk {
     int b = 0, kvh = 0, tile = 0;
-    Span cur, next;  // the sequence after b is fetched ahead of its use
+    Span cur;
     __device__ __forceinline__ void step(const PagedArgs& a) {
         if (++tile < cur.tiles) return;
         tile = 0;
         if (++kvh < a.Hkv) return;
         kvh = 0;
-        do {
-            ++b;
-            cur = next;
-            next = rest_of(a, b + 1);
-        } while (b < a.B && cur.tiles == 0);
+        cur = rest_of(a, ++b);
     }
 };
 
-template <typename TQ, typename TK, int DP, bool SPLIT>
-__global__ void __launch_bounds__(kDecThreads) paged_decode_kernel(const PagedArgs a, const PartArgs part) {
-    using S = DecodeSmem<DP>;
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {  // 8x8 matrix of 16-bit values held by a warp
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+template <typename TQ, typename TK, int DP, int NT, bool SPLIT>
+__global__ void __launch_bounds__(kDecThreads)
+    paged_decode_kernel(const PagedArgs a, const __grid_constant__ CacheMaps maps, const PartArgs part, int after_tc) {
+    using S = DecodeSmem<DP, NT, SPLIT>;
     constexpr int NS = S::stages;
-    constexpr int KSTEPS = DP / 16;
-    constexpr int CH = DP / 8;            // 16-byte chunks of a row
-    constexpr int RPI = 32 / CH;          // rows that one copy instruction of a warp covers
-    extern __shared__ __align__(128) uint8_t dec_smem[];
+    constexpr int KS = DP / 16;
+    constexpr int CH = DP / 8;   // 16-byte chunks of a row
+    constexpr int RPI = 32 / CH;  // rows that one copy instruction of a warp covers
+    extern __shared__ uint8_t dec_smem_raw[];
+    __shared__ __align__(8) uint64_t bars[kDecWarps][NS];
     __shared__ long long sums_s[kDecWarps];
     __shared__ int b_s;
     __shared__ long long before_s;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dec_smem_raw) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int rows = a.G <= 8 ? 8 : 16;   // rows of the merge area
-    uint8_t* ring = dec_smem + warp * S::ring;
-    float* merge_o = reinterpret_cast<float*>(dec_smem + kDecWarps * S::ring);  // [warp][rows][DP]
-    float* merge_m = merge_o + kDecWarps * rows * DP;                           // [warp][rows]
-    float* merge_l = merge_m + kDecWarps * rows;
-    pdl_wait();
+    const uint32_t ring = smem_u32(smem + warp * S::ring);
+    const uint32_t q_at = smem_u32(smem + kDecWarps * S::ring);
+    float* merge_o = reinterpret_cast<float*>(smem + kDecWarps * S::ring + (SPLIT ? 2 : 1) * S::q);  // [warp][rows][DP]
+    float* merge_m = merge_o + kDecWarps * S::rows * DP;                                              // [warp][rows]
+    float* merge_l = merge_m + kDecWarps * S::rows;
+    float* scale_s = merge_l + kDecWarps * S::rows;                                                    // [rows]
+    prefetch_indices(a);
+    if (lane == 0) {
+        for (int i = 0; i < NS; ++i) mbar_init(&bars[warp][i], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // After the tensor-core kernel of the same call nothing here depends on it,
+    // and it began only when what came before it was done.
+    if (!after_tc) pdl_wait();
 
     // this CTA's share of the line
     const int chunk = (a.B + kDecThreads - 1) / kDecThreads;
@@ -105,8 +128,8 @@ __global__ void __launch_bounds__(kDecThreads) paged_decode_kernel(const PagedAr
     }
     total *= a.Hkv;
     const int cta = blockIdx.x;
-    const int ctas = sharers(total, part.ctas);
-    const long long u0 = cta < ctas ? share_begin(total, ctas, cta) : 0, u1 = cta < ctas ? share_begin(total, ctas, cta + 1) : 0;
+    const Shares shares(total, part.ctas);
+    const long long u0 = cta < shares.ctas ? shares.begin(cta) : 0, u1 = cta < shares.ctas ? shares.begin(cta + 1) : 0;
     pdl_trigger();
     if (u0 < u1) {
         if (before * a.Hkv <= u0 && u0 < (before + mine) * a.Hkv) {
@@ -123,383 +146,464 @@ __global__ void __launch_bounds__(kDecThreads) paged_decode_kernel(const PagedAr
         Walk load;
         load.b = b_s;
         load.cur = rest_of(a, load.b);
-        load.next = rest_of(a, load.b + 1);
         const long long off = u0 - before_s * a.Hkv;
         load.kvh = (int)(off / load.cur.tiles);
         load.tile = (int)(off - (long long)load.kvh * load.cur.tiles);
         Walk at = load;
         const int count = (int)(u1 - u0);
-        const int rl = lane / CH, chunk16 = lane % CH;
-        const bool chunk_live = chunk16 * 8 < a.D;
+        const long long limit = g_wait_limit;
+        bool failed = false;
 
-        // this lane's key of a tile and its page (fetched a tile ahead)
-        struct Key {
-            int pos, page;  // pos -1: no key
+        // --- copies: lanes below 16 / box (one by one: below 16) have a row each
+        const int box = min(a.box, kDecodeBox);
+        const int step = a.box ? box : 1;
+        int page_next = 0;
+        auto pos_of = [&](const Walk& w) { return w.cur.base + w.tile * kDecKeys + warp * 16 + lane * step; };
+        auto fetch_page = [&](const Walk& w) {
+            const int p = pos_of(w);
+            return lane * step < 16 && p < w.cur.to ? page_id(a, w.b, p) : 0;
         };
-        auto key_of = [&](const Walk& w) {
-            const int p = w.cur.from + w.tile * kDecKeys + warp * 16 + (lane & 15);
-            Key k{-1, 0};
-            if (p < w.cur.to) k = Key{p, page_id(a, w.b, p)};
-            return k;
-        };
-        auto copy_tile = [&](int stage, int kvh, Key k) {
-            const int row = k.pos >= 0 ? (int)page_row(a, k.page, k.pos) : -1;
-            const uint32_t dst = smem_u32(ring + stage * 2 * S::sub);
+        auto copy_tile = [&](int stage, const Walk& w, int page) {
+            const int p = pos_of(w);
+            const bool live = lane * step < 16 && p < w.cur.to && p + step > w.cur.from;
+            const uint32_t dst = ring + stage * 2 * S::part;
+            const int row = live ? (int)page_row(a, page, p) : -1;
+            if (a.box) {
+                const int n = __popc(__ballot_sync(0xffffffffu, live));
+                if (lane == 0) mbar_expect_tx(&bars[warp][stage], (uint32_t)(n * box * DP * 4));
+                __syncwarp();
+                if (live) {
+                    const int y = row >= 0 ? row : (int)(a.pages * a.page_size);  // a bad page: zeros
 #pragma unroll
-            for (int i = 0; i < 16 / RPI; ++i) {
-                const int r = i * RPI + rl;
-                const int cr = __shfl_sync(0xffffffffu, row, r);
-                const bool live = cr >= 0 && chunk_live;
-                const int64_t src = live ? ((int64_t)cr * a.Hkv + kvh) * a.D + chunk16 * 8 : 0;
-                const uint32_t d = dst + r * (DP * 2) + ((chunk16 ^ (r & 7)) << 4);
-                cp_async16_zfill(d, static_cast<const TK*>(a.ck) + src, live);
-                cp_async16_zfill(d + S::sub, static_cast<const TK*>(a.cv) + src, live);
+                    for (int h = 0; h < DP / 64; ++h) {
+                        const uint32_t d = dst + h * 2048 + lane * box * 128;
+                        tma_rows(d, &maps.k, h * 64, w.kvh, y, &bars[warp][stage]);
+                        tma_rows(d + S::part, &maps.v, h * 64, w.kvh, y, &bars[warp][stage]);
+                    }
+                }
+            } else {
+                const int c = lane % CH;
+#pragma unroll
+                for (int i = 0; i < 16 / RPI; ++i) {
+                    const int r = i * RPI + lane / CH;
+                    const int cr = __shfl_sync(0xffffffffu, row, r);
+                    const bool on = cr >= 0 && c * 8 < a.D;
+                    const int64_t src = on ? ((int64_t)cr * a.Hkv + w.kvh) * a.D + c * 8 : 0;
+                    const uint32_t d = dst + (c >> 3) * 2048 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                    cp_async16_zfill(d, static_cast<const TK*>(a.ck) + src, on);
+                    cp_async16_zfill(d + S::part, static_cast<const TK*>(a.cv) + src, on);
+                }
+                cp_async_commit();
             }
         };
-        Key key_next = key_of(load);
+        // The queries of (b, kvh): thread i has 4 values of heads i / (DP / 4) + ...
+        constexpr int QV = S::rows * (DP / 4) / kDecThreads;  // float4 per thread
+        constexpr int QR = kDecThreads / (DP / 4);            // heads that the threads cover at a time
+        const int qd = (tid % (DP / 4)) * 4;
+        float4 qn[SPLIT ? QV : 1];
+        uint2 qh[SPLIT ? 1 : QV];
+        auto fetch_q = [&](int b, int kvh) {
 #pragma unroll
+            for (int i = 0; i < QV; ++i) {
+                const int g = tid / (DP / 4) + i * QR;
+                const bool on = g < a.G && qd < a.D && b < a.B;
+                const TQ* q = static_cast<const TQ*>(a.q) + ((int64_t)b * a.H + kvh * a.G + g) * a.D + qd;
+                if constexpr (SPLIT) qn[i] = on ? *reinterpret_cast<const float4*>(q) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                else qh[i] = on ? *reinterpret_cast<const uint2*>(q) : make_uint2(0, 0);
+            }
+        };
+        fetch_q(at.b, at.kvh);
+        page_next = fetch_page(load);
+#pragma unroll 1
         for (int i = 0; i < NS - 1; ++i) {
             if (i < count) {
-                copy_tile(i, load.kvh, key_next);
+                copy_tile(i, load, page_next);
                 load.step(a);
-                if (i + 1 < count) key_next = key_of(load);
+                if (i + 1 < count) page_next = fetch_page(load);
+            } else if (!a.box) {
+                cp_async_commit();
             }
-            cp_async_commit();
         }
 
-        uint32_t qf[KSTEPS][4], ql[SPLIT ? KSTEPS : 1][4];
-        float cs[2], m[2], l[2], o[DP / 8][4];
-        long long u = u0;
+        uint32_t qf[KS][2 * NT], ql[SPLIT ? KS : 1][2 * NT];
+        float cs[NT][2], m[NT][2], l[NT][2], o[KS][NT][4];
         bool fresh = true;
-        for (int j = 0; j < count; ++j, ++u) {
+        const int lr = lane & 7, mi = lane >> 3;
+#pragma unroll 1
+        for (int j = 0; j < count; ++j) {
             if (fresh) {
-                // the G query rows of (b, kvh) as A fragments (rows lane / 4 and + 8)
+                // queries to shared memory as B operands (head rows, 16-byte chunks
+                // in the order of chunk ^ row), then to registers
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int g = lane / 4 + 8 * r;
-                    const TQ* q = static_cast<const TQ*>(a.q) + ((int64_t)at.b * a.H + at.kvh * a.G + g) * a.D;
-                    float v[KSTEPS][4];
-                    float mx = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < KSTEPS; ++k)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int d = k * 16 + h * 8 + (lane & 3) * 2;
-                            const bool live = g < a.G && d < a.D;
-                            if constexpr (SPLIT) {
-                                const float2 x = live ? *reinterpret_cast<const float2*>(q + d) : make_float2(0.0f, 0.0f);
-                                v[k][2 * h] = x.x;
-                                v[k][2 * h + 1] = x.y;
-                                mx = fmaxf(mx, fmaxf(fabsf(x.x), fabsf(x.y)));
-                            } else {
-                                qf[k][r + 2 * h] = live ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
-                            }
-                        }
-                    cs[r] = a.scale * 1.4426950408889634f;
+                for (int i = 0; i < QV; ++i) {
+                    const int g = tid / (DP / 4) + i * QR;
+                    const uint32_t d = q_at + g * (DP * 2) + ((((qd >> 3) ^ (g & 7)) << 4) | ((qd & 4) << 1));
                     if constexpr (SPLIT) {
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                        float mx = fmaxf(fmaxf(fabsf(qn[i].x), fabsf(qn[i].y)), fmaxf(fabsf(qn[i].z), fabsf(qn[i].w)));
+#pragma unroll
+                        for (int s = DP / 8; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
                         float inv;
                         const float sc = query_scale(mx, inv);
-                        cs[r] *= inv;
-#pragma unroll
-                        for (int k = 0; k < KSTEPS; ++k)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h)
-                                split_f16(v[k][2 * h] * sc, v[k][2 * h + 1] * sc, qf[k][r + 2 * h], ql[k][r + 2 * h]);
-                    }
-                    m[r] = -INFINITY;
-                    l[r] = 0.0f;
-                }
-#pragma unroll
-                for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-                fresh = false;
-            }
-            cp_async_wait<NS - 2>();
-            __syncwarp();  // the tile has landed for every lane, and all have read the stage refilled next
-            if (j + NS - 1 < count) {
-                copy_tile((j + NS - 1) % NS, load.kvh, key_next);
-                load.step(a);
-                if (j + NS < count) key_next = key_of(load);
-            }
-            cp_async_commit();
-
-            const int first = at.cur.from + at.tile * kDecKeys + warp * 16;
-            if (first < at.cur.to) {
-                const uint32_t ks = smem_u32(ring + (j % NS) * 2 * S::sub), vs = ks + S::sub;
-                const int lr = lane & 7, mi = lane >> 3;
-                float sc[2][4] = {};
-#pragma unroll
-                for (int k = 0; k < KSTEPS; ++k) {
-                    uint32_t b[4];
-                    const int r = lr + (mi & 2) * 4, c = 2 * k + (mi & 1);
-                    ldsm4(b, ks + r * (DP * 2) + ((c ^ (r & 7)) << 4));
-                    mma16816<TK>(sc[0], qf[k], b[0], b[1]);
-                    mma16816<TK>(sc[1], qf[k], b[2], b[3]);
-                    if constexpr (SPLIT) {
-                        mma16816<TK>(sc[0], ql[k], b[0], b[1]);
-                        mma16816<TK>(sc[1], ql[k], b[2], b[3]);
-                    }
-                }
-                // scores of keys first + 8 n + 2 (lane % 4) + e, rows lane / 4 + 8 r
-                float mx[2] = {m[0], m[1]};
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = first + 8 * n + 2 * (lane & 3) + (e & 1);
-                        sc[n][e] = key < at.cur.to ? sc[n][e] * cs[e >> 1] : -INFINITY;
-                        mx[e >> 1] = fmaxf(mx[e >> 1], sc[n][e]);
-                    }
-                float keep[2];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-                    keep[r] = m[r] == -INFINITY ? 1.0f : exp2_fast(m[r] - mx[r]);
-                    m[r] = mx[r];
-                    l[r] *= keep[r];
-                }
-                if (__any_sync(0xffffffffu, keep[0] != 1.0f || keep[1] != 1.0f)) {
-#pragma unroll
-                    for (int n = 0; n < DP / 8; ++n) {
-                        o[n][0] *= keep[0];
-                        o[n][1] *= keep[0];
-                        o[n][2] *= keep[1];
-                        o[n][3] *= keep[1];
-                    }
-                }
-                const float ref[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-                uint32_t ph[4], pl[4];
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        sc[n][e] = exp2_fast(sc[n][e] - ref[e >> 1]);
-                        l[e >> 1] += sc[n][e];
-                    }
-                    if constexpr (SPLIT) {
-                        split_f16(sc[n][0], sc[n][1], ph[2 * n], pl[2 * n]);
-                        split_f16(sc[n][2], sc[n][3], ph[2 * n + 1], pl[2 * n + 1]);
+                        uint2 h, lo;
+                        split_f16(qn[i].x * sc, qn[i].y * sc, h.x, lo.x);
+                        split_f16(qn[i].z * sc, qn[i].w * sc, h.y, lo.y);
+                        asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(d), "r"(h.x), "r"(h.y) : "memory");
+                        asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(d + S::q), "r"(lo.x), "r"(lo.y) : "memory");
+                        if (qd == 0) scale_s[g] = a.scale * 1.4426950408889634f * inv;
                     } else {
-                        ph[2 * n] = Half2Of<TK>::pack(sc[n][0], sc[n][1]);
-                        ph[2 * n + 1] = Half2Of<TK>::pack(sc[n][2], sc[n][3]);
-                    }
-                }
-#pragma unroll
-                for (int d = 0; d < DP / 16; ++d) {
-                    uint32_t b[4];
-                    const int r = lr + (mi & 1) * 8, c = 2 * d + (mi >> 1);
-                    ldsm4_t(b, vs + r * (DP * 2) + ((c ^ (r & 7)) << 4));
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if constexpr (SPLIT) {
-                            // the instruction's sums truncate: a long chain of them would
-                            // drift, so each tile's is added with rounding
-                            float t[4] = {};
-                            mma16816<TK>(t, ph, b[2 * h], b[2 * h + 1]);
-                            mma16816<TK>(t, pl, b[2 * h], b[2 * h + 1]);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[2 * d + h][e] += t[e];
-                        } else {
-                            mma16816<TK>(o[2 * d + h], ph, b[2 * h], b[2 * h + 1]);
-                        }
-                    }
-                }
-            }
-
-            const bool last_of_head = at.tile + 1 == at.cur.tiles;
-            if (last_of_head || j + 1 == count) {
-                // join the warps' sums of (b, kvh)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-                    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-                    const int g = lane / 4 + 8 * r;
-                    if (g < a.G) {
-                        if ((lane & 3) == 0) {
-                            merge_m[warp * rows + g] = m[r];
-                            merge_l[warp * rows + g] = l[r];
-                        }
-                        float* mo = merge_o + (warp * rows + g) * DP;
-#pragma unroll
-                        for (int n = 0; n < DP / 8; ++n)
-                            *reinterpret_cast<float2*>(mo + n * 8 + 2 * (lane & 3)) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+                        asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(d), "r"(qh[i].x), "r"(qh[i].y) : "memory");
                     }
                 }
                 __syncthreads();
-                const long long tile0 = u - at.tile;  // of this head, in the line
-                const int c0 = share_of(total, ctas, tile0);
-                const int c1 = share_of(total, ctas, tile0 + at.cur.tiles - 1);
-                const bool done = c0 == c1 && at.cur.from == 0;  // no other part anywhere
-                for (int i = tid; i < a.G * DP; i += kDecThreads) {
-                    const int g = i / DP, d = i % DP;
-                    float M = merge_m[g];
 #pragma unroll
-                    for (int w = 1; w < kDecWarps; ++w) M = fmaxf(M, merge_m[w * rows + g]);
-                    float acc = 0.0f, sum = 0.0f;
+                for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int w = 0; w < kDecWarps; ++w) {
-                        const float mw = merge_m[w * rows + g];
-                        const float wt = mw == -INFINITY ? 0.0f : exp2_fast(mw - M);
-                        acc = fmaf(merge_o[(w * rows + g) * DP + d], wt, acc);
-                        sum = fmaf(merge_l[w * rows + g], wt, sum);
-                    }
-                    if (d >= a.D) continue;
-                    const int64_t row = (int64_t)at.b * a.H + at.kvh * a.G + g;
-                    if (done) {
-                        const float r = sum == 0.0f ? 0.0f : acc / sum;
-                        TQ* dst = static_cast<TQ*>(a.out) + row * a.D + d;
-                        if constexpr (sizeof(TQ) == 4) *dst = r;
-                        else if constexpr (sizeof(TK) == 2) {
-                            const uint32_t v = Half2Of<TK>::pack(r, 0.0f);
-                            *reinterpret_cast<uint16_t*>(dst) = (uint16_t)v;
+                    for (int k = 0; k < KS; k += 2) {
+                        const uint32_t src = q_at + (8 * n + lr) * (DP * 2) + (((2 * k + mi) ^ lr) << 4);
+                        uint32_t b[4];
+                        ldsm4(b, src);
+                        qf[k][2 * n] = b[0];
+                        qf[k][2 * n + 1] = b[1];
+                        qf[k + 1][2 * n] = b[2];
+                        qf[k + 1][2 * n + 1] = b[3];
+                        if constexpr (SPLIT) {
+                            ldsm4(b, src + S::q);
+                            ql[k][2 * n] = b[0];
+                            ql[k][2 * n + 1] = b[1];
+                            ql[k + 1][2 * n] = b[2];
+                            ql[k + 1][2 * n + 1] = b[3];
                         }
-                    } else if (c0 == cta) {
-                        const int64_t slot = part.by_row ? row : (int64_t)cta * part.slot_rows + g;
-                        part.head[slot * a.D + d] = acc;
-                    } else {
-                        part.tail[((int64_t)cta * part.slot_rows + g) * a.D + d] = acc;
                     }
-                    if (d == 0) {
-                        if (c0 == cta) part.stat[row] = make_float4(M, sum, __int_as_float(c0), __int_as_float(c1));
-                        else part.tail_stat[(int64_t)cta * part.slot_rows + g] = make_float2(M, sum);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        // above zero, so that a masked score (-inf) stays one
+                        cs[n][e] = fmaxf(SPLIT ? scale_s[8 * n + 2 * (lane & 3) + e] : a.scale * 1.4426950408889634f, 1e-37f);
+                        m[n][e] = -INFINITY;
+                        l[n][e] = 0.0f;
                     }
                 }
-                __syncthreads();  // the merge area is written again by the next head
+#pragma unroll
+                for (int d = 0; d < KS; ++d)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) o[d][n][0] = o[d][n][1] = o[d][n][2] = o[d][n][3] = 0.0f;
+                // the next head's are on their way meanwhile
+                if (at.kvh + 1 < a.Hkv) fetch_q(at.b, at.kvh + 1);
+                else fetch_q(at.b + 1, 0);
+                fresh = false;
+            }
+            // the stage that was read last is filled again
+            __syncwarp();
+            if (j + NS - 1 < count) {
+                copy_tile((j + NS - 1) % NS, load, page_next);
+                load.step(a);
+                if (j + NS < count) page_next = fetch_page(load);
+            } else if (!a.box) {
+                cp_async_commit();
+            }
+            const uint32_t ks = ring + (j % NS) * 2 * S::part, vs = ks + S::part;
+            const int first = at.cur.base + at.tile * kDecKeys + warp * 16;
+            if (a.box) {
+                if (!failed && !wait_bar(&bars[warp][j % NS], (uint32_t)((j / NS) & 1), limit)) {
+                    *a.err = kErrAttnWait;
+                    failed = true;
+                }
+                if (first < at.cur.from || first + 16 > at.cur.to) {
+                    // value rows that are no keys: their weights are zero, but what the
+                    // page holds there may be no number
+                    const int lo = max(0, min(16, at.cur.from - first)), hi = max(lo, min(16, at.cur.to - first));
+                    for (int i = lane; i < (lo + 16 - hi) * CH; i += 32) {
+                        const int q = i / CH, r = q < lo ? q : hi + q - lo, c = i % CH;
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(vs + (c >> 3) * 2048 + r * 128 + ((c & 7) << 4)), "r"(0) : "memory");
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before a copy overwrites them
+                }
+            } else {
+                cp_async_wait<NS - 1>();
+            }
+            __syncwarp();
+
+            if (first < at.cur.to && first + 16 > at.cur.from) {
+                float sc[NT][4] = {};
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    uint32_t ka[4];
+                    const int r = lr + (mi & 1) * 8, c = 2 * k + (mi >> 1);
+                    ldsm4(ka, ks + (c >> 3) * 2048 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma16816<TK>(sc[n], ka, qf[k][2 * n], qf[k][2 * n + 1]);
+                        if constexpr (SPLIT) mma16816<TK>(sc[n], ka, ql[k][2 * n], ql[k][2 * n + 1]);
+                    }
+                }
+                // keys first + lane / 4 (and + 8), heads 8 n + 2 (lane % 4) + e
+                const int k0 = first + lane / 4;
+                const bool on0 = k0 >= at.cur.from && k0 < at.cur.to, on1 = k0 + 8 >= at.cur.from && k0 + 8 < at.cur.to;
+                uint32_t ph[NT][2], pl[SPLIT ? NT : 1][2];
+                bool moved = false;
+                float keep[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float ref[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        sc[n][e] = on0 ? sc[n][e] * cs[n][e] : -INFINITY;
+                        sc[n][2 + e] = on1 ? sc[n][2 + e] * cs[n][e] : -INFINITY;
+                        float mx = fmaxf(sc[n][e], sc[n][2 + e]);
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        mx = fmaxf(mx, m[n][e]);
+                        keep[n][e] = m[n][e] == -INFINITY ? 1.0f : exp2_fast(m[n][e] - mx);  // nothing summed yet: nothing to scale
+                        moved |= keep[n][e] != 1.0f;
+                        m[n][e] = mx;
+                        ref[e] = mx == -INFINITY ? 0.0f : mx;
+                        sc[n][e] = exp2_fast(sc[n][e] - ref[e]);
+                        sc[n][2 + e] = exp2_fast(sc[n][2 + e] - ref[e]);
+                        l[n][e] = l[n][e] * keep[n][e] + (sc[n][e] + sc[n][2 + e]);
+                    }
+                    if constexpr (SPLIT) {
+                        split_f16(sc[n][0], sc[n][1], ph[n][0], pl[n][0]);
+                        split_f16(sc[n][2], sc[n][3], ph[n][1], pl[n][1]);
+                        pl[n][0] = transpose8(pl[n][0]);
+                        pl[n][1] = transpose8(pl[n][1]);
+                    } else {
+                        ph[n][0] = Half2Of<TK>::pack(sc[n][0], sc[n][1]);
+                        ph[n][1] = Half2Of<TK>::pack(sc[n][2], sc[n][3]);
+                    }
+                    ph[n][0] = transpose8(ph[n][0]);
+                    ph[n][1] = transpose8(ph[n][1]);
+                }
+                if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                    for (int d = 0; d < KS; ++d)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[d][n][e] *= keep[n][e & 1];
+                }
+#pragma unroll
+                for (int d = 0; d < KS; ++d) {
+                    uint32_t va[4];
+                    const int r = lr + (mi >> 1) * 8, c = 2 * d + (mi & 1);
+                    ldsm4_t(va, vs + (c >> 3) * 2048 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        if constexpr (SPLIT) {
+                            float t[4] = {};
+                            mma16816<TK>(t, va, ph[n][0], ph[n][1]);
+                            mma16816<TK>(t, va, pl[n][0], pl[n][1]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[d][n][e] += t[e];
+                        } else {
+                            mma16816<TK>(o[d][n], va, ph[n][0], ph[n][1]);
+                        }
+                    }
+                }
+            }
+
+            if (at.tile + 1 == at.cur.tiles || j + 1 == count) {
+                // join the warps' sums of (b, kvh)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float x = l[n][e];
+                        x += __shfl_xor_sync(0xffffffffu, x, 4);
+                        x += __shfl_xor_sync(0xffffffffu, x, 8);
+                        x += __shfl_xor_sync(0xffffffffu, x, 16);
+                        const int g = 8 * n + 2 * (lane & 3) + e;
+                        if (lane < 4) {
+                            merge_m[warp * S::rows + g] = m[n][e];
+                            merge_l[warp * S::rows + g] = x;
+                        }
+                        float* mo = merge_o + (warp * S::rows + g) * DP + lane / 4;
+                        if (g < a.G) {
+#pragma unroll
+                            for (int d = 0; d < KS; ++d) {
+                                mo[16 * d] = o[d][n][e];
+                                mo[16 * d + 8] = o[d][n][2 + e];
+                            }
+                        }
+                    }
+                __syncthreads();
+                const long long tile0 = u0 + j - at.tile;  // of this head, in the line
+                const int c0 = shares.of(tile0), c1 = shares.of(tile0 + at.cur.tiles - 1);
+                const bool done = c0 == c1 && at.cur.from == 0;  // no other part anywhere
+                for (int g = tid / (DP / 4); g < a.G; g += QR) {
+                    float mw[kDecWarps], M = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < kDecWarps; ++w) {
+                        mw[w] = merge_m[w * S::rows + g];
+                        M = fmaxf(M, mw[w]);
+                    }
+                    float sum = 0.0f;
+                    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (int w = 0; w < kDecWarps; ++w) {
+                        const float wt = mw[w] == -INFINITY ? 0.0f : exp2_fast(mw[w] - M);
+                        const float4 v = *reinterpret_cast<const float4*>(merge_o + (w * S::rows + g) * DP + qd);
+                        acc.x = fmaf(v.x, wt, acc.x);
+                        acc.y = fmaf(v.y, wt, acc.y);
+                        acc.z = fmaf(v.z, wt, acc.z);
+                        acc.w = fmaf(v.w, wt, acc.w);
+                        sum = fmaf(merge_l[w * S::rows + g], wt, sum);
+                    }
+                    if (qd >= a.D) continue;
+                    const int64_t row = (int64_t)at.b * a.H + at.kvh * a.G + g;
+                    const int64_t slot = (int64_t)cta * part.slot_rows + g;
+                    if (done) {
+                        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                        TQ* dst = static_cast<TQ*>(a.out) + row * a.D + qd;
+                        if constexpr (SPLIT)
+                            *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+                        else
+                            *reinterpret_cast<uint2*>(dst) =
+                                make_uint2(Half2Of<TK>::pack(acc.x * inv, acc.y * inv), Half2Of<TK>::pack(acc.z * inv, acc.w * inv));
+                    } else {
+                        float* dst = c0 == cta ? part.head + (part.by_row ? row : slot) * a.D : part.tail + slot * a.D;
+                        *reinterpret_cast<float4*>(dst + qd) = acc;
+                    }
+                    if (qd == 0) {
+                        if (c0 == cta) part.stat[row] = pack_stat(M, sum, PartPlace{c0, c1, g, at.cur.from > 0});
+                        else part.tail_stat[slot] = make_float2(M, sum);
+                    }
+                }
+                __syncthreads();  // the merge area and the queries are written again
                 fresh = true;
             }
             at.step(a);
         }
-        cp_async_wait<0>();
+        if (a.box) {
+            // a wait that gave up: nothing may land after the CTA has ended
+            if (failed)
+                for (int i = max(0, count - NS); i < count; ++i) mbar_drain(&bars[warp][i % NS], (uint32_t)((i / NS) & 1));
+        } else {
+            cp_async_wait<0>();
+        }
     }
     // kernels launched after this one count on everything before it
     pdl_wait();
 }
 
-// The parts of the query rows of one token: both kinds, each a first part and
-// those of the CTAs after it. A warp takes a head at a time; the token's place
-// is worked out once for the block's heads.
+// The parts of the query rows: kind 1, kind 0 where the row has it, each a
+// first part and those of the CTAs after it. One warp per row. What is where
+// stands in the row's entry, so nothing else has to be looked up first.
 template <typename TQ, typename T16>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const PagedArgs a, const PartArgs prefix, const PartArgs rest, int heads) {
+__global__ void __launch_bounds__(128) paged_combine_kernel(const PagedArgs a, const PartArgs prefix, const PartArgs rest) {
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     pdl_wait();
-    const int t = blockIdx.x;
-    const int b = a.qstarts ? span_of(a.qstarts, a.B, t) : t;
-    if (b < 0) return;
-    const SeqInfo s = seq_info(a, b);
-    const int limit = min(s.len, s.len - s.nq + (t - s.q0) + 1);
-    const bool on[2] = {!a.merged && min(s.prefix, limit) > 0, limit > (a.merged ? 0 : s.prefix)};
-    // first token of the row block that the prefix's CTAs share
-    const int q0 = on[0] ? (a.qstarts ? start_at(a.qstarts, s.first, a.T, a.err) : s.first) : 0;
+    if (row >= (int64_t)a.T * a.H) return;
+    float4 st[2];
+    st[1] = rest.stat[row];
+    st[0] = rest.by_row ? prefix.stat[row] : st[1];
+    if (a.qstarts) {  // rows of no sequence are not written
+        const int t = (int)(row / a.H);
+        if (t < __ldg(a.qstarts) || t >= __ldg(a.qstarts + a.B)) return;
+    }
+    const PartPlace place = place_of(st[1]);
+    const bool both = rest.by_row && place.prefix;
+    if (!both && place.c0 == place.c1) return;  // written by the CTA that had all of it
     const bool live = lane * 4 < a.D;
-    const int h1 = min(a.H, (int)(blockIdx.y + 1) * heads);
-    for (int h = blockIdx.y * heads + (threadIdx.x >> 5); h < h1; h += 4) {
-        const int64_t row = (int64_t)t * a.H + h;
-        float4 st[2];
-        if (on[0]) st[0] = prefix.stat[row];
-        if (on[1]) st[1] = rest.stat[row];
-        float M = -INFINITY, L = 0.0f;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        bool written = false;
+    float M = -INFINITY, L = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int kind = 0; kind < 2; ++kind) {
-            if (!on[kind]) continue;
-            const PartArgs& p = kind ? rest : prefix;
-            const int c0 = __float_as_int(st[kind].z), c1 = __float_as_int(st[kind].w);
-            if (c0 < 0 || c1 < c0 || c1 >= p.ctas) {  // start arrays that contradict each other: no CTA had the row
-                *a.err = kErrIndex;
-                continue;
-            }
-            if (kind == 1 && !on[0] && c0 == c1) {  // written by the CTA that had all of it
-                written = true;
-                continue;
-            }
-            const int r = (int)(((int64_t)max(0, t - (kind ? s.q0 : q0)) * a.G + h % a.G) % p.slot_rows);
-            const float* first = p.head + (p.by_row ? row : (int64_t)c0 * p.slot_rows + r) * a.D;
-            for (int base = c0; base <= c1; base += 32) {
-                const int c = base + lane;
-                float m = -INFINITY, l = 0.0f;
-                if (c <= c1) {
-                    if (c == c0) {
-                        m = st[kind].x;
-                        l = st[kind].y;
-                    } else {
-                        const float2 v = p.tail_stat[(int64_t)c * p.slot_rows + r];
-                        m = v.x;
-                        l = v.y;
-                    }
+    for (int kind = 0; kind < 2; ++kind) {
+        if (kind == 0 && !both) continue;
+        const PartArgs& p = kind ? rest : prefix;
+        const PartPlace at = kind ? place : place_of(st[0]);
+        if (at.c1 < at.c0 || at.c1 >= p.ctas || at.row >= p.slot_rows) {  // start arrays that contradict each other: no CTA had the row
+            *a.err = kErrIndex;
+            continue;
+        }
+        const float* first = p.head + (p.by_row ? row : (int64_t)at.c0 * p.slot_rows + at.row) * a.D;
+        for (int base = at.c0; base <= at.c1; base += 32) {
+            const int c = base + lane;
+            float m = -INFINITY, l = 0.0f;
+            if (c <= at.c1) {
+                if (c == at.c0) {
+                    m = st[kind].x;
+                    l = st[kind].y;
+                } else {
+                    const float2 v = p.tail_stat[(int64_t)c * p.slot_rows + at.row];
+                    m = v.x;
+                    l = v.y;
                 }
-                const float mx = fmaxf(M, warp_max(m));
-                if (mx == -INFINITY) continue;
-                const float keep = M == -INFINITY ? 0.0f : exp2_fast(M - mx);
-                const float w = m == -INFINITY ? 0.0f : exp2_fast(m - mx);
-                M = mx;
-                L = L * keep + warp_sum(l * w);
-                o.x *= keep;
-                o.y *= keep;
-                o.z *= keep;
-                o.w *= keep;
-                const int n = min(32, c1 - base + 1);
+            }
+            const float mx = fmaxf(M, warp_max(m));
+            if (mx == -INFINITY) continue;
+            const float keep = M == -INFINITY ? 0.0f : exp2_fast(M - mx);
+            const float w = m == -INFINITY ? 0.0f : exp2_fast(m - mx);
+            M = mx;
+            L = L * keep + warp_sum(l * w);
+            o.x *= keep;
+            o.y *= keep;
+            o.z *= keep;
+            o.w *= keep;
+            const int n = min(32, at.c1 - base + 1);
 #pragma unroll 8
-                for (int i = 0; i < n; ++i) {
-                    const float wi = __shfl_sync(0xffffffffu, w, i);
-                    const float* src = base + i == c0 ? first : p.tail + ((int64_t)(base + i) * p.slot_rows + r) * a.D;
-                    if (live) {
-                        const float4 v = *reinterpret_cast<const float4*>(src + lane * 4);
-                        o.x = fmaf(v.x, wi, o.x);
-                        o.y = fmaf(v.y, wi, o.y);
-                        o.z = fmaf(v.z, wi, o.z);
-                        o.w = fmaf(v.w, wi, o.w);
-                    }
+            for (int i = 0; i < n; ++i) {
+                const float wi = __shfl_sync(0xffffffffu, w, i);
+                const float* src = base + i == at.c0 ? first : p.tail + ((int64_t)(base + i) * p.slot_rows + at.row) * a.D;
+                if (live) {
+                    const float4 v = *reinterpret_cast<const float4*>(src + lane * 4);
+                    o.x = fmaf(v.x, wi, o.x);
+                    o.y = fmaf(v.y, wi, o.y);
+                    o.z = fmaf(v.z, wi, o.z);
+                    o.w = fmaf(v.w, wi, o.w);
                 }
             }
         }
-        if (!live || written) continue;
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-        TQ* dst = static_cast<TQ*>(a.out) + row * a.D + lane * 4;
-        if constexpr (sizeof(TQ) == 4) {
-            *reinterpret_cast<float4*>(dst) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-        } else {
-            *reinterpret_cast<uint2*>(dst) = make_uint2(Half2Of<T16>::pack(o.x * inv, o.y * inv), Half2Of<T16>::pack(o.z * inv, o.w * inv));
-        }
+    }
+    if (!live) return;
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    TQ* dst = static_cast<TQ*>(a.out) + row * a.D + lane * 4;
+    if constexpr (sizeof(TQ) == 4) {
+        *reinterpret_cast<float4*>(dst) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    } else {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(Half2Of<T16>::pack(o.x * inv, o.y * inv), Half2Of<T16>::pack(o.z * inv, o.w * inv));
     }
 }
 
-template <typename TQ, typename TK, int DP, bool SPLIT>
-void launch_decode_t(const PagedArgs& a, const PartArgs& rest, cudaStream_t s, bool pdl) {
-    auto kern = paged_decode_kernel<TQ, TK, DP, SPLIT>;
+template <typename TQ, typename TK, int DP, int NT, bool SPLIT>
+void launch_decode_t(const PagedArgs& a, const CacheMaps& maps, const PartArgs& rest, cudaStream_t s, bool pdl, bool after_tc) {
+    auto kern = paged_decode_kernel<TQ, TK, DP, NT, SPLIT>;
     allow_max_dynamic_smem(kern);
-    launch_kernel(kern, dim3((unsigned)rest.ctas), dim3(kDecThreads), DecodeSmem<DP>::bytes(a.G <= 8 ? 8 : 16), s, pdl, a, rest);
+    launch_kernel(kern, dim3((unsigned)rest.ctas), dim3(kDecThreads), DecodeSmem<DP, NT, SPLIT>::bytes, s, pdl, a, maps, rest,
+                  (int)after_tc);
 }
 
-template <int DP>
-void launch_decode_d(const PagedArgs& a, const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s, bool pdl) {
-    if (tq == BEACON_CUDA_DTYPE_F32) launch_decode_t<float, __half, DP, true>(a, rest, s, pdl);
-    else if (tk == BEACON_CUDA_DTYPE_F16) launch_decode_t<__half, __half, DP, false>(a, rest, s, pdl);
-    else launch_decode_t<__nv_bfloat16, __nv_bfloat16, DP, false>(a, rest, s, pdl);
+template <int DP, int NT>
+void launch_decode_d(const PagedArgs& a, const CacheMaps& maps, const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s,
+                     bool pdl, bool after_tc) {
+    using H = __half;
+    using B = __nv_bfloat16;
+    if (tq == BEACON_CUDA_DTYPE_F32) launch_decode_t<float, H, DP, NT, true>(a, maps, rest, s, pdl, after_tc);
+    else if (tk == BEACON_CUDA_DTYPE_F16) launch_decode_t<H, H, DP, NT, false>(a, maps, rest, s, pdl, after_tc);
+    else launch_decode_t<B, B, DP, NT, false>(a, maps, rest, s, pdl, after_tc);
 }
 
 }  // namespace
 
-int paged_decode_ctas(const BeaconCudaContext* ctx, const PagedArgs& a, bool split) {
-    (void)split;
+int paged_decode_ctas(const BeaconCudaContext* ctx, const PagedArgs& a) {
+    (void)a;
     return 2 * ctx->sm_count;
 }
 
-void launch_paged_decode(const PagedArgs& a, const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s, bool pdl) {
-    if (a.D <= 64) launch_decode_d<64>(a, rest, tq, tk, s, pdl);
-    else launch_decode_d<128>(a, rest, tq, tk, s, pdl);
+void launch_paged_decode(const PagedArgs& a, const CacheMaps& maps, const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s,
+                         bool pdl, bool after_tc) {
+    // up to 8 heads fit one column block of the matrix instructions
+    if (a.D <= 64 && a.G <= 8) launch_decode_d<64, 1>(a, maps, rest, tq, tk, s, pdl, after_tc);
+    else if (a.D <= 64) launch_decode_d<64, 2>(a, maps, rest, tq, tk, s, pdl, after_tc);
+    else if (a.G <= 8) launch_decode_d<128, 1>(a, maps, rest, tq, tk, s, pdl, after_tc);
+    else launch_decode_d<128, 2>(a, maps, rest, tq, tk, s, pdl, after_tc);
 }
 
 void launch_paged_combine(const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, int32_t tq, cudaStream_t s) {
-    // four heads a block (one a warp) until the device is full, then more
-    const int64_t blocks = (int64_t)a.T * ((a.H + 3) / 4);
-    const int heads = (int)std::min<int64_t>((a.H + 3) / 4, std::max<int64_t>(1, blocks / 2048)) * 4;
-    const dim3 grid((unsigned)a.T, (unsigned)((a.H + heads - 1) / heads));
-    if (tq == BEACON_CUDA_DTYPE_F32) launch_kernel(paged_combine_kernel<float, __half>, grid, dim3(128), 0, s, true, a, prefix, rest, heads);
-    else if (tq == BEACON_CUDA_DTYPE_F16) launch_kernel(paged_combine_kernel<__half, __half>, grid, dim3(128), 0, s, true, a, prefix, rest, heads);
-    else launch_kernel(paged_combine_kernel<__nv_bfloat16, __nv_bfloat16>, grid, dim3(128), 0, s, true, a, prefix, rest, heads);
+    const dim3 grid((unsigned)(((int64_t)a.T * a.H + 3) / 4));
+    if (tq == BEACON_CUDA_DTYPE_F32) launch_kernel(paged_combine_kernel<float, __half>, grid, dim3(128), 0, s, true, a, prefix, rest);
+    else if (tq == BEACON_CUDA_DTYPE_F16) launch_kernel(paged_combine_kernel<__half, __half>, grid, dim3(128), 0, s, true, a, prefix, rest);
+    else launch_kernel(paged_combine_kernel<__nv_bfloat16, __nv_bfloat16>, grid, dim3(128), 0, s, true, a, prefix, rest);
 }
 
 }  // namespace bc

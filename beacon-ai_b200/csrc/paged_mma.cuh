@@ -2,6 +2,7 @@
 // the paged attention kernels.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -70,6 +71,29 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uin
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Bounded wait (mbar_wait_bounded) whose limit is already in a register and
+// that reads the clock only when the barrier is not there yet.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, long long limit) {
+    if (mbar_test_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    if (limit >= kBoundedWaitLimit) {
+        while (!mbar_try_wait(bar, parity))
+            if (clock64() - t0 > limit) return false;
+        return true;
+    }
+    while (!mbar_test_wait(bar, parity))
+        if (clock64() - t0 > limit) return false;
+    return true;
+}
+
+// Rows [row, row + box) of one head, 64 values from x on, to shared memory.
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int head, int row, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(row), "r"(smem_u32(bar))
+        : "memory");
 }
 
 // The power of two that brings the largest magnitude mx of a 32-bit query row

@@ -15,9 +15,12 @@
 //    and are joined at the end. 32-bit queries come as two f16 parts (SPLIT):
 //    two products for the scores, and two for the sums, whose weights are
 //    split likewise.
-// P replaces S: the packed weights (64 columns, then 64 of their remainders)
-// lie where the scores were, and are the A operand of O += P V from tensor
-// memory; V is read N-major.
+// P replaces S in place, 32 keys at a time: the 16 columns of packed weights
+// (then 16 of their remainders) lie where the 32 scores were, and are the A
+// operand of O += P V from tensor memory; V is read N-major. The scores are
+// read twice (maximum, weights; 50 cycles a tile) in short loops: holding all
+// 128 in registers takes straight code of 20 KB, whose first pass through the
+// instruction cache costs 15,000 cycles, more than the work of a small call.
 // Key and value rows come in page by page by tensor copies (TMA) of up to 128
 // rows into a ring of tiles in the 128-byte swizzle, requested by four warps;
 // rows of a value tile that are no keys of the block are zeroed there (their
@@ -46,10 +49,8 @@ namespace {
 constexpr int kTile = 128;              // rows of a row tile, keys of a key tile
 constexpr int kSoftWarps = 8;
 constexpr int kLoadWarp = 8, kLoadWarps = 4;
-constexpr int kMmaWarp = 12;            // with three idle warps: registers move by groups of four warps
-constexpr int kTcThreads = 512;
-// registers: 128 a thread at launch; 2 x 176 + 104 + 56 = 4 x 128
-constexpr int kSoftRegs = 176, kLoadRegs = 104, kMmaRegs = 56;
+constexpr int kMmaWarp = 12;
+constexpr int kTcThreads = 32 * (kMmaWarp + 1);
 constexpr uint32_t kTmemCols = 512;     // S 2 x 128, O 2 x DP
 constexpr float kRescale = 8.0f;        // log2 of the largest weight
 
@@ -116,11 +117,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
         : "r"(addr));
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                 : "memory");
-}
 __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
@@ -128,8 +124,7 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
                    "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const float (&v)[16]) {
-    const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(addr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
@@ -164,21 +159,6 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t at) {
     return v;
 }
 
-// Bounded wait (mbar_wait_bounded) whose limit is already in a register and
-// that reads the clock only when the barrier is not there yet.
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, long long limit) {
-    if (mbar_test_wait(bar, parity)) return true;
-    const long long t0 = clock64();
-    if (limit >= kBoundedWaitLimit) {
-        while (!mbar_try_wait(bar, parity))
-            if (clock64() - t0 > limit) return false;
-        return true;
-    }
-    while (!mbar_test_wait(bar, parity))
-        if (clock64() - t0 > limit) return false;
-    return true;
-}
-
 // The rows that share keys: a group's queries against its prefix (kind 0), or a
 // sequence's queries against its own keys (kind 1).
 struct Block {
@@ -194,14 +174,24 @@ __device__ __forceinline__ Block block_of(const PagedArgs& a, int e) {
     Block k;
     const int groups = a.merged ? 0 : a.groups;
     if (e < groups) {
-        const int lo = start_at(a.gstarts, e, a.B, a.err), hi = start_at(a.gstarts, e + 1, a.B, a.err);
-        if (hi < lo) *a.err = kErrIndex;
-        if (hi <= lo) return k;
-        k.b = lo;
-        k.key1 = min(prefix_len(a, e), kv_len(a, lo));
-        k.tok0 = a.qstarts ? start_at(a.qstarts, lo, a.T, a.err) : lo;
-        const int tok1 = a.qstarts ? start_at(a.qstarts, hi, a.T, a.err) : hi;
-        k.rows = max(0, tok1 - k.tok0) * a.G;
+        bool bad = false;
+        int lo = __ldg(a.gstarts + e), hi = __ldg(a.gstarts + e + 1);
+        const int p = __ldg(a.prefix + e);
+        lo = keep_in(lo, a.B, bad);
+        hi = keep_in(hi, a.B, bad);
+        if (hi > lo) {
+            const int len = __ldg(a.lens + lo);
+            int t0 = lo, t1 = hi;
+            if (a.qstarts) {
+                t0 = __ldg(a.qstarts + lo);
+                t1 = __ldg(a.qstarts + hi);
+            }
+            k.b = lo;
+            k.key1 = min(keep_in(p, capacity(a), bad), keep_in(len, capacity(a), bad));
+            k.tok0 = keep_in(t0, a.T, bad);
+            k.rows = max(0, keep_in(t1, a.T, bad) - k.tok0) * a.G;
+        }
+        if (bad || hi < lo) *a.err = kErrIndex;
         return k;
     }
     const SeqInfo s = seq_info(a, e - groups);
@@ -221,11 +211,12 @@ __device__ __forceinline__ Block block_of(const PagedArgs& a, int e) {
     k.len = s.len;
     return k;
 }
-// Key tiles that row tile rt of a block needs (its last row sees the most keys).
+// Key tiles that row tile rt of a block needs (its last row sees the most keys);
+// rows of a sequence have one at least, which then shows them nothing.
 __device__ __forceinline__ int tiles_of(const PagedArgs& a, const Block& k, int rt, int block_rows) {
     int end = k.key1;
     if (k.kind) end = min(end, k.len - k.nq + (min((rt + 1) * block_rows, k.rows) - 1) / a.G + 1);
-    return end > k.key0 ? (end - k.base + kTile - 1) / kTile : 0;
+    return end > k.key0 ? (end - k.base + kTile - 1) / kTile : k.kind;
 }
 __device__ __forceinline__ int tiles_of_block(const PagedArgs& a, const Block& k, int block_rows) {
     const int n = (k.rows + block_rows - 1) / block_rows;
@@ -269,13 +260,6 @@ struct Piece {
     }
 };
 
-__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int head, int row, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(row), "r"(smem_u32(bar))
-        : "memory");
-}
-
 template <typename TQ, typename T16, int DP, bool SPLIT, bool TWO>
 __global__ void __launch_bounds__(kTcThreads, 1)
     paged_tc_kernel(const PagedArgs a, const __grid_constant__ CacheMaps maps, const PartArgs prefix, const PartArgs rest, int entries,
@@ -303,7 +287,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(&full_bar[i], a.box ? 1 : kLoadWarps * 32);
             mbar_init(&empty_bar[i], 1);
         }
-        mbar_init(&qfull_bar, kLoadWarps * 32);
+        mbar_init(&qfull_bar, (SPLIT ? kSoftWarps : kLoadWarps) * 32);
         mbar_init(&qempty_bar, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_bar[i], 1);
@@ -321,6 +305,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    prefetch_indices(a);
     pdl_wait();
 
     // this CTA's share of the line
@@ -347,8 +332,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     total *= a.Hkv;
     pdl_trigger();
-    const int cta = blockIdx.x, ctas = sharers(total, line_ctas);
-    const long long u0 = cta < ctas ? share_begin(total, ctas, cta) : 0, u1 = cta < ctas ? share_begin(total, ctas, cta + 1) : 0;
+    const int cta = blockIdx.x;
+    const Shares shares(total, line_ctas);
+    const long long u0 = cta < shares.ctas ? shares.begin(cta) : 0, u1 = cta < shares.ctas ? shares.begin(cta + 1) : 0;
     if (u0 < u1 && before * a.Hkv <= u0 && u0 < (before + mine) * a.Hkv) {
         int e = e0;
         for (; e < e1; ++e) {
@@ -386,7 +372,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
     if (warp >= kLoadWarp && warp < kLoadWarp + kLoadWarps) {
         // --- producers: queries, then key and value tiles in the order of their use
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
         const int pw = warp - kLoadWarp;
         const int64_t stride = (int64_t)a.Hkv * a.D * 2;  // bytes from one cache row to the next
         const int c = lane % CH;                          // this lane's chunk of the rows it copies
@@ -499,7 +484,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     give_up();
                     ok = false;
                 }
-                const int lo = max(0, p.k.key0 - pos0), hi = min(kTile, p.k.key1 - pos0);  // rows [lo, hi) are keys
+                const int lo = max(0, p.k.key0 - pos0), hi = max(lo, min(kTile, p.k.key1 - pos0));  // rows [lo, hi) are keys
                 for (int i = lane; i < (lo + kTile - hi) * CH; i += 32) {
                     const int q = i / CH, r = q < lo ? q : hi + q - lo, cc = i % CH;
                     st_shared16(dst + (cc >> 3) * (kTile * 128) + r * 128 + ((cc & 7) << 4), 0, 0, 0, 0);
@@ -519,7 +504,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 page = ahead;
             };
             while (ok && f < min(3, 2 * p.n)) load_next();
-            if (seg > 0) {
+            if (seg > 0 && !SPLIT) {
                 if (!a.box) {
                     // the last products of the piece before need all of its tiles
                     cp_async_wait<0>();
@@ -538,38 +523,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const int br = p.rt * BR + i * kTile + pw * 32 + lane;
                 const int qrow = br < p.k.rows ? (p.k.tok0 + br / a.G) * a.H + p.kvh * a.G + br % a.G : -1;
                 const uint32_t dst = smem_u32(q_smem) + (TWO ? i * SM::tile : 0);
-                if constexpr (SPLIT) {
-                    // a warp takes a row at a time, sixteen on their way: each lane four values
-#pragma unroll 1
-                    for (int r0 = 0; r0 < 32; r0 += 16) {
-                        float4 x[16];
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            const int qr = __shfl_sync(0xffffffffu, qrow, r0 + k);
-                            x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                            if (qr >= 0 && lane * 4 < a.D)
-                                x[k] = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (int64_t)qr * a.D + lane * 4);
-                        }
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            const int r = pw * 32 + r0 + k;
-                            float mx = fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w)));
-                            mx = warp_max(mx);
-                            float inv;
-                            const float sc = query_scale(mx, inv);
-                            if (lane == 0) qscale_s[seg & 1][r] = a.scale * 1.4426950408889634f * inv;
-                            if (lane * 4 < DP) {
-                                uint2 h, l;
-                                split_f16(x[k].x * sc, x[k].y * sc, h.x, l.x);
-                                split_f16(x[k].z * sc, x[k].w * sc, h.y, l.y);
-                                const int cc = lane >> 1;
-                                const uint32_t at = dst + (cc >> 3) * (kTile * 128) + r * 128 + (((cc & 7) ^ (r & 7)) << 4) + (lane & 1) * 8;
-                                asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(at), "r"(h.x), "r"(h.y) : "memory");
-                                asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(at + SM::tile), "r"(l.x), "r"(l.y) : "memory");
-                            }
-                        }
-                    }
-                } else {
+                if constexpr (!SPLIT) {
 #pragma unroll 8
                     for (int k = 0; k < 32 / RPI; ++k) {
                         const int rr = k * RPI + lane / CH;
@@ -584,9 +538,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (!SPLIT) {
                 cp_async_commit();
                 cp_async_wait<0>();
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                arrive(&qfull_bar);
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            arrive(&qfull_bar);
             while (ok && f < 2 * p.n) load_next();
         }
         // nothing may land after the CTA has ended
@@ -595,7 +549,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (a.box && pw == 0)
             for (int i = max(0, it - NST); i < it; ++i) mbar_drain(&full_bar[i % NST], (uint32_t)((i / NST) & 1));
     } else if (warp >= kMmaWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
         if (warp == kMmaWarp) {
             // the whole warp waits; its elected thread issues
             int it = 0, np[2] = {0, 0};
@@ -642,7 +595,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int k = 0; k < kTile / 16; ++k)
 #pragma unroll
                         for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
-                            mma_ts(o, p + part * 64 + k * 8, b + k * (2048 >> 4), kDescHi, id_pv, k + part > 0 || !first);
+                            mma_ts(o, p + (k >> 1) * 32 + (k & 1) * 8 + part * 16, b + k * (2048 >> 4), kDescHi, id_pv, k + part > 0 || !first);
                     if (last) commit(&empty_bar[st]);
                 }
                 __syncwarp();
@@ -688,7 +641,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
     } else {
         // --- softmax: stream s, row r of its tile
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         const int s = warp >> 2, r = tid & (kTile - 1);
         const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_col = tmem + lane_at + s * kTile;
@@ -719,6 +671,44 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
             }
+            if constexpr (SPLIT) {
+                // the block's queries as two f16 parts: 16 rows a warp, a row at a
+                // time (each lane four values), eight on their way
+                if (seg > 0) wait(&qempty_bar, (uint32_t)((seg - 1) & 1));
+                if (!ok) break;
+                const int mine = p.rt * BR + warp * 16 + (lane & 15);
+                const int qrow = mine < p.k.rows ? (p.k.tok0 + mine / a.G) * a.H + p.kvh * a.G + mine % a.G : -1;
+#pragma unroll 1
+                for (int r0 = 0; r0 < 16; r0 += 8) {
+                    float4 x[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int qr = __shfl_sync(0xffffffffu, qrow, r0 + k);
+                        x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (qr >= 0 && lane * 4 < a.D)
+                            x[k] = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (int64_t)qr * a.D + lane * 4);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int qr = warp * 16 + r0 + k;
+                        const float mx = warp_max(fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w))));
+                        float inv;
+                        const float sc = query_scale(mx, inv);
+                        if (lane == 0) qscale_s[seg & 1][qr] = a.scale * 1.4426950408889634f * inv;
+                        if (lane * 4 < DP) {
+                            uint2 h, l;
+                            split_f16(x[k].x * sc, x[k].y * sc, h.x, l.x);
+                            split_f16(x[k].z * sc, x[k].w * sc, h.y, l.y);
+                            const int cc = lane >> 1;
+                            const uint32_t at = smem_u32(q_smem) + (cc >> 3) * (kTile * 128) + qr * 128 + (((cc & 7) ^ (qr & 7)) << 4) + (lane & 1) * 8;
+                            asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(at), "r"(h.x), "r"(h.y) : "memory");
+                            asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(at + SM::tile), "r"(l.x), "r"(l.y) : "memory");
+                        }
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                arrive(&qfull_bar);
+            }
             wait(&qfull_bar, (uint32_t)(seg & 1));
             if (!ok) break;
             // above zero, so that a masked score (-inf) stays one
@@ -736,23 +726,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const int key = p.k.base + (p.tile + t) * kTile;
                 const int seen = limit - key, skip = p.k.key0 - key;  // columns [skip, seen) are visible
                 const bool whole = __all_sync(0xffffffffu, seen >= kTile && skip <= 0);
-                float v[kTile];
+                float v[32];
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < kTile; c += 32) {
+                    tmem_ld32(s_col + c, v);
+                    tmem_wait_ld();
+                    if (!whole) {
 #pragma unroll
-                for (int c = 0; c < kTile; c += 32) tmem_ld32(s_col + c, *reinterpret_cast<float(*)[32]>(v + c));
-                tmem_wait_ld();
-                if (!whole) {
+                        for (int i = 0; i < 32; ++i)
+                            if (c + i >= seen || c + i < skip) v[i] = -INFINITY;
+                    }
+                    float x[4] = {top, v[0], v[1], v[2]};
 #pragma unroll
-                    for (int i = 0; i < kTile; ++i)
-                        if (i >= seen || i < skip) v[i] = -INFINITY;
+                    for (int i = 3; i < 27; i += 8)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) x[k] = max3(x[k], v[i + k], v[i + 4 + k]);
+                    x[0] = max3(x[0], v[27], v[28]);
+                    x[1] = max3(x[1], v[29], v[30]);
+                    x[2] = max3(x[2], x[3], v[31]);
+                    top = max3(x[0], x[1], x[2]);
                 }
-                float top[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-                for (int i = 4; i < kTile - 4; i += 8)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) top[j] = max3(top[j], v[i + j], v[i + 4 + j]);
-                top[0] = max3(top[0], top[1], fmaxf(top[2], top[3]));
-                top[0] = max3(max3(top[0], v[kTile - 4], v[kTile - 3]), v[kTile - 2], v[kTile - 1]);
-                const float mx = fmaxf(m, top[0] * cs);
+                const float mx = fmaxf(m, top * cs);
                 const bool move = m != -INFINITY && mx > m + kRescale;
                 if (t >= (TWO ? 1 : 2) && __any_sync(0xffffffffu, move)) {
                     const float keep = move ? exp2_fast(m - mx) : 1.0f;
@@ -760,34 +755,40 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll 1
                     for (int c = 0; c < DP; c += 16) {
                         float w[16];
+                        uint32_t x[16];
                         const uint32_t o_at = tmem + lane_at + 2 * kTile + s * DP + c;
                         tmem_ld16(o_at, w);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) w[i] *= keep;
-                        tmem_st16(o_at, w);
+                        for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(w[i] * keep);
+                        tmem_st16(o_at, x);
                     }
                 }
                 if (move || m == -INFINITY) m = mx;
                 const float ref = m == -INFINITY ? 0.0f : m;
                 const float2 cs2 = make_float2(cs, cs), ref2 = make_float2(-ref, -ref);
                 float2 sum[2] = {make_float2(l, 0.0f), make_float2(0.0f, 0.0f)};
-                // the weights, 16 at a time: the packed ones take the registers of few scores
+#pragma unroll 1
+                for (int c = 0; c < kTile; c += 32) {
+                    tmem_ld32(s_col + c, v);
+                    tmem_wait_ld();
+                    if (!whole) {
 #pragma unroll
-                for (int c = 0; c < kTile / 16; ++c) {
-                    uint32_t w[8], w2[8];
+                        for (int i = 0; i < 32; ++i)
+                            if (c + i >= seen || c + i < skip) v[i] = -INFINITY;
+                    }
+                    uint32_t w[16], w2[16];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int k = c * 16 + 2 * i;
-                        float2 x = fma2(make_float2(v[k], v[k + 1]), cs2, ref2);
+                    for (int i = 0; i < 16; ++i) {
+                        float2 x = fma2(make_float2(v[2 * i], v[2 * i + 1]), cs2, ref2);
                         x.x = exp2_fast(x.x);
                         x.y = exp2_fast(x.y);
                         sum[i & 1] = add2(sum[i & 1], x);
                         if constexpr (SPLIT) split_f16(x.x, x.y, w[i], w2[i]);
                         else w[i] = Half2Of<T16>::pack(x.x, x.y);
                     }
-                    tmem_st8(s_col + c * 8, w);
-                    if constexpr (SPLIT) tmem_st8(s_col + 64 + c * 8, w2);
+                    tmem_st16(s_col + c, w);
+                    if constexpr (SPLIT) tmem_st16(s_col + c + 16, w2);
                 }
                 sum[0] = add2(sum[0], sum[1]);
                 l = sum[0].x + sum[0].y;
@@ -813,7 +814,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             const PartArgs& part = p.k.kind ? rest : prefix;
             const long long first = p.u - p.tile;
-            const int c0 = share_of(total, ctas, first), c1 = share_of(total, ctas, first + p.tiles - 1);
+            const int c0 = shares.of(first), c1 = shares.of(first + p.tiles - 1);
             const bool done = c0 == c1 && p.k.kind && p.k.key0 == 0;  // no other part anywhere
             const int64_t orow = (int64_t)tok * a.H + p.kvh * a.G + row % a.G;
             const int slot_row = (TWO ? s * kTile : 0) + r;
@@ -899,7 +900,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
             }
             if (live && (TWO || s == 0)) {
-                if (c0 == cta) part.stat[orow] = make_float4(M, L, __int_as_float(c0), __int_as_float(c1));
+                if (c0 == cta) part.stat[orow] = pack_stat(M, L, PartPlace{c0, c1, slot_row, p.k.key0 > 0});
                 else part.tail_stat[slot] = make_float2(M, L);
             }
             if (!TWO) {
