@@ -216,10 +216,10 @@ void run_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream, Paged
         }
         bool pdl = !scratch.of_graph();  // a graph's allocation comes first
         if (tc) {
-            launch_paged_tc(plan, a, maps, prefix, rest, tq, tk, stream->s, pdl);
+            launch_paged_tc(ctx, plan, a, maps, prefix, rest, tq, tk, stream->s, pdl);
             pdl = true;
         }
-        if (decode) launch_paged_decode(a, dmaps, rest, tq, tk, stream->s, pdl, tc);
+        if (decode) launch_paged_decode(ctx, a, dmaps, rest, tq, tk, stream->s, pdl, tc);
         launch_paged_combine(a, prefix, rest, tq, stream->s);
         return;
     }

@@ -94,7 +94,7 @@ struct CacheMaps {  // tensor maps of the caches: boxes of some rows by 64 value
 constexpr int kDecodeBox = 16;  // most rows of a copy box of paged_decode_kernel
 int paged_decode_ctas(const BeaconCudaContext* ctx, const PagedArgs& a);
 // after_tc: the launch before it is paged_tc_kernel of the same call.
-void launch_paged_decode(const PagedArgs& a, const CacheMaps& maps, const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s,
+void launch_paged_decode(const BeaconCudaContext* ctx, const PagedArgs& a, const CacheMaps& maps, const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s,
                          bool pdl, bool after_tc);
 // Rows of a block and CTAs of the tensor-core kernel (paged_tc.cu), for the
 // prefixes and, when with_rest, the rest of every sequence.
@@ -105,7 +105,7 @@ struct PagedTcPlan {
     int ctas = 0;
 };
 PagedTcPlan plan_paged_tc(const BeaconCudaContext* ctx, const PagedArgs& a, bool split, bool with_rest);
-void launch_paged_tc(const PagedTcPlan& plan, const PagedArgs& a, const CacheMaps& maps, const PartArgs& prefix,
+void launch_paged_tc(const BeaconCudaContext* ctx, const PagedTcPlan& plan, const PagedArgs& a, const CacheMaps& maps, const PartArgs& prefix,
                      const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s, bool pdl);
 void launch_paged_combine(const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, int32_t tq, cudaStream_t s);
 
@@ -119,21 +119,25 @@ __device__ __forceinline__ int keep_in(int v, long long most, bool& bad) {
 }
 __device__ __forceinline__ long long capacity(const PagedArgs& a) { return (long long)a.max_pages * a.page_size; }
 
-// Asks for the index arrays before anything reads them, so that the first use
-// of each (one depends on another) does not wait for memory in turn. Requests
-// only: what an earlier kernel still writes is read after pdl_wait.
-__device__ __forceinline__ void prefetch_indices(const PagedArgs& a) {
-    auto ask = [](const int32_t* p, long long n) {
-        for (long long i = threadIdx.x * 32LL; i < n && i < 32LL * 2 * blockDim.x; i += 32LL * blockDim.x)
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
+// Asks for the index arrays and the queries (a share of the larger ones per
+// CTA) before anything reads them, so that the first use of each, which depends
+// on the one before, does not wait for memory in turn. Requests only: what an
+// earlier kernel still writes is read after pdl_wait.
+__device__ __forceinline__ void prefetch_inputs(const PagedArgs& a, int q_bytes) {
+    auto ask = [](const void* p, long long bytes, long long first, long long step) {
+        for (long long i = first; i * 128 < bytes && i < first + 4 * step; i += step)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p) + i * 128));
     };
-    ask(a.lens, a.B);
-    if (a.qstarts) ask(a.qstarts, a.B + 1);
+    const int t = threadIdx.x, n = blockDim.x;
+    ask(a.lens, a.B * 4LL, t, n);
+    if (a.qstarts) ask(a.qstarts, (a.B + 1) * 4LL, t, n);
     if (a.gstarts) {
-        ask(a.gstarts, a.groups + 1);
-        ask(a.prefix, a.groups);
+        ask(a.gstarts, (a.groups + 1) * 4LL, t, n);
+        ask(a.prefix, a.groups * 4LL, t, n);
     }
-    ask(a.table, (long long)a.B * a.max_pages);
+    const long long all = (long long)gridDim.x * n, at = (long long)t * gridDim.x + blockIdx.x;
+    ask(a.table, (long long)a.B * a.max_pages * 4, at, all);
+    ask(a.q, (long long)a.T * a.H * a.D * q_bytes, at, all);
 }
 
 // The i with starts[i] <= x < starts[i + 1] of an ascending array of n + 1

@@ -22,6 +22,7 @@
 #include "kernels.h"
 #include "paged_attn.h"
 #include "paged_mma.cuh"
+#include "rotary.h"
 
 namespace bc {
 namespace {
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(kDecThreads)
     float* merge_m = merge_o + kDecWarps * S::rows * DP;                                              // [warp][rows]
     float* merge_l = merge_m + kDecWarps * S::rows;
     float* scale_s = merge_l + kDecWarps * S::rows;                                                    // [rows]
-    prefetch_indices(a);
+    prefetch_inputs(a, sizeof(TQ));
     if (lane == 0) {
         for (int i = 0; i < NS; ++i) mbar_init(&bars[warp][i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -504,54 +505,65 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedArgs a, c
     const PartPlace place = place_of(st[1]);
     const bool both = rest.by_row && place.prefix;
     if (!both && place.c0 == place.c1) return;  // written by the CTA that had all of it
+    // the parts in one line, a lane each
+    const PartPlace pre = place_of(st[0]);
+    const bool bad = place.c1 < place.c0 || place.c1 >= rest.ctas || place.row >= rest.slot_rows ||
+                     (both && (pre.c1 < pre.c0 || pre.c1 >= prefix.ctas || pre.row >= prefix.slot_rows));
+    if (bad) {  // start arrays that contradict each other: no CTA had the row
+        *a.err = kErrIndex;
+        return;
+    }
+    const int n0 = both ? pre.c1 - pre.c0 + 1 : 0, n = n0 + place.c1 - place.c0 + 1;
     const bool live = lane * 4 < a.D;
     float M = -INFINITY, L = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int kind = 0; kind < 2; ++kind) {
-        if (kind == 0 && !both) continue;
-        const PartArgs& p = kind ? rest : prefix;
-        const PartPlace at = kind ? place : place_of(st[0]);
-        if (at.c1 < at.c0 || at.c1 >= p.ctas || at.row >= p.slot_rows) {  // start arrays that contradict each other: no CTA had the row
-            *a.err = kErrIndex;
-            continue;
-        }
-        const float* first = p.head + (p.by_row ? row : (int64_t)at.c0 * p.slot_rows + at.row) * a.D;
-        for (int base = at.c0; base <= at.c1; base += 32) {
-            const int c = base + lane;
-            float m = -INFINITY, l = 0.0f;
-            if (c <= at.c1) {
-                if (c == at.c0) {
-                    m = st[kind].x;
-                    l = st[kind].y;
-                } else {
-                    const float2 v = p.tail_stat[(int64_t)c * p.slot_rows + at.row];
-                    m = v.x;
-                    l = v.y;
-                }
+    for (int base = 0; base < n; base += 32) {
+        const int idx = base + lane;
+        const bool zero = idx < n0;
+        const PartArgs& p = zero ? prefix : rest;
+        const PartPlace at = zero ? pre : place;
+        const int c = at.c0 + (zero ? idx : idx - n0);
+        const int64_t slot = (int64_t)c * p.slot_rows + at.row;
+        float m = -INFINITY, l = 0.0f;
+        const float* src = p.tail + slot * a.D;
+        if (idx < n) {
+            if (c == at.c0) {
+                m = zero ? st[0].x : st[1].x;
+                l = zero ? st[0].y : st[1].y;
+                src = p.head + (p.by_row ? row : slot) * a.D;
+            } else {
+                const float2 v = p.tail_stat[slot];
+                m = v.x;
+                l = v.y;
             }
-            const float mx = fmaxf(M, warp_max(m));
-            if (mx == -INFINITY) continue;
-            const float keep = M == -INFINITY ? 0.0f : exp2_fast(M - mx);
-            const float w = m == -INFINITY ? 0.0f : exp2_fast(m - mx);
-            M = mx;
-            L = L * keep + warp_sum(l * w);
-            o.x *= keep;
-            o.y *= keep;
-            o.z *= keep;
-            o.w *= keep;
-            const int n = min(32, at.c1 - base + 1);
-#pragma unroll 8
-            for (int i = 0; i < n; ++i) {
-                const float wi = __shfl_sync(0xffffffffu, w, i);
-                const float* src = base + i == at.c0 ? first : p.tail + ((int64_t)(base + i) * p.slot_rows + at.row) * a.D;
-                if (live) {
-                    const float4 v = *reinterpret_cast<const float4*>(src + lane * 4);
-                    o.x = fmaf(v.x, wi, o.x);
-                    o.y = fmaf(v.y, wi, o.y);
-                    o.z = fmaf(v.z, wi, o.z);
-                    o.w = fmaf(v.w, wi, o.w);
-                }
+        }
+        const float mx = fmaxf(M, warp_max(m));
+        if (mx == -INFINITY) continue;
+        const float keep = M == -INFINITY ? 0.0f : exp2_fast(M - mx);
+        const float w = m == -INFINITY ? 0.0f : exp2_fast(m - mx);
+        M = mx;
+        L = L * keep + warp_sum(l * w);
+        o.x *= keep;
+        o.y *= keep;
+        o.z *= keep;
+        o.w *= keep;
+        const int k = min(32, n - base);
+        for (int i = 0; i < k; i += 8) {  // eight loads in flight
+            float4 v[8];
+            float wi[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                wi[q] = __shfl_sync(0xffffffffu, w, i + q);
+                const float* s = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)src, i + q));
+                v[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (live && i + q < k) v[q] = *reinterpret_cast<const float4*>(s + lane * 4);
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                o.x = fmaf(v[q].x, wi[q], o.x);
+                o.y = fmaf(v[q].y, wi[q], o.y);
+                o.z = fmaf(v[q].z, wi[q], o.z);
+                o.w = fmaf(v[q].w, wi[q], o.w);
             }
         }
     }
@@ -566,21 +578,22 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedArgs a, c
 }
 
 template <typename TQ, typename TK, int DP, int NT, bool SPLIT>
-void launch_decode_t(const PagedArgs& a, const CacheMaps& maps, const PartArgs& rest, cudaStream_t s, bool pdl, bool after_tc) {
+void launch_decode_t(const BeaconCudaContext* ctx, const PagedArgs& a, const CacheMaps& maps, const PartArgs& rest, cudaStream_t s, bool pdl, bool after_tc) {
     auto kern = paged_decode_kernel<TQ, TK, DP, NT, SPLIT>;
-    allow_max_dynamic_smem(kern);
+    static std::atomic<uint64_t> allowed{0};
+    allow_smem_once(kern, ctx, allowed);
     launch_kernel(kern, dim3((unsigned)rest.ctas), dim3(kDecThreads), DecodeSmem<DP, NT, SPLIT>::bytes, s, pdl, a, maps, rest,
                   (int)after_tc);
 }
 
 template <int DP, int NT>
-void launch_decode_d(const PagedArgs& a, const CacheMaps& maps, const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s,
+void launch_decode_d(const BeaconCudaContext* ctx, const PagedArgs& a, const CacheMaps& maps, const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s,
                      bool pdl, bool after_tc) {
     using H = __half;
     using B = __nv_bfloat16;
-    if (tq == BEACON_CUDA_DTYPE_F32) launch_decode_t<float, H, DP, NT, true>(a, maps, rest, s, pdl, after_tc);
-    else if (tk == BEACON_CUDA_DTYPE_F16) launch_decode_t<H, H, DP, NT, false>(a, maps, rest, s, pdl, after_tc);
-    else launch_decode_t<B, B, DP, NT, false>(a, maps, rest, s, pdl, after_tc);
+    if (tq == BEACON_CUDA_DTYPE_F32) launch_decode_t<float, H, DP, NT, true>(ctx, a, maps, rest, s, pdl, after_tc);
+    else if (tk == BEACON_CUDA_DTYPE_F16) launch_decode_t<H, H, DP, NT, false>(ctx, a, maps, rest, s, pdl, after_tc);
+    else launch_decode_t<B, B, DP, NT, false>(ctx, a, maps, rest, s, pdl, after_tc);
 }
 
 }  // namespace
@@ -590,13 +603,13 @@ int paged_decode_ctas(const BeaconCudaContext* ctx, const PagedArgs& a) {
     return 2 * ctx->sm_count;
 }
 
-void launch_paged_decode(const PagedArgs& a, const CacheMaps& maps, const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s,
+void launch_paged_decode(const BeaconCudaContext* ctx, const PagedArgs& a, const CacheMaps& maps, const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s,
                          bool pdl, bool after_tc) {
     // up to 8 heads fit one column block of the matrix instructions
-    if (a.D <= 64 && a.G <= 8) launch_decode_d<64, 1>(a, maps, rest, tq, tk, s, pdl, after_tc);
-    else if (a.D <= 64) launch_decode_d<64, 2>(a, maps, rest, tq, tk, s, pdl, after_tc);
-    else if (a.G <= 8) launch_decode_d<128, 1>(a, maps, rest, tq, tk, s, pdl, after_tc);
-    else launch_decode_d<128, 2>(a, maps, rest, tq, tk, s, pdl, after_tc);
+    if (a.D <= 64 && a.G <= 8) launch_decode_d<64, 1>(ctx, a, maps, rest, tq, tk, s, pdl, after_tc);
+    else if (a.D <= 64) launch_decode_d<64, 2>(ctx, a, maps, rest, tq, tk, s, pdl, after_tc);
+    else if (a.G <= 8) launch_decode_d<128, 1>(ctx, a, maps, rest, tq, tk, s, pdl, after_tc);
+    else launch_decode_d<128, 2>(ctx, a, maps, rest, tq, tk, s, pdl, after_tc);
 }
 
 void launch_paged_combine(const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, int32_t tq, cudaStream_t s) {

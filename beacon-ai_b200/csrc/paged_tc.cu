@@ -42,6 +42,7 @@
 #include "kernels.h"
 #include "paged_attn.h"
 #include "paged_mma.cuh"
+#include "rotary.h"
 
 namespace bc {
 namespace {
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    prefetch_indices(a);
+    prefetch_inputs(a, sizeof(TQ));
     pdl_wait();
 
     // this CTA's share of the line
@@ -922,24 +923,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 template <typename TQ, typename T16, int DP, bool SPLIT, bool TWO>
-void launch_tc_t(const PagedTcPlan& plan, const PagedArgs& a, const CacheMaps& maps, const PartArgs& prefix, const PartArgs& rest, cudaStream_t s, bool pdl) {
+void launch_tc_t(const BeaconCudaContext* ctx, const PagedTcPlan& plan, const PagedArgs& a, const CacheMaps& maps, const PartArgs& prefix, const PartArgs& rest, cudaStream_t s, bool pdl) {
     auto kern = paged_tc_kernel<TQ, T16, DP, SPLIT, TWO>;
-    allow_max_dynamic_smem(kern);
+    static std::atomic<uint64_t> allowed{0};
+    allow_smem_once(kern, ctx, allowed);
     const int entries = (a.merged ? 0 : a.groups) + (plan.rest ? a.B : 0);
     launch_kernel(kern, dim3((unsigned)plan.ctas), dim3(kTcThreads), TcSmem<DP, SPLIT, TWO>::bytes, s, pdl, a, maps, prefix, rest, entries,
                   plan.ctas);
 }
 
 template <int DP>
-void launch_tc_d(const PagedTcPlan& plan, const PagedArgs& a, const CacheMaps& maps, const PartArgs& prefix, const PartArgs& rest, int32_t tq, int32_t tk,
+void launch_tc_d(const BeaconCudaContext* ctx, const PagedTcPlan& plan, const PagedArgs& a, const CacheMaps& maps, const PartArgs& prefix, const PartArgs& rest, int32_t tq, int32_t tk,
                  cudaStream_t s, bool pdl) {
     using H = __half;
     using B = __nv_bfloat16;
-    if (tq == BEACON_CUDA_DTYPE_F32) launch_tc_t<float, H, DP, true, false>(plan, a, maps, prefix, rest, s, pdl);
-    else if (tk == BEACON_CUDA_DTYPE_F16 && plan.two) launch_tc_t<H, H, DP, false, true>(plan, a, maps, prefix, rest, s, pdl);
-    else if (tk == BEACON_CUDA_DTYPE_F16) launch_tc_t<H, H, DP, false, false>(plan, a, maps, prefix, rest, s, pdl);
-    else if (plan.two) launch_tc_t<B, B, DP, false, true>(plan, a, maps, prefix, rest, s, pdl);
-    else launch_tc_t<B, B, DP, false, false>(plan, a, maps, prefix, rest, s, pdl);
+    if (tq == BEACON_CUDA_DTYPE_F32) launch_tc_t<float, H, DP, true, false>(ctx, plan, a, maps, prefix, rest, s, pdl);
+    else if (tk == BEACON_CUDA_DTYPE_F16 && plan.two) launch_tc_t<H, H, DP, false, true>(ctx, plan, a, maps, prefix, rest, s, pdl);
+    else if (tk == BEACON_CUDA_DTYPE_F16) launch_tc_t<H, H, DP, false, false>(ctx, plan, a, maps, prefix, rest, s, pdl);
+    else if (plan.two) launch_tc_t<B, B, DP, false, true>(ctx, plan, a, maps, prefix, rest, s, pdl);
+    else launch_tc_t<B, B, DP, false, false>(ctx, plan, a, maps, prefix, rest, s, pdl);
 }
 
 }  // namespace
@@ -954,10 +956,10 @@ PagedTcPlan plan_paged_tc(const BeaconCudaContext* ctx, const PagedArgs& a, bool
     return p;
 }
 
-void launch_paged_tc(const PagedTcPlan& plan, const PagedArgs& a, const CacheMaps& maps, const PartArgs& prefix,
+void launch_paged_tc(const BeaconCudaContext* ctx, const PagedTcPlan& plan, const PagedArgs& a, const CacheMaps& maps, const PartArgs& prefix,
                      const PartArgs& rest, int32_t tq, int32_t tk, cudaStream_t s, bool pdl) {
-    if (a.D <= 64) launch_tc_d<64>(plan, a, maps, prefix, rest, tq, tk, s, pdl);
-    else launch_tc_d<128>(plan, a, maps, prefix, rest, tq, tk, s, pdl);
+    if (a.D <= 64) launch_tc_d<64>(ctx, plan, a, maps, prefix, rest, tq, tk, s, pdl);
+    else launch_tc_d<128>(ctx, plan, a, maps, prefix, rest, tq, tk, s, pdl);
 }
 
 }  // namespace bc

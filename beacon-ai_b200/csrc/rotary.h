@@ -2,9 +2,11 @@
 // and cache-append operations (rotary.cu).
 #pragma once
 
+#include <atomic>
 #include <memory>
 
 #include "internal.h"
+#include "kernels.h"
 
 struct BeaconCudaRope {
     BeaconCudaContext* ctx = nullptr;
@@ -55,5 +57,15 @@ class OutTensor {
 // Tensors of an operation must live on its context.
 void check_tensor(const BeaconCudaContext* ctx, const BeaconCudaTensor* t, const char* what);
 void check_stream(const BeaconCudaContext* ctx, const BeaconCudaStream* stream, const char* what);
+// allow_max_dynamic_smem once per device for a kernel (`done`: one flag word of
+// its own, a bit per device): the two driver calls cost more than a launch.
+template <typename K>
+void allow_smem_once(K kern, const BeaconCudaContext* ctx, std::atomic<uint64_t>& done) {
+    const uint64_t bit = 1ull << (ctx->device & 63);
+    if (ctx->device < 64 && (done.load(std::memory_order_acquire) & bit)) return;
+    allow_max_dynamic_smem(kern);
+    done.fetch_or(bit, std::memory_order_release);
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 }  // namespace bc
