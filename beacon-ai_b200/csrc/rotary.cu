@@ -5,13 +5,16 @@
 // All three are one pass over rows of `dim` values: read a head, optionally
 // scale it by w / sqrt(mean(x^2) + eps), turn its first rotary_dim values, and
 // write it to a dense row or to its cache page, so one kernel does them. It is
-// bound by memory: 16-byte loads, each value read and written once.
+// bound by memory: 16-byte loads and stores, each value read and written once.
 //
-// A block takes whole tokens. It first computes the sine and cosine of every
-// pair for its tokens into shared memory (a 64-bit product position * f_i / 2pi
-// reduced to one turn, then sincospif in 32 bits, so the angle of position 10^6
-// is as good as that of position 1) and all heads of the token use them: the
-// 64-bit work is per token, not per head.
+// A block takes a few tokens. A head is held by as many lanes as its 2 x
+// 16-byte slots need, so a warp has several heads at a time, and the loads of
+// its next four steps (128 bytes a lane) are in flight at once. The sines and
+// cosines of the block's tokens are computed once into shared memory while the
+// first loads are on their way: the angle is a 64-bit product position * f_i /
+// 2 pi reduced to one turn, then sincospif in 32 bits, so position 10^6 is as
+// exact as position 1. (Every warp computing its own: 1200 instructions a
+// token and 60 us for 8192 x 32 heads of 128 bf16 values, 20 us of memory.)
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -21,6 +24,7 @@
 #include "common.cuh"
 #include "internal.h"
 #include "kernels.h"
+#include "paged_mma.cuh"
 #include "rotary.h"
 
 namespace bc {
@@ -59,8 +63,10 @@ void check_stream(const BeaconCudaContext* ctx, const BeaconCudaStream* stream, 
 namespace {
 
 constexpr int kRowThreads = 256;
-constexpr int kMaxTokens = 32;     // tokens of one block
+constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kMaxTokens = 32;  // of a block
 constexpr int kMaxHeadDim = 512;
+constexpr int kRowSteps = 4;  // heads whose loads a lane has in flight: 128 bytes
 
 struct RowSegment {                // heads of one input tensor
     const void* src = nullptr;     // [T][heads][dim]
@@ -74,7 +80,6 @@ struct RowSegment {                // heads of one input tensor
 struct RowArgs {
     RowSegment seg[2];
     int64_t tokens = 0;
-    int heads = 0;  // of both segments
     int dim = 0, rotary = 0;
     float eps = 0.0f, amplitude = 1.0f;
     const int32_t* positions = nullptr;
@@ -85,32 +90,52 @@ struct RowArgs {
     int64_t seqs = 0, max_pages = 0, pages = 0, page_size = 0;
     int* err = nullptr;
     // launch shape
-    int block_tokens = 1;  // tokens of one block
-    int lanes = 1;         // threads of one head (power of two)
-    int parts = 1;         // blocks that share a block's heads (grid.y)
+    int lanes = 1;         // of one head (power of two)
+    int block_tokens = 1;  // tokens of a block
+    int part_groups = 0;   // head groups (heads that a warp holds at a time) of a block, of each token
 };
 
+// 16 bytes of values as floats, and floats stored as values, two at a time: 16-bit
+// values are never handled one by one.
 template <typename T>
-__device__ __forceinline__ float to_f32(T v);
+struct Slot;
 template <>
-__device__ __forceinline__ float to_f32(float v) { return v; }
-template <>
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
-
-template <typename T, int N>
-struct alignas(sizeof(T) * N) Pack {
-    T v[N];
+struct Slot<float> {
+    static constexpr int V = 4;
+    static __device__ __forceinline__ void unpack(const uint4& x, float* f) {
+        f[0] = __uint_as_float(x.x), f[1] = __uint_as_float(x.y), f[2] = __uint_as_float(x.z), f[3] = __uint_as_float(x.w);
+    }
 };
+template <typename T>
+struct Slot16 {
+    static constexpr int V = 8;
+    static __device__ __forceinline__ void unpack(const uint4& x, float* f) {
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 v = Half2Of<T>::unpack(w[i]);
+            f[2 * i] = v.x;
+            f[2 * i + 1] = v.y;
+        }
+    }
+};
+template <>
+struct Slot<__half> : Slot16<__half> {};
+template <>
+struct Slot<__nv_bfloat16> : Slot16<__nv_bfloat16> {};
+
+template <typename T, int V>
+__device__ __forceinline__ void store_slot(T* dst, const float* f) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+    } else if constexpr (V == 4) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(Half2Of<T>::pack(f[0], f[1]), Half2Of<T>::pack(f[2], f[3]));
+    } else {
+        *reinterpret_cast<uint4*>(dst) = make_uint4(Half2Of<T>::pack(f[0], f[1]), Half2Of<T>::pack(f[2], f[3]),
+                                                    Half2Of<T>::pack(f[4], f[5]), Half2Of<T>::pack(f[6], f[7]));
+    }
+}
 
 __device__ __forceinline__ float load_weight(const void* w, int32_t dtype, int i) {
     return dtype == BEACON_CUDA_DTYPE_F16 ? __half2float(static_cast<const __half*>(w)[i])
@@ -130,35 +155,64 @@ __device__ __forceinline__ int64_t cache_row(const RowArgs& a, int64_t t) {
     return -1;
 }
 
-// Sine and cosine of the block's tokens into shared memory, and their cache rows.
-__device__ __forceinline__ void fill_tables(const RowArgs& a, int64_t t0, int nt, float2* cs, int64_t* rows) {
-    const int half = a.rotary / 2;
-    for (int i = threadIdx.x; i < nt * half; i += blockDim.x) {
-        const int t = i / half, j = i - t * half;
-        double turn = (double)a.positions[t0 + t] * a.turns[j];
-        turn -= rint(turn);
-        float s, c;
-        sincospif(2.0f * (float)turn, &s, &c);
-        cs[i] = make_float2(c * a.amplitude, s * a.amplitude);
-    }
-    if (a.table)
-        for (int t = threadIdx.x; t < nt; t += blockDim.x) rows[t] = cache_row(a, t0 + t);
+__device__ __forceinline__ float2 turn_at(const RowArgs& a, int position, int pair) {
+    double turn = (double)position * __ldg(a.turns + pair);
+    turn -= rint(turn);
+    float s, c;
+    sincospif(2.0f * (float)turn, &s, &c);
+    return make_float2(c * a.amplitude, s * a.amplitude);
 }
 
-// Each head is handled by `lanes` threads, each with two slots of V values.
+// What a block computes before its heads: sines and cosines, norm weights in 32
+// bits, cache rows.
+struct RowTables {
+    float2* cs;      // [tokens][rotary / 2]
+    float* weight;   // [dim]
+    int64_t* rows;   // [tokens]
+};
+__device__ __forceinline__ RowTables row_tables(const RowArgs& a, uint8_t* smem) {
+    RowTables s;
+    s.rows = reinterpret_cast<int64_t*>(smem);
+    s.weight = reinterpret_cast<float*>(s.rows + kMaxTokens);
+    s.cs = reinterpret_cast<float2*>(s.weight + ((a.dim + 3) & ~3));
+    return s;
+}
+inline size_t row_tables_bytes(const RowArgs& a) {
+    return kMaxTokens * sizeof(int64_t) + ((a.dim + 3) & ~3) * sizeof(float) + (size_t)a.block_tokens * (a.rotary / 2) * sizeof(float2);
+}
+__device__ __forceinline__ void fill_tables(const RowArgs& a, const RowSegment& sg, const RowTables& s, int64_t t0, int nt) {
+    const int half = a.rotary / 2;
+    if (sg.turn)
+        for (int i = threadIdx.x; i < nt * half; i += blockDim.x) {
+            const int t = i / half;
+            s.cs[i] = turn_at(a, a.positions[t0 + t], i - t * half);
+        }
+    if (sg.weight)
+        for (int i = threadIdx.x; i < a.dim; i += blockDim.x) s.weight[i] = load_weight(sg.weight, sg.weight_dtype, i);
+    if (a.table)
+        for (int t = threadIdx.x; t < nt; t += blockDim.x) s.rows[t] = cache_row(a, t0 + t);
+}
+
+// Each head is handled by `lanes` lanes, each with two slots of V values.
 // HALF: slot 0 holds values of the first half of the rotated part and slot 1
-// their partners; the threads after those take the unrotated rest, two slots
-// each. Interleaved: slots 2l and 2l + 1, whose pairs lie inside a slot.
-template <typename TI, typename TO, bool HALF>
-__global__ void __launch_bounds__(kRowThreads) row_kernel(const RowArgs a) {
-    constexpr int V = 16 / sizeof(TI);
-    extern __shared__ float2 cs_s[];
-    __shared__ int64_t rows_s[kMaxTokens];
+// their partners; the lanes after those take the unrotated rest, two slots
+// each. Interleaved: slots 2l and 2l + 1, whose pairs lie inside a slot. Either
+// way lane l turns pairs l V .. l V + V - 1.
+// A block has the tokens [t0, t0 + nt) of one segment; a warp has one group of
+// heads after another (as many heads as its lanes hold) and goes through the
+// tokens, or shares them where there are fewer groups than warps.
+template <typename TI, typename TO, bool HALF, bool NORM>
+__global__ void __launch_bounds__(kRowThreads, 3) row_kernel(const __grid_constant__ RowArgs a) {
+    constexpr int V = Slot<TI>::V;
+    constexpr int U = kRowSteps;
+    extern __shared__ __align__(16) uint8_t row_smem[];
+    const RowTables tab = row_tables(a, row_smem);
+    const RowSegment& sg = a.seg[blockIdx.z];
     const int64_t t0 = (int64_t)blockIdx.x * a.block_tokens;
     const int nt = (int)min((int64_t)a.block_tokens, a.tokens - t0);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & (a.lanes - 1), groups = 32 / a.lanes;
     const int half = a.rotary / 2;
-    const int lane = threadIdx.x & (a.lanes - 1);
-    // this thread's slots of every head
+    // this lane's slots of every head
     int at0, at1;
     bool turn;
     if (HALF) {
@@ -169,99 +223,99 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const RowArgs a) {
     } else {
         at0 = lane * 2 * V;
         at1 = at0 + V;
-        turn = true;
+        turn = at0 < a.rotary;
     }
-    const bool has0 = at0 < a.dim, has1 = at1 < a.dim;
-    const int per = kRowThreads / a.lanes;  // heads of one step
-    const int total = nt * a.heads;
-    const int step = per * (int)gridDim.y;
-    int r = (int)blockIdx.y * per + threadIdx.x / a.lanes;
+    turn = turn && sg.turn;
+    const bool has1 = at1 < a.dim;
+    // the block's head groups, and the warps that share one
+    const int ng = (sg.heads + groups - 1) / groups, g0 = blockIdx.y * a.part_groups, n = min(ng, g0 + a.part_groups) - g0;
+    if (n <= 0) return;
+    const int cols = min(n, kRowWarps), share = kRowWarps / cols;
+    const int first = warp / cols < share ? warp / cols : nt;  // first token of this warp; then every share-th
+    const int stride = sg.heads * a.dim;                       // values from one token to the next
+    int g = g0 + warp % cols;
+    int h = g * groups + (threadIdx.x & 31) / a.lanes;
+    const TI* src = static_cast<const TI*>(sg.src) + t0 * stride + (int64_t)h * a.dim + at0;
+    const int to1 = at1 - at0;
+    bool live = h < sg.heads && at0 < a.dim;
 
-    Pack<TI, V> x0{}, x1{};
-    auto load = [&](int i) {
-        const int t = i / a.heads, h = i - t * a.heads;
-        const bool second = h >= a.seg[0].heads;
-        const RowSegment& sg = a.seg[second ? 1 : 0];
-        const TI* src = static_cast<const TI*>(sg.src) +
-                        ((t0 + t) * sg.heads + (second ? h - a.seg[0].heads : h)) * a.dim;
-        if (has0) x0 = *reinterpret_cast<const Pack<TI, V>*>(src + at0);
-        if (has1) x1 = *reinterpret_cast<const Pack<TI, V>*>(src + at1);
+    uint4 x0[U], x1[U];
+    auto load = [&](int t) {
+        const TI* p = src + (int64_t)t * stride;
+#pragma unroll
+        for (int u = 0; u < U; ++u, t += share, p += share * stride)
+            if (live && t < nt) {
+                x0[u] = *reinterpret_cast<const uint4*>(p);
+                if (has1) x1[u] = *reinterpret_cast<const uint4*>(p + to1);
+            }
     };
-    // the first heads are on their way while the angles are computed
-    if (r < total) load(r);
-    fill_tables(a, t0, nt, cs_s, rows_s);
+    load(first);
+    fill_tables(a, sg, tab, t0, nt);
     __syncthreads();
-    for (int base = r - (int)(threadIdx.x / a.lanes); base < total; base += step, r += step) {
-        const bool live = r < total;  // a head's lanes agree, so shuffles among them are whole
-        const int i = live ? r : 0;
-        const int t = i / a.heads, h = i - t * a.heads;
-        const bool second = h >= a.seg[0].heads;
-        const RowSegment& sg = a.seg[second ? 1 : 0];
-        float f0[V], f1[V];
+    for (;;) {
+#pragma unroll 1
+        for (int t = first; t < nt;) {
+            const float2* cs = tab.cs + t * half + lane * V;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            f0[j] = to_f32(x0.v[j]);
-            f1[j] = to_f32(x1.v[j]);
-        }
-        if (r + step < total) load(r + step);
-        if (sg.weight) {
-            float ss = 0.0f;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                if (has0) ss = fmaf(f0[j], f0[j], ss);
-                if (has1) ss = fmaf(f1[j], f1[j], ss);
-            }
-            for (int o = a.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float inv = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                if (has0) f0[j] = f0[j] * inv * load_weight(sg.weight, sg.weight_dtype, at0 + j);
-                if (has1) f1[j] = f1[j] * inv * load_weight(sg.weight, sg.weight_dtype, at1 + j);
-            }
-        }
-        if (sg.turn && half) {
-            const float2* cs = cs_s + t * half;
-            if (HALF) {
-                if (turn) {
+            for (int u = 0; u < U; ++u, t += share, cs += share * half) {
+                if (t >= nt) break;  // the warp's lanes agree
+                float f0[V], f1[V];
+                Slot<TI>::unpack(x0[u], f0);
+                Slot<TI>::unpack(x1[u], f1);
+                if (NORM) {
+                    float ss = 0.0f;
 #pragma unroll
                     for (int j = 0; j < V; ++j) {
-                        const float2 c = cs[at0 + j];
-                        const float u = f0[j], w = f1[j];
-                        f0[j] = u * c.x - w * c.y;
-                        f1[j] = w * c.x + u * c.y;
+                        if (live) ss = fmaf(f0[j], f0[j], ss);
+                        if (live && has1) ss = fmaf(f1[j], f1[j], ss);
+                    }
+                    for (int o = a.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                    const float inv = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
+                    if (live) {
+#pragma unroll
+                        for (int j = 0; j < V; j += 4) {
+                            const float4 p = *reinterpret_cast<const float4*>(tab.weight + at0 + j);
+                            f0[j] *= inv * p.x, f0[j + 1] *= inv * p.y, f0[j + 2] *= inv * p.z, f0[j + 3] *= inv * p.w;
+                            if (has1) {
+                                const float4 q = *reinterpret_cast<const float4*>(tab.weight + at1 + j);
+                                f1[j] *= inv * q.x, f1[j + 1] *= inv * q.y, f1[j + 2] *= inv * q.z, f1[j + 3] *= inv * q.w;
+                            }
+                        }
                     }
                 }
-            } else {
+                if (turn) {
 #pragma unroll
-                for (int j = 0; j < V; j += 2) {
-                    if (at0 + j < a.rotary) {
-                        const float2 c = cs[(at0 + j) / 2];
-                        const float u = f0[j], w = f0[j + 1];
-                        f0[j] = u * c.x - w * c.y;
-                        f0[j + 1] = u * c.y + w * c.x;
-                    }
-                    if (at1 + j < a.rotary) {
-                        const float2 c = cs[(at1 + j) / 2];
-                        const float u = f1[j], w = f1[j + 1];
-                        f1[j] = u * c.x - w * c.y;
-                        f1[j + 1] = u * c.y + w * c.x;
+                    for (int j = 0; j < V; j += 2) {
+                        // pairs lane V + j and + j + 1 (the rotated part has a multiple of 4 values)
+                        if (!HALF && at0 + 2 * j >= a.rotary) continue;
+                        const float4 c = *reinterpret_cast<const float4*>(cs + j);
+                        float& p0 = HALF ? f0[j] : (2 * j < V ? f0[(2 * j) % V] : f1[(2 * j) % V]);
+                        float& p1 = HALF ? f1[j] : (2 * j < V ? f0[(2 * j + 1) % V] : f1[(2 * j + 1) % V]);
+                        float& q0 = HALF ? f0[j + 1] : (2 * j < V ? f0[(2 * j + 2) % V] : f1[(2 * j + 2) % V]);
+                        float& q1 = HALF ? f1[j + 1] : (2 * j < V ? f0[(2 * j + 3) % V] : f1[(2 * j + 3) % V]);
+                        const float x = p0, y = p1;
+                        p0 = x * c.x - y * c.y;
+                        p1 = y * c.x + x * c.y;
+                        const float z = q0, w = q1;
+                        q0 = z * c.z - w * c.w;
+                        q1 = w * c.z + z * c.w;
                     }
                 }
+                const int64_t row = a.table ? tab.rows[t] : t0 + t;
+                if (live && row >= 0) {
+                    TO* dst = static_cast<TO*>(sg.dst) + row * stride + (h * a.dim + at0);
+                    store_slot<TO, V>(dst, f0);
+                    if (has1) store_slot<TO, V>(dst + to1, f1);
+                }
             }
+            if (t < nt) load(t);
         }
-        int64_t row = t0 + t;
-        if (a.table) row = rows_s[t];
-        if (live && row >= 0) {
-            Pack<TO, V> y0, y1;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                y0.v[j] = from_f32<TO>(f0[j]);
-                y1.v[j] = from_f32<TO>(f1[j]);
-            }
-            TO* dst = static_cast<TO*>(sg.dst) + (row * sg.heads + (second ? h - a.seg[0].heads : h)) * a.dim;
-            if (has0) *reinterpret_cast<Pack<TO, V>*>(dst + at0) = y0;
-            if (has1) *reinterpret_cast<Pack<TO, V>*>(dst + at1) = y1;
-        }
+        g += cols;
+        if (g >= g0 + n) break;
+        h += cols * groups;
+        src += (int64_t)cols * groups * a.dim;
+        live = h < sg.heads && at0 < a.dim;
+        load(first);
     }
 }
 
@@ -280,54 +334,53 @@ __device__ __forceinline__ void st_value(void* p, int32_t dtype, int64_t i, floa
     }
 }
 
-// The same for dims and addresses that 16-byte slots do not fit: one warp per
-// head, a pair of values at a time (rotated pairs, then the rest two by two).
-__global__ void __launch_bounds__(kRowThreads) row_scalar_kernel(const RowArgs a, int32_t ti, int32_t to, bool half_layout) {
-    extern __shared__ float2 cs_s[];
-    __shared__ int64_t rows_s[kMaxTokens];
+// The same for dims and addresses that 16-byte slots do not fit: a head at a
+// time, a pair of values a lane (rotated pairs, then the rest two by two).
+__global__ void __launch_bounds__(kRowThreads) row_scalar_kernel(const __grid_constant__ RowArgs a, int32_t ti, int32_t to, bool half_layout) {
+    constexpr int N = kMaxHeadDim / 64;  // pairs of a lane
+    extern __shared__ __align__(16) uint8_t row_smem[];
+    const RowSegment& sg = a.seg[blockIdx.z];
+    const bool norm = sg.weight != nullptr;
+    const RowTables tab = row_tables(a, row_smem);
     const int64_t t0 = (int64_t)blockIdx.x * a.block_tokens;
     const int nt = (int)min((int64_t)a.block_tokens, a.tokens - t0);
-    const int half = a.rotary / 2, lane = threadIdx.x & 31;
-    fill_tables(a, t0, nt, cs_s, rows_s);
+    const int lane = threadIdx.x & 31;
+    const int half = a.rotary / 2, pairs = half + (a.dim - a.rotary + 1) / 2;
+    const int g0 = blockIdx.y * a.part_groups, n = min(sg.heads, g0 + a.part_groups) - g0;
+    if (n <= 0) return;
+    fill_tables(a, sg, tab, t0, nt);
     __syncthreads();
-    const int pairs = half + (a.dim - a.rotary + 1) / 2;
-    for (int r = (int)(blockIdx.y * (kRowThreads / 32) + threadIdx.x / 32); r < nt * a.heads;
-         r += (kRowThreads / 32) * (int)gridDim.y) {
-        const int t = r / a.heads, h = r - t * a.heads;
-        const bool second = h >= a.seg[0].heads;
-        const RowSegment& sg = a.seg[second ? 1 : 0];
-        const int hh = second ? h - a.seg[0].heads : h;
-        const int64_t src = ((t0 + t) * sg.heads + hh) * a.dim;
-        const int64_t row = a.table ? rows_s[t] : t0 + t;
-        float u[kMaxHeadDim / 64], w[kMaxHeadDim / 64];
+    for (int i = threadIdx.x >> 5; i < nt * n; i += kRowWarps) {
+        const int t = i / n, h = g0 + i % n;
+        const int64_t row = a.table ? tab.rows[t] : t0 + t;
+        const int64_t src = ((t0 + t) * sg.heads + h) * a.dim, dst = (row * sg.heads + h) * a.dim;
+        const float* weight = tab.weight;
+        float u[N], w[N];
         float ss = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kMaxHeadDim / 64; ++k) {
+        for (int k = 0; k < N; ++k) {
             const int j = lane + 32 * k;
-            if (j >= pairs) break;
             const int i0 = j < half ? (half_layout ? j : 2 * j) : a.rotary + 2 * (j - half);
             const int i1 = j < half && half_layout ? j + half : i0 + 1;
-            u[k] = ld_value(sg.src, ti, src + i0);
-            w[k] = i1 < a.dim ? ld_value(sg.src, ti, src + i1) : 0.0f;
+            u[k] = j < pairs ? ld_value(sg.src, ti, src + i0) : 0.0f;
+            w[k] = j < pairs && i1 < a.dim ? ld_value(sg.src, ti, src + i1) : 0.0f;
             ss = fmaf(u[k], u[k], fmaf(w[k], w[k], ss));
         }
-        float inv = 1.0f;
-        if (sg.weight) inv = 1.0f / sqrtf(warp_sum(ss) / (float)a.dim + a.eps);
+        const float inv = norm ? 1.0f / sqrtf(warp_sum(ss) / (float)a.dim + a.eps) : 1.0f;
         if (row < 0) continue;
-        const int64_t dst = (row * sg.heads + hh) * a.dim;
 #pragma unroll
-        for (int k = 0; k < kMaxHeadDim / 64; ++k) {
+        for (int k = 0; k < N; ++k) {
             const int j = lane + 32 * k;
-            if (j >= pairs) break;
+            if (j >= pairs) continue;
             const int i0 = j < half ? (half_layout ? j : 2 * j) : a.rotary + 2 * (j - half);
             const int i1 = j < half && half_layout ? j + half : i0 + 1;
             float x = u[k], y = w[k];
-            if (sg.weight) {
-                x = x * inv * load_weight(sg.weight, sg.weight_dtype, i0);
-                if (i1 < a.dim) y = y * inv * load_weight(sg.weight, sg.weight_dtype, i1);
+            if (norm) {
+                x *= inv * weight[i0];
+                if (i1 < a.dim) y *= inv * weight[i1];
             }
             if (sg.turn && j < half) {
-                const float2 c = cs_s[t * half + j];
+                const float2 c = tab.cs[t * half + j];
                 const float x2 = x * c.x - y * c.y;
                 y = y * c.x + x * c.y;
                 x = x2;
@@ -338,60 +391,56 @@ __global__ void __launch_bounds__(kRowThreads) row_scalar_kernel(const RowArgs a
     }
 }
 
-template <typename TI, typename TO>
+template <typename TI, typename TO, bool NORM>
 void launch_rows_t(const RowArgs& a, bool half_layout, dim3 grid, size_t smem, cudaStream_t s) {
     if (half_layout)
-        row_kernel<TI, TO, true><<<grid, kRowThreads, smem, s>>>(a);
+        row_kernel<TI, TO, true, NORM><<<grid, kRowThreads, smem, s>>>(a);
     else
-        row_kernel<TI, TO, false><<<grid, kRowThreads, smem, s>>>(a);
+        row_kernel<TI, TO, false, NORM><<<grid, kRowThreads, smem, s>>>(a);
+}
+
+template <typename TI>
+void launch_rows_to(const RowArgs& a, int32_t to, bool half_layout, dim3 grid, size_t smem, cudaStream_t s) {
+    if (a.seg[0].weight) launch_rows_t<TI, TI, true>(a, half_layout, grid, smem, s);  // norms keep the dtype
+    else if (to == BEACON_CUDA_DTYPE_F32) launch_rows_t<TI, float, false>(a, half_layout, grid, smem, s);
+    else if (to == BEACON_CUDA_DTYPE_F16) launch_rows_t<TI, __half, false>(a, half_layout, grid, smem, s);
+    else launch_rows_t<TI, __nv_bfloat16, false>(a, half_layout, grid, smem, s);
 }
 
 void launch_rows(BeaconCudaContext* ctx, RowArgs a, int32_t ti, int32_t to, const BeaconCudaRope* rope, cudaStream_t s) {
-    a.heads = a.seg[0].heads + a.seg[1].heads;
-    if (a.tokens == 0 || a.heads == 0 || a.dim == 0) return;
+    if (a.tokens == 0) return;
     const bool half_layout = rope && rope->layout == BEACON_CUDA_ROPE_HALF;
     if (rope) {
         a.rotary = rope->rotary_dim;
         a.amplitude = rope->amplitude;
         a.turns = static_cast<const double*>(rope->turns->ptr);
     }
-    const int esize = (int)plain_elem_bytes(ti), V = 16 / esize;
+    const int V = 16 / (int)plain_elem_bytes(ti);
     const int slots = half_layout ? a.rotary / 2 / V + (a.dim - a.rotary + 2 * V - 1) / (2 * V) : (a.dim + 2 * V - 1) / (2 * V);
     bool vec = a.dim % V == 0 && a.rotary % (half_layout ? 2 * V : V) == 0 && slots <= 32;
     for (const RowSegment& sg : a.seg)
-        vec = vec && aligned16(sg.src) &&
-              reinterpret_cast<uintptr_t>(sg.dst) % (V * plain_elem_bytes(to)) == 0;
-    int per = kRowThreads / 32;  // heads of a block's step
-    if (vec) {
-        a.lanes = 1;
-        while (a.lanes < slots) a.lanes *= 2;
-        per = kRowThreads / a.lanes;
-    }
-    // one step of the block's threads covers a block's heads, and more blocks
-    // than that share them while the device is not full (small batches)
-    a.block_tokens = std::min(kMaxTokens, std::max(1, per / a.heads));
+        vec = vec && aligned16(sg.src) && reinterpret_cast<uintptr_t>(sg.dst) % (V * plain_elem_bytes(to)) == 0;
+    a.lanes = 32;
+    while (vec && a.lanes / 2 >= slots) a.lanes /= 2;
+    const int hpg = vec ? 32 / a.lanes : 1;
+    const int groups = (std::max(a.seg[0].heads, a.seg[1].heads) + hpg - 1) / hpg, segs = a.seg[1].heads ? 2 : 1;
+    // A block's warps have eight steps each (so the tables cost little) while
+    // that leaves four blocks an SM; fewer tokens, then a token's groups shared
+    // out, as the device would stay empty.
+    const int64_t want = (4 * ctx->sm_count + segs - 1) / segs;
+    int64_t tokens = std::clamp<int64_t>(8 * kRowWarps / groups, 1, kMaxTokens);
+    if (a.rotary) tokens = std::clamp<int64_t>(8192 / a.rotary, 1, tokens);  // 32 KB of angles
+    a.block_tokens = (int)std::clamp<int64_t>(a.tokens / want, 1, tokens);
     const int64_t blocks = (a.tokens + a.block_tokens - 1) / a.block_tokens;
     if (blocks > 0x7FFFFFFF) shape_err("too many tokens");
-    const int steps = (a.block_tokens * a.heads + per - 1) / per;
-    a.parts = (int)std::min<int64_t>(steps, std::max<int64_t>(1, 4 * ctx->sm_count / blocks));
-    const dim3 grid((unsigned)blocks, (unsigned)std::min(a.parts, 65535));
-    // at most 16 KB: the angles of the values that one step of the threads holds
-    const size_t smem = (size_t)a.block_tokens * (a.rotary / 2) * sizeof(float2);
-    if (!vec) {
-        row_scalar_kernel<<<grid, kRowThreads, smem, s>>>(a, ti, to, half_layout);
-        BC_LAUNCHED("row_scalar_kernel");
-        return;
-    }
-    const int32_t F32 = BEACON_CUDA_DTYPE_F32, F16 = BEACON_CUDA_DTYPE_F16, BF16 = BEACON_CUDA_DTYPE_BF16;
-    if (ti == F32 && to == F32) launch_rows_t<float, float>(a, half_layout, grid, smem, s);
-    else if (ti == F32 && to == F16) launch_rows_t<float, __half>(a, half_layout, grid, smem, s);
-    else if (ti == F32 && to == BF16) launch_rows_t<float, __nv_bfloat16>(a, half_layout, grid, smem, s);
-    else if (ti == F16 && to == F16) launch_rows_t<__half, __half>(a, half_layout, grid, smem, s);
-    else if (ti == F16 && to == F32) launch_rows_t<__half, float>(a, half_layout, grid, smem, s);
-    else if (ti == F16 && to == BF16) launch_rows_t<__half, __nv_bfloat16>(a, half_layout, grid, smem, s);
-    else if (ti == BF16 && to == BF16) launch_rows_t<__nv_bfloat16, __nv_bfloat16>(a, half_layout, grid, smem, s);
-    else if (ti == BF16 && to == F16) launch_rows_t<__nv_bfloat16, __half>(a, half_layout, grid, smem, s);
-    else launch_rows_t<__nv_bfloat16, float>(a, half_layout, grid, smem, s);
+    const int64_t parts = std::clamp<int64_t>(want / blocks, 1, (groups + kRowWarps - 1) / kRowWarps);
+    a.part_groups = (int)((groups + parts - 1) / parts);
+    const dim3 grid((unsigned)blocks, (unsigned)((groups + a.part_groups - 1) / a.part_groups), (unsigned)segs);
+    const size_t smem = row_tables_bytes(a);
+    if (!vec) row_scalar_kernel<<<grid, kRowThreads, smem, s>>>(a, ti, to, half_layout);
+    else if (ti == BEACON_CUDA_DTYPE_F32) launch_rows_to<float>(a, to, half_layout, grid, smem, s);
+    else if (ti == BEACON_CUDA_DTYPE_F16) launch_rows_to<__half>(a, to, half_layout, grid, smem, s);
+    else launch_rows_to<__nv_bfloat16>(a, to, half_layout, grid, smem, s);
     BC_LAUNCHED("row_kernel");
 }
 
