@@ -9,7 +9,7 @@
 //
 // A block takes a few tokens. A head is held by as many lanes as its 2 x
 // 16-byte slots need, so a warp has several heads at a time, and the loads of
-// its next four steps (128 bytes a lane) are in flight at once. The sines and
+// its next two tokens (64 bytes a lane, 32 warps an SM) are in flight at once. The sines and
 // cosines of the block's tokens are computed once into shared memory while the
 // first loads are on their way: the angle is a 64-bit product position * f_i /
 // 2 pi reduced to one turn, then sincospif in 32 bits, so position 10^6 is as
@@ -66,7 +66,7 @@ constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kMaxTokens = 32;  // of a block
 constexpr int kMaxHeadDim = 512;
-constexpr int kRowSteps = 4;  // heads whose loads a lane has in flight: 128 bytes
+constexpr int kRowSteps = 2;  // tokens whose loads a lane has in flight: 64 bytes, four blocks an SM
 
 struct RowSegment {                // heads of one input tensor
     const void* src = nullptr;     // [T][heads][dim]
@@ -81,7 +81,7 @@ struct RowArgs {
     RowSegment seg[2];
     int64_t tokens = 0;
     int dim = 0, rotary = 0;
-    float eps = 0.0f, amplitude = 1.0f;
+    float eps = 0.0f, inv_dim = 0.0f, amplitude = 1.0f;
     const int32_t* positions = nullptr;
     const double* turns = nullptr;  // [rotary / 2]
     // cache pages
@@ -123,6 +123,9 @@ template <>
 struct Slot<__half> : Slot16<__half> {};
 template <>
 struct Slot<__nv_bfloat16> : Slot16<__nv_bfloat16> {};
+
+__device__ __forceinline__ float2 get2(const float* f) { return make_float2(f[0], f[1]); }
+__device__ __forceinline__ void put2(float* f, float2 v) { f[0] = v.x, f[1] = v.y; }
 
 template <typename T, int V>
 __device__ __forceinline__ void store_slot(T* dst, const float* f) {
@@ -166,26 +169,32 @@ __device__ __forceinline__ float2 turn_at(const RowArgs& a, int position, int pa
 // What a block computes before its heads: sines and cosines, norm weights in 32
 // bits, cache rows.
 struct RowTables {
-    float2* cs;      // [tokens][rotary / 2]
+    float* cos;      // [tokens][half_stride]: rotary / 2 entries, rows 16-byte aligned
+    float* sin;      // the same
     float* weight;   // [dim]
     int64_t* rows;   // [tokens]
 };
+__host__ __device__ __forceinline__ int half_stride(const RowArgs& a) { return (a.rotary / 2 + 3) & ~3; }
 __device__ __forceinline__ RowTables row_tables(const RowArgs& a, uint8_t* smem) {
     RowTables s;
     s.rows = reinterpret_cast<int64_t*>(smem);
     s.weight = reinterpret_cast<float*>(s.rows + kMaxTokens);
-    s.cs = reinterpret_cast<float2*>(s.weight + ((a.dim + 3) & ~3));
+    s.cos = s.weight + ((a.dim + 3) & ~3);
+    s.sin = s.cos + a.block_tokens * half_stride(a);
     return s;
 }
 inline size_t row_tables_bytes(const RowArgs& a) {
-    return kMaxTokens * sizeof(int64_t) + ((a.dim + 3) & ~3) * sizeof(float) + (size_t)a.block_tokens * (a.rotary / 2) * sizeof(float2);
+    return kMaxTokens * sizeof(int64_t) + ((a.dim + 3) & ~3) * sizeof(float) + 2 * (size_t)a.block_tokens * half_stride(a) * sizeof(float);
 }
 __device__ __forceinline__ void fill_tables(const RowArgs& a, const RowSegment& sg, const RowTables& s, int64_t t0, int nt) {
     const int half = a.rotary / 2;
     if (sg.turn)
         for (int i = threadIdx.x; i < nt * half; i += blockDim.x) {
             const int t = i / half;
-            s.cs[i] = turn_at(a, a.positions[t0 + t], i - t * half);
+            const int pair = i - t * half, at = t * half_stride(a) + pair;
+            const float2 c = turn_at(a, a.positions[t0 + t], pair);
+            s.cos[at] = c.x;
+            s.sin[at] = c.y;
         }
     if (sg.weight)
         for (int i = threadIdx.x; i < a.dim; i += blockDim.x) s.weight[i] = load_weight(sg.weight, sg.weight_dtype, i);
@@ -202,7 +211,7 @@ __device__ __forceinline__ void fill_tables(const RowArgs& a, const RowSegment& 
 // heads after another (as many heads as its lanes hold) and goes through the
 // tokens, or shares them where there are fewer groups than warps.
 template <typename TI, typename TO, bool HALF, bool NORM>
-__global__ void __launch_bounds__(kRowThreads, 3) row_kernel(const __grid_constant__ RowArgs a) {
+__global__ void __launch_bounds__(kRowThreads, 4) row_kernel(const __grid_constant__ RowArgs a) {
     constexpr int V = Slot<TI>::V;
     constexpr int U = kRowSteps;
     extern __shared__ __align__(16) uint8_t row_smem[];
@@ -211,7 +220,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) row_kernel(const __grid_consta
     const int64_t t0 = (int64_t)blockIdx.x * a.block_tokens;
     const int nt = (int)min((int64_t)a.block_tokens, a.tokens - t0);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & (a.lanes - 1), groups = 32 / a.lanes;
-    const int half = a.rotary / 2;
+    const int half = a.rotary / 2, hs = half_stride(a);
     // this lane's slots of every head
     int at0, at1;
     bool turn;
@@ -255,9 +264,9 @@ __global__ void __launch_bounds__(kRowThreads, 3) row_kernel(const __grid_consta
     for (;;) {
 #pragma unroll 1
         for (int t = first; t < nt;) {
-            const float2* cs = tab.cs + t * half + lane * V;
+            int at = t * hs + lane * V;  // this lane's first pair in the tables
 #pragma unroll
-            for (int u = 0; u < U; ++u, t += share, cs += share * half) {
+            for (int u = 0; u < U; ++u, t += share, at += share * hs) {
                 if (t >= nt) break;  // the warp's lanes agree
                 float f0[V], f1[V];
                 Slot<TI>::unpack(x0[u], f0);
@@ -270,35 +279,49 @@ __global__ void __launch_bounds__(kRowThreads, 3) row_kernel(const __grid_consta
                         if (live && has1) ss = fmaf(f1[j], f1[j], ss);
                     }
                     for (int o = a.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                    const float inv = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
+                    const float inv = rsqrtf(fmaf(ss, a.inv_dim, a.eps));
                     if (live) {
 #pragma unroll
                         for (int j = 0; j < V; j += 4) {
+                            const float2 in = make_float2(inv, inv);
                             const float4 p = *reinterpret_cast<const float4*>(tab.weight + at0 + j);
-                            f0[j] *= inv * p.x, f0[j + 1] *= inv * p.y, f0[j + 2] *= inv * p.z, f0[j + 3] *= inv * p.w;
+                            put2(f0 + j, mul2(get2(f0 + j), mul2(in, make_float2(p.x, p.y))));
+                            put2(f0 + j + 2, mul2(get2(f0 + j + 2), mul2(in, make_float2(p.z, p.w))));
                             if (has1) {
                                 const float4 q = *reinterpret_cast<const float4*>(tab.weight + at1 + j);
-                                f1[j] *= inv * q.x, f1[j + 1] *= inv * q.y, f1[j + 2] *= inv * q.z, f1[j + 3] *= inv * q.w;
+                                put2(f1 + j, mul2(get2(f1 + j), mul2(in, make_float2(q.x, q.y))));
+                                put2(f1 + j + 2, mul2(get2(f1 + j + 2), mul2(in, make_float2(q.z, q.w))));
                             }
                         }
                     }
                 }
                 if (turn) {
 #pragma unroll
-                    for (int j = 0; j < V; j += 2) {
-                        // pairs lane V + j and + j + 1 (the rotated part has a multiple of 4 values)
+                    for (int j = 0; j < V; j += 4) {
+                        // pairs lane V + j .. + 3 (the rotated part has a multiple of 4 values;
+                        // entries of pairs that it does not have are not used)
                         if (!HALF && at0 + 2 * j >= a.rotary) continue;
-                        const float4 c = *reinterpret_cast<const float4*>(cs + j);
-                        float& p0 = HALF ? f0[j] : (2 * j < V ? f0[(2 * j) % V] : f1[(2 * j) % V]);
-                        float& p1 = HALF ? f1[j] : (2 * j < V ? f0[(2 * j + 1) % V] : f1[(2 * j + 1) % V]);
-                        float& q0 = HALF ? f0[j + 1] : (2 * j < V ? f0[(2 * j + 2) % V] : f1[(2 * j + 2) % V]);
-                        float& q1 = HALF ? f1[j + 1] : (2 * j < V ? f0[(2 * j + 3) % V] : f1[(2 * j + 3) % V]);
-                        const float x = p0, y = p1;
-                        p0 = x * c.x - y * c.y;
-                        p1 = y * c.x + x * c.y;
-                        const float z = q0, w = q1;
-                        q0 = z * c.z - w * c.w;
-                        q1 = w * c.z + z * c.w;
+                        const float4 c = *reinterpret_cast<const float4*>(tab.cos + at + j), s = *reinterpret_cast<const float4*>(tab.sin + at + j);
+                        if (HALF) {
+                            const float2 c2[2] = {make_float2(c.x, c.y), make_float2(c.z, c.w)}, s2[2] = {make_float2(s.x, s.y), make_float2(s.z, s.w)};
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const float2 x = get2(f0 + j + 2 * i), y = get2(f1 + j + 2 * i);
+                                put2(f0 + j + 2 * i, fma2(make_float2(-y.x, -y.y), s2[i], mul2(x, c2[i])));
+                                put2(f1 + j + 2 * i, fma2(x, s2[i], mul2(y, c2[i])));
+                            }
+                        } else {
+                            const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                // pair j + i of the lane's 2 V values
+                                float* f = 2 * (j + i) < V ? f0 + 2 * (j + i) : f1 + 2 * (j + i) - V;
+                                if (at0 + 2 * (j + i) >= a.rotary) continue;
+                                const float x = f[0], y = f[1];
+                                f[0] = x * cv[i] - y * sv[i];
+                                f[1] = y * cv[i] + x * sv[i];
+                            }
+                        }
                     }
                 }
                 const int64_t row = a.table ? tab.rows[t] : t0 + t;
@@ -366,7 +389,7 @@ __global__ void __launch_bounds__(kRowThreads) row_scalar_kernel(const __grid_co
             w[k] = j < pairs && i1 < a.dim ? ld_value(sg.src, ti, src + i1) : 0.0f;
             ss = fmaf(u[k], u[k], fmaf(w[k], w[k], ss));
         }
-        const float inv = norm ? 1.0f / sqrtf(warp_sum(ss) / (float)a.dim + a.eps) : 1.0f;
+        const float inv = norm ? rsqrtf(fmaf(warp_sum(ss), a.inv_dim, a.eps)) : 1.0f;
         if (row < 0) continue;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
@@ -380,7 +403,7 @@ __global__ void __launch_bounds__(kRowThreads) row_scalar_kernel(const __grid_co
                 if (i1 < a.dim) y *= inv * weight[i1];
             }
             if (sg.turn && j < half) {
-                const float2 c = tab.cs[t * half + j];
+                const float2 c = make_float2(tab.cos[t * half_stride(a) + j], tab.sin[t * half_stride(a) + j]);
                 const float x2 = x * c.x - y * c.y;
                 y = y * c.x + x * c.y;
                 x = x2;
@@ -409,6 +432,7 @@ void launch_rows_to(const RowArgs& a, int32_t to, bool half_layout, dim3 grid, s
 
 void launch_rows(BeaconCudaContext* ctx, RowArgs a, int32_t ti, int32_t to, const BeaconCudaRope* rope, cudaStream_t s) {
     if (a.tokens == 0) return;
+    a.inv_dim = 1.0f / (float)a.dim;
     const bool half_layout = rope && rope->layout == BEACON_CUDA_ROPE_HALF;
     if (rope) {
         a.rotary = rope->rotary_dim;

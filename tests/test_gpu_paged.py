@@ -96,7 +96,7 @@ def test_rope_scaled(be, s, dtype, layout, scaling, T, H, D, rd):
 @pytest.mark.parametrize("layout", ["interleaved", "half"])
 @pytest.mark.parametrize("T,H,D,rd,offset", [(3, 2, 6, 4, 0), (2, 5, 80, 20, 0), (4, 3, 128, 128, 1), (2, 2, 7, 2, 3),
                                              (1, 1, 512, 512, 0), (2, 1, 512, 384, 0), (5, 70, 64, 64, 0),
-                                             (300, 2, 96, 48, 0)])
+                                             (300, 2, 96, 48, 0), (9, 3, 24, 12, 0), (700, 3, 64, 20, 0)])
 def test_rope_odd_sizes_and_alignment(be, s, dtype, layout, T, H, D, rd, offset):
     """Head sizes and addresses that 16-byte loads do not fit, and the largest head."""
     rng = np.random.default_rng(D + offset)
