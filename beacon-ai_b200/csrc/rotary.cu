@@ -9,7 +9,7 @@
 //
 // A block takes a few tokens. A head is held by as many lanes as its 2 x
 // 16-byte slots need, so a warp has several heads at a time, and the loads of
-// its next two tokens (64 bytes a lane, 32 warps an SM) are in flight at once. The sines and
+// its next two tokens (64 bytes a lane, 32 warps an SM) are always in flight. The sines and
 // cosines of the block's tokens are computed once into shared memory while the
 // first loads are on their way: the angle is a 64-bit product position * f_i /
 // 2 pi reduced to one turn, then sincospif in 32 bits, so position 10^6 is as
@@ -93,6 +93,7 @@ struct RowArgs {
     int lanes = 1;         // of one head (power of two)
     int block_tokens = 1;  // tokens of a block
     int part_groups = 0;   // head groups (heads that a warp holds at a time) of a block, of each token
+    int parts0 = 0;        // blocks (grid.y) that share the first segment's heads; the others have the second's
 };
 
 // 16 bytes of values as floats, and floats stored as values, two at a time: 16-bit
@@ -216,7 +217,8 @@ __global__ void __launch_bounds__(kRowThreads, 4) row_kernel(const __grid_consta
     constexpr int U = kRowSteps;
     extern __shared__ __align__(16) uint8_t row_smem[];
     const RowTables tab = row_tables(a, row_smem);
-    const RowSegment& sg = a.seg[blockIdx.z];
+    const int second = (int)blockIdx.y >= a.parts0, part = blockIdx.y - (second ? a.parts0 : 0);
+    const RowSegment& sg = a.seg[second];
     const int64_t t0 = (int64_t)blockIdx.x * a.block_tokens;
     const int nt = (int)min((int64_t)a.block_tokens, a.tokens - t0);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & (a.lanes - 1), groups = 32 / a.lanes;
@@ -237,8 +239,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) row_kernel(const __grid_consta
     turn = turn && sg.turn;
     const bool has1 = at1 < a.dim;
     // the block's head groups, and the warps that share one
-    const int ng = (sg.heads + groups - 1) / groups, g0 = blockIdx.y * a.part_groups, n = min(ng, g0 + a.part_groups) - g0;
-    if (n <= 0) return;
+    const int ng = (sg.heads + groups - 1) / groups, g0 = part * a.part_groups, n = min(ng, g0 + a.part_groups) - g0;
     const int cols = min(n, kRowWarps), share = kRowWarps / cols;
     const int first = warp / cols < share ? warp / cols : nt;  // first token of this warp; then every share-th
     const int stride = sg.heads * a.dim;                       // values from one token to the next
@@ -249,16 +250,15 @@ __global__ void __launch_bounds__(kRowThreads, 4) row_kernel(const __grid_consta
     bool live = h < sg.heads && at0 < a.dim;
 
     uint4 x0[U], x1[U];
-    auto load = [&](int t) {
-        const TI* p = src + (int64_t)t * stride;
-#pragma unroll
-        for (int u = 0; u < U; ++u, t += share, p += share * stride)
-            if (live && t < nt) {
-                x0[u] = *reinterpret_cast<const uint4*>(p);
-                if (has1) x1[u] = *reinterpret_cast<const uint4*>(p + to1);
-            }
+    auto load = [&](int u, int t) {
+        if (live && t < nt) {
+            const TI* p = src + t * (int64_t)stride;
+            x0[u] = *reinterpret_cast<const uint4*>(p);
+            if (has1) x1[u] = *reinterpret_cast<const uint4*>(p + to1);
+        }
     };
-    load(first);
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(u, first + u * share);
     fill_tables(a, sg, tab, t0, nt);
     __syncthreads();
     for (;;) {
@@ -271,6 +271,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) row_kernel(const __grid_consta
                 float f0[V], f1[V];
                 Slot<TI>::unpack(x0[u], f0);
                 Slot<TI>::unpack(x1[u], f1);
+                load(u, t + U * share);
                 if (NORM) {
                     float ss = 0.0f;
 #pragma unroll
@@ -331,14 +332,14 @@ __global__ void __launch_bounds__(kRowThreads, 4) row_kernel(const __grid_consta
                     if (has1) store_slot<TO, V>(dst + to1, f1);
                 }
             }
-            if (t < nt) load(t);
         }
         g += cols;
         if (g >= g0 + n) break;
         h += cols * groups;
         src += (int64_t)cols * groups * a.dim;
         live = h < sg.heads && at0 < a.dim;
-        load(first);
+#pragma unroll
+        for (int u = 0; u < U; ++u) load(u, first + u * share);
     }
 }
 
@@ -362,15 +363,15 @@ __device__ __forceinline__ void st_value(void* p, int32_t dtype, int64_t i, floa
 __global__ void __launch_bounds__(kRowThreads) row_scalar_kernel(const __grid_constant__ RowArgs a, int32_t ti, int32_t to, bool half_layout) {
     constexpr int N = kMaxHeadDim / 64;  // pairs of a lane
     extern __shared__ __align__(16) uint8_t row_smem[];
-    const RowSegment& sg = a.seg[blockIdx.z];
+    const int second = (int)blockIdx.y >= a.parts0, part = blockIdx.y - (second ? a.parts0 : 0);
+    const RowSegment& sg = a.seg[second];
     const bool norm = sg.weight != nullptr;
     const RowTables tab = row_tables(a, row_smem);
     const int64_t t0 = (int64_t)blockIdx.x * a.block_tokens;
     const int nt = (int)min((int64_t)a.block_tokens, a.tokens - t0);
     const int lane = threadIdx.x & 31;
     const int half = a.rotary / 2, pairs = half + (a.dim - a.rotary + 1) / 2;
-    const int g0 = blockIdx.y * a.part_groups, n = min(sg.heads, g0 + a.part_groups) - g0;
-    if (n <= 0) return;
+    const int g0 = part * a.part_groups, n = min(sg.heads, g0 + a.part_groups) - g0;
     fill_tables(a, sg, tab, t0, nt);
     __syncthreads();
     for (int i = threadIdx.x >> 5; i < nt * n; i += kRowWarps) {
@@ -447,19 +448,20 @@ void launch_rows(BeaconCudaContext* ctx, RowArgs a, int32_t ti, int32_t to, cons
     a.lanes = 32;
     while (vec && a.lanes / 2 >= slots) a.lanes /= 2;
     const int hpg = vec ? 32 / a.lanes : 1;
-    const int groups = (std::max(a.seg[0].heads, a.seg[1].heads) + hpg - 1) / hpg, segs = a.seg[1].heads ? 2 : 1;
-    // A block's warps have eight steps each (so the tables cost little) while
-    // that leaves four blocks an SM; fewer tokens, then a token's groups shared
-    // out, as the device would stay empty.
-    const int64_t want = (4 * ctx->sm_count + segs - 1) / segs;
-    int64_t tokens = std::clamp<int64_t>(8 * kRowWarps / groups, 1, kMaxTokens);
-    if (a.rotary) tokens = std::clamp<int64_t>(8192 / a.rotary, 1, tokens);  // 32 KB of angles
-    a.block_tokens = (int)std::clamp<int64_t>(a.tokens / want, 1, tokens);
+    const int g0 = (a.seg[0].heads + hpg - 1) / hpg, g1 = (a.seg[1].heads + hpg - 1) / hpg;
+    // As many blocks as run at once (four an SM), each with a warp per head
+    // group and up to 32 tokens, so that the tables cost little; for fewer
+    // tokens, blocks of one token and fewer groups.
+    const int64_t want = 4 * ctx->sm_count;
+    a.part_groups = (int)std::clamp<int64_t>((g0 + g1) * a.tokens / want, 1, kRowWarps);
+    a.parts0 = (g0 + a.part_groups - 1) / a.part_groups;
+    const int parts = a.parts0 + (g1 + a.part_groups - 1) / a.part_groups;
+    int64_t tokens = kMaxTokens;
+    if (a.rotary) tokens = std::clamp<int64_t>(6144 / a.rotary, 1, tokens);  // 24 KB of angles
+    a.block_tokens = (int)std::clamp<int64_t>((a.tokens * parts + want - 1) / want, 1, tokens);
     const int64_t blocks = (a.tokens + a.block_tokens - 1) / a.block_tokens;
     if (blocks > 0x7FFFFFFF) shape_err("too many tokens");
-    const int64_t parts = std::clamp<int64_t>(want / blocks, 1, (groups + kRowWarps - 1) / kRowWarps);
-    a.part_groups = (int)((groups + parts - 1) / parts);
-    const dim3 grid((unsigned)blocks, (unsigned)((groups + a.part_groups - 1) / a.part_groups), (unsigned)segs);
+    const dim3 grid((unsigned)blocks, (unsigned)parts);
     const size_t smem = row_tables_bytes(a);
     if (!vec) row_scalar_kernel<<<grid, kRowThreads, smem, s>>>(a, ti, to, half_layout);
     else if (ti == BEACON_CUDA_DTYPE_F32) launch_rows_to<float>(a, to, half_layout, grid, smem, s);
