@@ -17,10 +17,7 @@
 //    split likewise.
 // P replaces S in place, 32 keys at a time: the 16 columns of packed weights
 // (then 16 of their remainders) lie where the 32 scores were, and are the A
-// operand of O += P V from tensor memory; V is read N-major. The scores are
-// read twice (maximum, weights; 50 cycles a tile) in short loops: holding all
-// 128 in registers takes straight code of 20 KB, whose first pass through the
-// instruction cache costs 15,000 cycles, more than the work of a small call.
+// operand of O += P V from tensor memory; V is read N-major.
 // Key and value rows come in page by page by tensor copies (TMA) of up to 128
 // rows into a ring of tiles in the 128-byte swizzle, requested by four warps;
 // rows of a value tile that are no keys of the block are zeroed there (their
@@ -117,7 +114,20 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
           "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The wait for the loads above passes their registers on, so that no use of
+// them is moved before it.
+__device__ __forceinline__ void tmem_wait_ld(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
+                   "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]),
+                   "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
+                   "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])::"memory");
+}
+__device__ __forceinline__ void tmem_wait_ld(float (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
+                   "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
+}
 __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
@@ -647,19 +657,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int row = p.rt * BR + (TWO ? s * kTile : 0) + r;  // of the block
             const bool live = row < p.k.rows;
             const int tok = p.k.tok0 + row / a.G;
-            int limit = 0x7FFFFFFF;  // rows behind the block: whatever comes out is not written
-            if (live) {
-                if (p.k.kind) {
-                    limit = min(p.k.len, p.k.len - p.k.nq + row / a.G + 1);
-                } else {
-                    const int b = a.qstarts ? span_of(a.qstarts, a.B, tok) : tok;
-                    limit = 0;
-                    if (b >= 0) {
-                        const SeqInfo si = seq_info(a, b);
-                        limit = min(p.k.key1, min(si.len, si.len - si.nq + (tok - si.q0) + 1));
-                    }
-                }
-            }
             if constexpr (SPLIT) {
                 // the block's queries as two f16 parts: 16 rows a warp, a row at a
                 // time (each lane four values), eight on their way
@@ -698,6 +695,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 arrive(&qfull_bar);
             }
+            int limit = 0x7FFFFFFF;  // rows behind the block: whatever comes out is not written
+            if (live) {
+                if (p.k.kind) {
+                    limit = min(p.k.len, p.k.len - p.k.nq + row / a.G + 1);
+                } else {
+                    const int b = a.qstarts ? span_of(a.qstarts, a.B, tok) : tok;
+                    limit = 0;
+                    if (b >= 0) {
+                        const SeqInfo si = seq_info(a, b);
+                        limit = min(p.k.key1, min(si.len, si.len - si.nq + (tok - si.q0) + 1));
+                    }
+                }
+            }
             wait(&qfull_bar, (uint32_t)(seg & 1));
             if (!ok) break;
             // above zero, so that a masked score (-inf) stays one
@@ -714,28 +724,46 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 const int key = p.k.base + (p.tile + t) * kTile;
                 const int seen = limit - key, skip = p.k.key0 - key;  // columns [skip, seen) are visible
-                const bool whole = __all_sync(0xffffffffu, seen >= kTile && skip <= 0);
-                float v[32];
-                float top = -INFINITY;
+                if (!__all_sync(0xffffffffu, seen >= kTile && skip <= 0)) {
+                    // a tile that not all rows see whole: the scores that are not seen
+                    // become -inf where they lie
 #pragma unroll 1
-                for (int c = 0; c < kTile; c += 32) {
-                    tmem_ld32(s_col + c, v);
-                    tmem_wait_ld();
-                    if (!whole) {
+                    for (int c = 0; c < kTile; c += 16) {
+                        float w[16];
+                        uint32_t x[16];
+                        tmem_ld16(s_col + c, w);
+                        tmem_wait_ld(w);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (c + i >= seen || c + i < skip) v[i] = -INFINITY;
+                        for (int i = 0; i < 16; ++i) x[i] = c + i >= seen || c + i < skip ? 0xFF800000u : __float_as_uint(w[i]);
+                        tmem_st16(s_col + c, x);
                     }
+                    tmem_wait_st();
+                }
+                // Two buffers: the next 32 scores are on their way while these are
+                // used. (They are read twice, maximum and weights: 128 registers for
+                // them, or the maximum of 32 at a time, cost more.)
+                float va[32], vb[32];
+                auto top_of = [&](const float (&v)[32], float top) {
                     float x[4] = {top, v[0], v[1], v[2]};
 #pragma unroll
                     for (int i = 3; i < 27; i += 8)
 #pragma unroll
                         for (int k = 0; k < 4; ++k) x[k] = max3(x[k], v[i + k], v[i + 4 + k]);
-                    x[0] = max3(x[0], v[27], v[28]);
-                    x[1] = max3(x[1], v[29], v[30]);
-                    x[2] = max3(x[2], x[3], v[31]);
-                    top = max3(x[0], x[1], x[2]);
-                }
+                    return max3(max3(x[0], v[27], v[28]), max3(x[1], v[29], v[30]), max3(x[2], x[3], v[31]));
+                };
+                tmem_ld32(s_col, va);
+                tmem_wait_ld(va);
+                tmem_ld32(s_col + 32, vb);
+                float top = top_of(va, -INFINITY);
+                tmem_wait_ld(vb);
+                tmem_ld32(s_col + 64, va);
+                top = top_of(vb, top);
+                tmem_wait_ld(va);
+                tmem_ld32(s_col + 96, vb);
+                top = top_of(va, top);
+                tmem_wait_ld(vb);
+                tmem_ld32(s_col, va);
+                top = top_of(vb, top);
                 const float mx = fmaxf(m, top * cs);
                 const bool move = m != -INFINITY && mx > m + kRescale;
                 if (t >= (TWO ? 1 : 2) && __any_sync(0xffffffffu, move)) {
@@ -747,7 +775,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         uint32_t x[16];
                         const uint32_t o_at = tmem + lane_at + 2 * kTile + s * DP + c;
                         tmem_ld16(o_at, w);
-                        tmem_wait_ld();
+                        tmem_wait_ld(w);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(w[i] * keep);
                         tmem_st16(o_at, x);
@@ -757,15 +785,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const float ref = m == -INFINITY ? 0.0f : m;
                 const float2 cs2 = make_float2(cs, cs), ref2 = make_float2(-ref, -ref);
                 float2 sum[2] = {make_float2(l, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll 1
-                for (int c = 0; c < kTile; c += 32) {
-                    tmem_ld32(s_col + c, v);
-                    tmem_wait_ld();
-                    if (!whole) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (c + i >= seen || c + i < skip) v[i] = -INFINITY;
-                    }
+                auto weights = [&](const float (&v)[32], int c) {
                     uint32_t w[16], w2[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
@@ -778,7 +798,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                     tmem_st16(s_col + c, w);
                     if constexpr (SPLIT) tmem_st16(s_col + c + 16, w2);
-                }
+                };
+                tmem_wait_ld(va);
+                tmem_ld32(s_col + 32, vb);
+                weights(va, 0);
+                tmem_wait_ld(vb);
+                tmem_ld32(s_col + 64, va);
+                weights(vb, 32);
+                tmem_wait_ld(va);
+                tmem_ld32(s_col + 96, vb);
+                weights(va, 64);
+                tmem_wait_ld(vb);
+                weights(vb, 96);
                 sum[0] = add2(sum[0], sum[1]);
                 l = sum[0].x + sum[0].y;
                 tmem_wait_st();
@@ -825,14 +856,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             auto sums_of = [&](int col, float (&v)[16]) {
                 const uint32_t o_at = tmem + lane_at + 2 * kTile + col;
                 tmem_ld16(o_at + (TWO ? s * DP : 0), v);
-                tmem_wait_ld();
+                tmem_wait_ld(v);
                 if (!TWO) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) v[i] *= w0;
                     if (both) {
                         float y[16];
                         tmem_ld16(o_at + DP, y);
-                        tmem_wait_ld();
+                        tmem_wait_ld(y);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) v[i] = fmaf(y[i], w1, v[i]);
                     }
