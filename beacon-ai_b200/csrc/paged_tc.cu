@@ -389,16 +389,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             value = j >= 0 && (j >= pairs || (j & 1) == 0);
             return j < 0 ? f : j >= pairs ? p.n - la + (j - pairs) : value ? j / 2 : j / 2 + la;
         };
-        // this lane's first row of a tile (copies row by row: 32 rows a warp;
-        // tensor copies: a box a lane) and its page
+        // this lane's first key of a tile (copies row by row: 32 rows a warp; tensor
+        // copies: a box a lane), its page, and the cache row: -1 if there is none
         auto pos_of = [&](const Piece& p, int t) {
             return p.k.base + (p.tile + t) * kTile + (a.box ? lane * a.box : pw * 32 + lane);
         };
-        auto page_of = [&](const Piece& p, int f) {
-            bool value;
-            const int pos = f < 2 * p.n ? pos_of(p, key_tile(p, f, value)) : p.k.key1;
-            if (pos >= p.k.key1 || (a.box && lane * a.box >= kTile)) return 0;
+        auto page_of = [&](const Piece& p, int t) {
+            const int pos = pos_of(p, t);
+            if (t >= p.n || pos >= p.k.key1 || (a.box && lane * a.box >= kTile)) return 0;
             return page_id(a, pos < p.k.cut ? p.k.first : p.k.b, pos);
+        };
+        auto row_of = [&](const Piece& p, int t, int page) {
+            const int pos = pos_of(p, t);
+            if (pos >= p.k.key1 || (a.box && lane * a.box >= kTile)) return -1;
+            const int row = (int)page_row(a, page, pos);
+            return row < 0 && a.box ? (int)(a.pages * a.page_size) : row;  // a bad page: a box outside, zeros
         };
         auto room = [&]() {  // waits for the stage of tile `it`
             const uint32_t par = (uint32_t)((it / NST - 1) & 1);
@@ -428,13 +433,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 cp_async16_zfill(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), live ? src + cr * stride : static_cast<const uint8_t*>(cache), live);
             }
         };
-        auto load_tile = [&](const Piece& p, int f, int page) {
-            bool value;
-            const int t = key_tile(p, f, value);
+        auto load_tile = [&](const Piece& p, int t, bool value, int row) {
             if (!room()) return;
-            const int pos = pos_of(p, t);
             if (!a.box) {
-                copy_rows(smem_u32(ring + (size_t)(it % NST) * SM::tile), p, value ? a.cv : a.ck, pw * 32, pos < p.k.key1 ? (int)page_row(a, page, pos) : -1);
+                copy_rows(smem_u32(ring + (size_t)(it % NST) * SM::tile), p, value ? a.cv : a.ck, pw * 32, row);
                 cp_async_commit();
                 ++it;
                 if (it - told > 2) {  // two tiles stay in flight
@@ -446,8 +448,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int st = it++ % NST;
             const int pos0 = p.k.base + (p.tile + t) * kTile;
             const uint32_t dst = smem_u32(ring + (size_t)st * SM::tile);
-            const bool live = lane * a.box < kTile && pos < p.k.key1;
-            if (__any_sync(0xffffffffu, live && pos < p.k.cut && pos + a.box > p.k.cut)) {
+            const bool live = row >= 0;
+            if (pos0 < p.k.cut && pos0 + kTile > p.k.cut && (p.k.cut & (a.box - 1))) {
                 // a box whose rows lie in two tables: this tile row by row
                 if (pw > 0) return;
                 for (int r0 = 0; r0 < kTile; r0 += 32) {
@@ -471,11 +473,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // requests take a hundred cycles each, from all four
             if (pw == 0 && lane == 0) mbar_expect_tx(bar, (uint32_t)(boxes * a.box * DP * 2));
             if (live && (part || lane % kLoadWarps == pw)) {
-                int64_t row = page_row(a, page, pos);
-                if (row < 0) row = a.pages * a.page_size;  // outside: zeros
 #pragma unroll
                 for (int h = 0; h < DP / 64; ++h)
-                    tma_rows(dst + h * (kTile * 128) + lane * a.box * 128, value ? &maps.v : &maps.k, h * 64, p.kvh, (int)row, bar);
+                    tma_rows(dst + h * (kTile * 128) + lane * a.box * 128, value ? &maps.v : &maps.k, h * 64, p.kvh, row, bar);
             }
             if (part) {
                 if (!wait_bar(bar, (uint32_t)(nfix++ & 1), limit_cycles)) {
@@ -496,11 +496,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         int seg = 0;
         for (Piece p = pc; ok && p.u < u1; p.next(a, BR, u1), ++seg) {
             // the first tiles are on their way while the queries are brought in
-            int f = 0, page = page_of(p, 0);
+            // A key tile's pages are fetched when the one before it is requested, and
+            // its rows kept for the value tile, up to LA + 1 of them.
+            int f = 0, page = page_of(p, 0), rows[3] = {-1, -1, -1}, kept = 0;
             auto load_next = [&]() {
-                const int ahead = page_of(p, f + 1);
-                load_tile(p, f++, page);
-                page = ahead;
+                bool value;
+                const int t = key_tile(p, f++, value);
+                int row = rows[0];
+                if (value) {
+                    rows[0] = rows[1];
+                    rows[1] = rows[2];
+                    --kept;
+                } else {
+                    row = row_of(p, t, page);
+                    page = page_of(p, t + 1);
+                    if (kept == 0) rows[0] = row;
+                    else if (kept == 1) rows[1] = row;
+                    else rows[2] = row;
+                    ++kept;
+                }
+                load_tile(p, t, value, row);
             };
             while (ok && f < min(3, 2 * p.n)) load_next();
             if (seg > 0 && !SPLIT) {
