@@ -158,6 +158,7 @@ PartArgs carve_part(Carve& c, const PagedArgs& a, int ctas, int slot_rows, bool 
     p.head = c.take<float>((by_row ? rows : slots) * a.D);
     p.tail_stat = c.take<float2>(slots);
     p.tail = c.take<float>(slots * a.D);
+    p.cuts = c.take<int>(8 * ctas);
     p.by_row = by_row;
     p.slot_rows = slot_rows;
     p.ctas = ctas;

@@ -47,6 +47,10 @@ struct PartArgs {
     float* head = nullptr;    // [T * H][D], or [ctas][slot_rows][D] when !by_row
     float2* tail_stat = nullptr;  // [ctas][slot_rows]
     float* tail = nullptr;        // [ctas][slot_rows][D]
+    // Without prefixes only the row blocks that are cut have to be joined: per
+    // CTA the one whose first part it has, as [8]: last CTA (-1: none), first
+    // token, first row, rows of its sequence's queries, KV head.
+    int* cuts = nullptr;
     int by_row = 0;    // heads are kept per row: a row has both kinds
     int slot_rows = 0;  // rows of a row block, at most 256
     int ctas = 0;       // at most 4096

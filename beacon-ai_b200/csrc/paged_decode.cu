@@ -132,6 +132,7 @@ __global__ void __launch_bounds__(kDecThreads)
     const Shares shares(total, part.ctas);
     const long long u0 = cta < shares.ctas ? shares.begin(cta) : 0, u1 = cta < shares.ctas ? shares.begin(cta + 1) : 0;
     pdl_trigger();
+    if (tid == 0) part.cuts[cta * 8] = -1;  // no row block of this CTA is cut at its end, until one is
     if (u0 < u1) {
         if (before * a.Hkv <= u0 && u0 < (before + mine) * a.Hkv) {
             int b = cb0;
@@ -430,6 +431,14 @@ __global__ void __launch_bounds__(kDecThreads)
                 const long long tile0 = u0 + j - at.tile;  // of this head, in the line
                 const int c0 = shares.of(tile0), c1 = shares.of(tile0 + at.cur.tiles - 1);
                 const bool done = c0 == c1 && at.cur.from == 0;  // no other part anywhere
+                if (tid == 0 && c0 == cta && c1 > c0) {  // the row block whose parts have to be joined
+                    int* rec = part.cuts + cta * 8;
+                    rec[0] = c1;
+                    rec[1] = at.b;
+                    rec[2] = 0;
+                    rec[3] = a.G;
+                    rec[4] = at.kvh;
+                }
                 for (int g = tid / (DP / 4); g < a.G; g += QR) {
                     float mw[kDecWarps], M = -INFINITY;
 #pragma unroll
@@ -486,24 +495,25 @@ __global__ void __launch_bounds__(kDecThreads)
     pdl_wait();
 }
 
-// The parts of the query rows: kind 1, kind 0 where the row has it, each a
-// first part and those of the CTAs after it. One warp per row. What is where
-// stands in the row's entry, so nothing else has to be looked up first.
+// The parts of the query rows where there are prefixes: kind 1, kind 0 where the
+// row has it, each a first part and those of the CTAs after it. One warp per
+// row. What is where stands in the row's entry, so nothing else has to be
+// looked up first.
 template <typename TQ, typename T16>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const PagedArgs a, const PartArgs prefix, const PartArgs rest) {
+__global__ void __launch_bounds__(128) paged_join_rows_kernel(const PagedArgs a, const PartArgs prefix, const PartArgs rest) {
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     pdl_wait();
     if (row >= (int64_t)a.T * a.H) return;
     float4 st[2];
     st[1] = rest.stat[row];
-    st[0] = rest.by_row ? prefix.stat[row] : st[1];
+    st[0] = prefix.stat[row];
     if (a.qstarts) {  // rows of no sequence are not written
         const int t = (int)(row / a.H);
         if (t < __ldg(a.qstarts) || t >= __ldg(a.qstarts + a.B)) return;
     }
     const PartPlace place = place_of(st[1]);
-    const bool both = rest.by_row && place.prefix;
+    const bool both = place.prefix;
     if (!both && place.c0 == place.c1) return;  // written by the CTA that had all of it
     // the parts in one line, a lane each
     const PartPlace pre = place_of(st[0]);
@@ -577,6 +587,101 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedArgs a, c
     }
 }
 
+// The same without prefixes: only the row blocks that were cut have to be
+// joined (grid: CTA, rows of its block); the blocks for other CTAs leave at
+// once. A row has two or three parts mostly, so a warp has four rows, eight
+// lanes for the parts of each, and sixteen loads in flight.
+template <typename TQ, typename T16>
+__global__ void __launch_bounds__(128) paged_join_cuts_kernel(const PagedArgs a, const PartArgs p) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_wait();
+    const int c0 = blockIdx.x;
+    const int4 rec = *reinterpret_cast<const int4*>(p.cuts + c0 * 8);
+    if (rec.x < 0) return;
+    const int kvh = p.cuts[c0 * 8 + 4];
+    const int r = (blockIdx.y * 4 + warp) * 4 + lane / 8, br = rec.z + r;
+    const bool on = r < p.slot_rows && br < rec.w;
+    const int64_t row = (int64_t)(rec.y + br / a.G) * a.H + kvh * a.G + br % a.G;
+    const int n = rec.x - c0 + 1;
+    const bool live = lane * 4 < a.D;
+    float M = -INFINITY, L = 0.0f;
+    float4 o[4] = {};
+    for (int base = 0; base < n; base += 8) {
+        const int c = c0 + base + (lane & 7);
+        const int64_t slot = (int64_t)c * p.slot_rows + r;
+        float m = -INFINITY, l = 0.0f;
+        if (on && c <= rec.x) {
+            if (c == c0) {
+                const float4 st = p.stat[row];
+                m = st.x;
+                l = st.y;
+            } else {
+                const float2 v = p.tail_stat[slot];
+                m = v.x;
+                l = v.y;
+            }
+        }
+        float mx = m;
+#pragma unroll
+        for (int k = 1; k < 8; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+        mx = fmaxf(mx, M);
+        const float keep = M == -INFINITY ? 0.0f : exp2_fast(M - mx);
+        const float w = m == -INFINITY ? 0.0f : exp2_fast(m - mx);
+        float lw = l * w;
+#pragma unroll
+        for (int k = 1; k < 8; k <<= 1) lw += __shfl_xor_sync(0xffffffffu, lw, k);
+        M = mx;
+        L = L * keep + lw;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float kq = __shfl_sync(0xffffffffu, keep, q * 8);
+            o[q].x *= kq;
+            o[q].y *= kq;
+            o[q].z *= kq;
+            o[q].w *= kq;
+        }
+        for (int i = 0; i < min(8, n - base); i += 4) {
+            float4 v[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int cc = c0 + base + i + k;
+                const float* src = (cc == c0 ? p.head : p.tail) + ((int64_t)cc * p.slot_rows + (blockIdx.y * 4 + warp) * 4) * a.D + lane * 4;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    v[k][q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (cc <= rec.x && live && (blockIdx.y * 4 + warp) * 4 + q < p.slot_rows && br - lane / 8 + q < rec.w)
+                        v[k][q] = *reinterpret_cast<const float4*>(src + q * a.D);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float wq = __shfl_sync(0xffffffffu, w, q * 8 + i + k);
+                    o[q].x = fmaf(v[k][q].x, wq, o[q].x);
+                    o[q].y = fmaf(v[k][q].y, wq, o[q].y);
+                    o[q].z = fmaf(v[k][q].z, wq, o[q].z);
+                    o[q].w = fmaf(v[k][q].w, wq, o[q].w);
+                }
+        }
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const float iq = __shfl_sync(0xffffffffu, inv, q * 8);
+        const bool go = __shfl_sync(0xffffffffu, (int)on, q * 8) && live;
+        const int64_t to = __shfl_sync(0xffffffffu, row, q * 8);
+        if (!go) continue;
+        TQ* dst = static_cast<TQ*>(a.out) + to * a.D + lane * 4;
+        if constexpr (sizeof(TQ) == 4) {
+            *reinterpret_cast<float4*>(dst) = make_float4(o[q].x * iq, o[q].y * iq, o[q].z * iq, o[q].w * iq);
+        } else {
+            *reinterpret_cast<uint2*>(dst) =
+                make_uint2(Half2Of<T16>::pack(o[q].x * iq, o[q].y * iq), Half2Of<T16>::pack(o[q].z * iq, o[q].w * iq));
+        }
+    }
+}
+
 template <typename TQ, typename TK, int DP, int NT, bool SPLIT>
 void launch_decode_t(const BeaconCudaContext* ctx, const PagedArgs& a, const CacheMaps& maps, const PartArgs& rest, cudaStream_t s, bool pdl, bool after_tc) {
     auto kern = paged_decode_kernel<TQ, TK, DP, NT, SPLIT>;
@@ -613,10 +718,15 @@ void launch_paged_decode(const BeaconCudaContext* ctx, const PagedArgs& a, const
 }
 
 void launch_paged_combine(const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, int32_t tq, cudaStream_t s) {
-    const dim3 grid((unsigned)(((int64_t)a.T * a.H + 3) / 4));
-    if (tq == BEACON_CUDA_DTYPE_F32) launch_kernel(paged_combine_kernel<float, __half>, grid, dim3(128), 0, s, true, a, prefix, rest);
-    else if (tq == BEACON_CUDA_DTYPE_F16) launch_kernel(paged_combine_kernel<__half, __half>, grid, dim3(128), 0, s, true, a, prefix, rest);
-    else launch_kernel(paged_combine_kernel<__nv_bfloat16, __nv_bfloat16>, grid, dim3(128), 0, s, true, a, prefix, rest);
+    auto go = [&](auto rows, auto cuts) {
+        if (rest.by_row)
+            launch_kernel(rows, dim3((unsigned)(((int64_t)a.T * a.H + 3) / 4)), dim3(128), 0, s, true, a, prefix, rest);
+        else
+            launch_kernel(cuts, dim3((unsigned)rest.ctas, (unsigned)((rest.slot_rows + 15) / 16)), dim3(128), 0, s, true, a, rest);
+    };
+    if (tq == BEACON_CUDA_DTYPE_F32) go(paged_join_rows_kernel<float, __half>, paged_join_cuts_kernel<float, __half>);
+    else if (tq == BEACON_CUDA_DTYPE_F16) go(paged_join_rows_kernel<__half, __half>, paged_join_cuts_kernel<__half, __half>);
+    else go(paged_join_rows_kernel<__nv_bfloat16, __nv_bfloat16>, paged_join_cuts_kernel<__nv_bfloat16, __nv_bfloat16>);
 }
 
 }  // namespace bc

@@ -22,7 +22,7 @@
 // rows into a ring of tiles in the 128-byte swizzle, requested by four warps;
 // rows of a value tile that are no keys of the block are zeroed there (their
 // weights are zero, but what a page holds behind its last row may be no
-// number). 16-byte asynchronous copies by four warps, which zero-fill, serve
+// number). 16-byte asynchronous copies by the same warps, which zero-fill, serve
 // page sizes that are no multiple of 8 (they reach 8 bytes a cycle and
 // multiprocessor: the tensor copies are what feeds the matrix unit). One
 // thread issues the products. The key tiles of all blocks form one line that the CTAs
@@ -114,20 +114,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
           "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
-// The wait for the loads above passes their registers on, so that no use of
-// them is moved before it.
-__device__ __forceinline__ void tmem_wait_ld(float (&v)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
-                   "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]),
-                   "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
-                   "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])::"memory");
-}
-__device__ __forceinline__ void tmem_wait_ld(float (&v)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
-                   "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
-}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
@@ -346,6 +333,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     __syncthreads();
 
+    // no row block of this CTA is cut at its end, until one is
+    if (tid == 0) {
+        rest.cuts[cta * 8] = -1;
+        if (prefix.cuts) prefix.cuts[cta * 8] = -1;
+    }
     Piece pc;
     if (u0 < u1) {
         pc.e = entry_s;
@@ -389,21 +381,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             value = j >= 0 && (j >= pairs || (j & 1) == 0);
             return j < 0 ? f : j >= pairs ? p.n - la + (j - pairs) : value ? j / 2 : j / 2 + la;
         };
-        // this lane's first key of a tile (copies row by row: 32 rows a warp; tensor
-        // copies: a box a lane), its page, and the cache row: -1 if there is none
-        auto pos_of = [&](const Piece& p, int t) {
-            return p.k.base + (p.tile + t) * kTile + (a.box ? lane * a.box : pw * 32 + lane);
-        };
+        // Tensor copies, a box a lane: the lane's first key of a tile, its page, and
+        // the cache row: -1 if there is none
+        auto pos_of = [&](const Piece& p, int t) { return p.k.base + (p.tile + t) * kTile + lane * a.box; };
         auto page_of = [&](const Piece& p, int t) {
             const int pos = pos_of(p, t);
-            if (t >= p.n || pos >= p.k.key1 || (a.box && lane * a.box >= kTile)) return 0;
+            if (!a.box || t >= p.n || pos >= p.k.key1 || lane * a.box >= kTile) return 0;
             return page_id(a, pos < p.k.cut ? p.k.first : p.k.b, pos);
         };
         auto row_of = [&](const Piece& p, int t, int page) {
             const int pos = pos_of(p, t);
-            if (pos >= p.k.key1 || (a.box && lane * a.box >= kTile)) return -1;
+            if (!a.box || pos >= p.k.key1 || lane * a.box >= kTile) return -1;
             const int row = (int)page_row(a, page, pos);
-            return row < 0 && a.box ? (int)(a.pages * a.page_size) : row;  // a bad page: a box outside, zeros
+            return row < 0 ? (int)(a.pages * a.page_size) : row;  // a bad page: a box outside, zeros
         };
         auto room = [&]() {  // waits for the stage of tile `it`
             const uint32_t par = (uint32_t)((it / NST - 1) & 1);
@@ -420,8 +410,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             ok = __all_sync(0xffffffffu, ok);  // the lanes copy for each other: they go on or give up together
             return ok;
         };
-        // 32 rows of a tile one by one, 16 bytes a lane; each lane knows one cache row
-        auto copy_rows = [&](uint32_t dst, const Piece& p, const void* cache, int r0, int row) {
+        // Rows r0 .. r0 + 31 of a tile one by one, 16 bytes a lane (each lane looks one row up)
+        auto copy_rows = [&](uint32_t dst, const Piece& p, const void* cache, int pos0, int r0) {
+            const int q = pos0 + r0 + lane;
+            const int row = q < p.k.key1 ? (int)page_row(a, page_id(a, q < p.k.cut ? p.k.first : p.k.b, q), q) : -1;
             dst += (c >> 3) * (kTile * 128);
             const uint8_t* src = static_cast<const uint8_t*>(cache) + (p.kvh * a.D + c * 8) * 2;
 #pragma unroll 8
@@ -435,8 +427,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         };
         auto load_tile = [&](const Piece& p, int t, bool value, int row) {
             if (!room()) return;
+            const int pos0 = p.k.base + (p.tile + t) * kTile;
+            const uint32_t dst = smem_u32(ring + (size_t)(it % NST) * SM::tile);
             if (!a.box) {
-                copy_rows(smem_u32(ring + (size_t)(it % NST) * SM::tile), p, value ? a.cv : a.ck, pw * 32, row);
+                for (int r0 = pw * 32; r0 < kTile; r0 += kLoadWarps * 32) copy_rows(dst, p, value ? a.cv : a.ck, pos0, r0);
                 cp_async_commit();
                 ++it;
                 if (it - told > 2) {  // two tiles stay in flight
@@ -446,17 +440,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 return;
             }
             const int st = it++ % NST;
-            const int pos0 = p.k.base + (p.tile + t) * kTile;
-            const uint32_t dst = smem_u32(ring + (size_t)st * SM::tile);
             const bool live = row >= 0;
             if (pos0 < p.k.cut && pos0 + kTile > p.k.cut && (p.k.cut & (a.box - 1))) {
                 // a box whose rows lie in two tables: this tile row by row
                 if (pw > 0) return;
-                for (int r0 = 0; r0 < kTile; r0 += 32) {
-                    const int q = pos0 + r0 + lane;
-                    copy_rows(dst, p, value ? a.cv : a.ck, r0,
-                              q < p.k.key1 ? (int)page_row(a, page_id(a, q < p.k.cut ? p.k.first : p.k.b, q), q) : -1);
-                }
+                for (int r0 = 0; r0 < kTile; r0 += 32) copy_rows(dst, p, value ? a.cv : a.ck, pos0, r0);
                 cp_async_commit();
                 cp_async_wait<0>();
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -470,7 +458,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             uint64_t* bar = part ? &fix_bar : &full_bar[st];
             const int boxes = __popc(__ballot_sync(0xffffffffu, live));
             // one arrival and all bytes from the first warp; the copies, whose
-            // requests take a hundred cycles each, from all four
+            // requests take a hundred cycles each, from all warps
             if (pw == 0 && lane == 0) mbar_expect_tx(bar, (uint32_t)(boxes * a.box * DP * 2));
             if (live && (part || lane % kLoadWarps == pw)) {
 #pragma unroll
@@ -531,20 +519,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
+            if constexpr (!SPLIT) {
 #pragma unroll 1
-            for (int i = 0; i < (TWO ? 2 : 1); ++i) {
-                // this lane's query row, as a row of [T * H][D]; -1: behind the block
-                const int br = p.rt * BR + i * kTile + pw * 32 + lane;
-                const int qrow = br < p.k.rows ? (p.k.tok0 + br / a.G) * a.H + p.kvh * a.G + br % a.G : -1;
-                const uint32_t dst = smem_u32(q_smem) + (TWO ? i * SM::tile : 0);
-                if constexpr (!SPLIT) {
+                for (int r0 = pw * 32; r0 < BR; r0 += kLoadWarps * 32) {
+                    // this lane's query row, as a row of [T * H][D]; -1: behind the block
+                    const int br = p.rt * BR + r0 + lane;
+                    const int qrow = br < p.k.rows ? (p.k.tok0 + br / a.G) * a.H + p.kvh * a.G + br % a.G : -1;
+                    const uint32_t dst = smem_u32(q_smem) + (r0 / kTile) * SM::tile + (c >> 3) * (kTile * 128);
 #pragma unroll 8
                     for (int k = 0; k < 32 / RPI; ++k) {
                         const int rr = k * RPI + lane / CH;
                         const int qr = __shfl_sync(0xffffffffu, qrow, rr);
                         const bool live = qr >= 0 && chunk_live;
-                        const int r = pw * 32 + rr;
-                        cp_async16_zfill(dst + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                        const int r = r0 % kTile + rr;
+                        cp_async16_zfill(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4),
                                          static_cast<const TQ*>(a.q) + (live ? (int64_t)qr * a.D + c * 8 : 0), live);
                     }
                 }
@@ -747,7 +735,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         float w[16];
                         uint32_t x[16];
                         tmem_ld16(s_col + c, w);
-                        tmem_wait_ld(w);
+                        tmem_wait_ld();
 #pragma unroll
                         for (int i = 0; i < 16; ++i) x[i] = c + i >= seen || c + i < skip ? 0xFF800000u : __float_as_uint(w[i]);
                         tmem_st16(s_col + c, x);
@@ -766,19 +754,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         for (int k = 0; k < 4; ++k) x[k] = max3(x[k], v[i + k], v[i + 4 + k]);
                     return max3(max3(x[0], v[27], v[28]), max3(x[1], v[29], v[30]), max3(x[2], x[3], v[31]));
                 };
+                float top = -INFINITY;
                 tmem_ld32(s_col, va);
-                tmem_wait_ld(va);
-                tmem_ld32(s_col + 32, vb);
-                float top = top_of(va, -INFINITY);
-                tmem_wait_ld(vb);
-                tmem_ld32(s_col + 64, va);
-                top = top_of(vb, top);
-                tmem_wait_ld(va);
-                tmem_ld32(s_col + 96, vb);
-                top = top_of(va, top);
-                tmem_wait_ld(vb);
-                tmem_ld32(s_col, va);
-                top = top_of(vb, top);
+#pragma unroll 1
+                for (int c = 0; c < kTile; c += 64) {
+                    tmem_wait_ld();
+                    tmem_ld32(s_col + c + 32, vb);
+                    top = top_of(va, top);
+                    tmem_wait_ld();
+                    tmem_ld32(s_col + ((c + 64) & (kTile - 1)), va);  // last: the first ones again
+                    top = top_of(vb, top);
+                }
                 const float mx = fmaxf(m, top * cs);
                 const bool move = m != -INFINITY && mx > m + kRescale;
                 if (t >= (TWO ? 1 : 2) && __any_sync(0xffffffffu, move)) {
@@ -790,7 +776,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         uint32_t x[16];
                         const uint32_t o_at = tmem + lane_at + 2 * kTile + s * DP + c;
                         tmem_ld16(o_at, w);
-                        tmem_wait_ld(w);
+                        tmem_wait_ld();
 #pragma unroll
                         for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(w[i] * keep);
                         tmem_st16(o_at, x);
@@ -814,17 +800,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     tmem_st16(s_col + c, w);
                     if constexpr (SPLIT) tmem_st16(s_col + c + 16, w2);
                 };
-                tmem_wait_ld(va);
-                tmem_ld32(s_col + 32, vb);
-                weights(va, 0);
-                tmem_wait_ld(vb);
-                tmem_ld32(s_col + 64, va);
-                weights(vb, 32);
-                tmem_wait_ld(va);
-                tmem_ld32(s_col + 96, vb);
-                weights(va, 64);
-                tmem_wait_ld(vb);
-                weights(vb, 96);
+#pragma unroll 1
+                for (int c = 0; c < kTile; c += 64) {
+                    tmem_wait_ld();
+                    tmem_ld32(s_col + c + 32, vb);
+                    weights(va, c);
+                    tmem_wait_ld();
+                    if (c == 0) tmem_ld32(s_col + 64, va);
+                    weights(vb, c + 32);
+                }
                 sum[0] = add2(sum[0], sum[1]);
                 l = sum[0].x + sum[0].y;
                 tmem_wait_st();
@@ -859,6 +843,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // shared memory the warp writes 8 rows by 64 bytes per instruction
             // (a thread writing its own row touches 32 lines at once: 14,000
             // cycles for 256 rows of 128 sums).
+            if (c0 == cta && c1 > c0 && tid == 0) {  // the row block whose parts have to be joined
+                int* rec = part.cuts + cta * 8;
+                rec[0] = c1;
+                rec[1] = p.k.tok0;
+                rec[2] = p.rt * BR;
+                rec[3] = p.k.rows;
+                rec[4] = p.kvh;
+            }
             const int64_t own = !live ? -1 : (done || (c0 == cta && part.by_row) ? orow : slot) * a.D;
             int64_t to[4];
 #pragma unroll
@@ -871,14 +863,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             auto sums_of = [&](int col, float (&v)[16]) {
                 const uint32_t o_at = tmem + lane_at + 2 * kTile + col;
                 tmem_ld16(o_at + (TWO ? s * DP : 0), v);
-                tmem_wait_ld(v);
+                tmem_wait_ld();
                 if (!TWO) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) v[i] *= w0;
                     if (both) {
                         float y[16];
                         tmem_ld16(o_at + DP, y);
-                        tmem_wait_ld(y);
+                        tmem_wait_ld();
 #pragma unroll
                         for (int i = 0; i < 16; ++i) v[i] = fmaf(y[i], w1, v[i]);
                     }
