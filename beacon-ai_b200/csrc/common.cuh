@@ -161,7 +161,13 @@ enum DeviceErr : int {
     kErrAttnWait = 3,      // decode attention: a bounded wait gave up
     kErrGemmWait = 4,      // tensor-core GEMM: a bounded pipeline wait gave up
     kErrGemvWait = 5,      // persistent GEMV: a bounded wait gave up
-    kErrIndex = 6,         // an index held in a device tensor is out of range (stream error word)
+};
+
+// A stream's error words, host memory that its kernels write (0 = none).
+enum StreamErr : int {
+    kErrWordIndex = 0,  // an index held in a device tensor is out of range
+    kErrWordWait = 1,   // a bounded wait gave up
+    kErrWords = 2,
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

@@ -152,7 +152,7 @@ struct BeaconCudaContext {
     bool comm_aborted = false;  // a failed or timed-out collective aborted the communicator
     int nranks = 1, rank = 0;
     int comm_timeout_ms = 60000;
-    // host-mapped error words handed to streams (stream_error_word); slots are
+    // host-mapped error words handed to streams (stream_error_word); they are
     // never reused, so a graph that outlives its stream reports to nobody else
     std::vector<int*> err_slabs;
     int err_used = 0;  // words taken from the last slab
@@ -197,10 +197,10 @@ inline cudaStream_t stream_of(BeaconCudaStream* s) { return s ? s->s : nullptr; 
 // device wait of an op on this stream gave up, clear the flag, re-zero the
 // stream's arrival counters (a warp that gave up never arrived) and throw
 // BEACON_CUDA_ERR_DEVICE_TIMEOUT.
-// An index error that a kernel recorded in the stream's error word is thrown
-// as SHAPE_MISMATCH and cleared.
+// What kernels recorded in the stream's error words is cleared and thrown: a
+// wait that gave up as DEVICE_TIMEOUT, an index out of range as SHAPE_MISMATCH.
 void check_stream_timeout(BeaconCudaStream* stream);
-// The stream's error word, made at its first use (also during capture).
+// The stream's error words (StreamErr), made at their first use (also during capture).
 int* stream_error_word(BeaconCudaStream* stream);
 // The same for every stream of the context (after a device synchronisation).
 void check_context_timeouts(BeaconCudaContext* ctx);

@@ -191,7 +191,7 @@ __device__ __forceinline__ SeqInfo seq_info(const PagedArgs& a, int b) {
         bad = true;
         s.nq = 0;
     }
-    if (bad) *a.err = kErrIndex;
+    if (bad) a.err[kErrWordIndex] = 1;
     return s;
 }
 
@@ -205,7 +205,7 @@ __device__ __forceinline__ int page_id(const PagedArgs& a, int b, int p) {
 }
 __device__ __forceinline__ int64_t page_row(const PagedArgs& a, int page, int p) {
     if (page >= 0 && page < a.pages) return (int64_t)page * a.page_size + (p - page_index(a, p) * a.page_size);
-    *a.err = kErrIndex;
+    a.err[kErrWordIndex] = 1;
     return -1;
 }
 

@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kDecThreads)
             }
             // the stage that was read last is filled again
             __syncwarp();
-            if (j + NS - 1 < count) {
+            if (j + NS - 1 < count && !failed) {
                 copy_tile((j + NS - 1) % NS, load, page_next);
                 load.step(a);
                 if (j + NS < count) page_next = fetch_page(load);
@@ -306,9 +306,11 @@ __global__ void __launch_bounds__(kDecThreads)
             const int first = at.cur.base + at.tile * kDecKeys + warp * 16;
             if (a.box) {
                 if (!failed && !wait_bar(&bars[warp][j % NS], (uint32_t)((j / NS) & 1), limit)) {
-                    *a.err = kErrAttnWait;
-                    failed = true;
+                    // reported; the ring stays in step as long as the copy comes at all
+                    a.err[kErrWordWait] = 1;
+                    failed = !mbar_drain(&bars[warp][j % NS], (uint32_t)((j / NS) & 1));
                 }
+                failed = __any_sync(0xffffffffu, failed);
                 if (first < at.cur.from || first + 16 > at.cur.to) {
                     // value rows that are no keys: their weights are zero, but what the
                     // page holds there may be no number
@@ -483,13 +485,9 @@ __global__ void __launch_bounds__(kDecThreads)
             }
             at.step(a);
         }
-        if (a.box) {
-            // a wait that gave up: nothing may land after the CTA has ended
-            if (failed)
-                for (int i = max(0, count - NS); i < count; ++i) mbar_drain(&bars[warp][i % NS], (uint32_t)((i / NS) & 1));
-        } else {
-            cp_async_wait<0>();
-        }
+        // Nothing lands after the CTA has ended: every copy was waited for above, and
+        // when one did not come no more were requested.
+        if (!a.box) cp_async_wait<0>();
     }
     // kernels launched after this one count on everything before it
     pdl_wait();
@@ -520,7 +518,7 @@ __global__ void __launch_bounds__(128) paged_join_rows_kernel(const PagedArgs a,
     const bool bad = place.c1 < place.c0 || place.c1 >= rest.ctas || place.row >= rest.slot_rows ||
                      (both && (pre.c1 < pre.c0 || pre.c1 >= prefix.ctas || pre.row >= prefix.slot_rows));
     if (bad) {  // start arrays that contradict each other: no CTA had the row
-        *a.err = kErrIndex;
+        a.err[kErrWordIndex] = 1;
         return;
     }
     const int n0 = both ? pre.c1 - pre.c0 + 1 : 0, n = n0 + place.c1 - place.c0 + 1;

@@ -177,7 +177,7 @@ __device__ __forceinline__ Block block_of(const PagedArgs& a, int e) {
             k.tok0 = keep_in(t0, a.T, bad);
             k.rows = max(0, keep_in(t1, a.T, bad) - k.tok0) * a.G;
         }
-        if (bad || hi < lo) *a.err = kErrIndex;
+        if (bad || hi < lo) a.err[kErrWordIndex] = 1;
         return k;
     }
     const SeqInfo s = seq_info(a, e - groups);
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     const long long limit_cycles = g_wait_limit;
     auto give_up = [&]() {
-        *a.err = kErrAttnWait;
+        a.err[kErrWordWait] = 1;
         failed_s = 1;
     };
 
@@ -548,8 +548,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // nothing may land after the CTA has ended
         cp_async_wait<0>();
         if (!a.box && ok) announce(it);
-        if (a.box && pw == 0)
-            for (int i = max(0, it - NST); i < it; ++i) mbar_drain(&full_bar[i % NST], (uint32_t)((i / NST) & 1));
+        // (after a wait that gave up some warp's part may not have been requested:
+        // one limit for all stages, far beyond any copy's time)
+        if (a.box && pw == 0) {
+            const long long t0 = clock64();
+            for (int i = max(0, it - NST); i < it; ++i)
+                while (!mbar_try_wait(&full_bar[i % NST], (uint32_t)((i / NST) & 1)) && clock64() - t0 <= kBoundedWaitLimit) {
+                }
+        }
     } else if (warp >= kMmaWarp) {
         if (warp == kMmaWarp) {
             // the whole warp waits; its elected thread issues

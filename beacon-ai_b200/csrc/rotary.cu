@@ -155,7 +155,7 @@ __device__ __forceinline__ int64_t cache_row(const RowArgs& a, int64_t t) {
         const int64_t page = a.table[b * a.max_pages + p / a.page_size];
         if (page >= 0 && page < a.pages) return page * a.page_size + p % a.page_size;
     }
-    *a.err = kErrIndex;
+    a.err[kErrWordIndex] = 1;
     return -1;
 }
 

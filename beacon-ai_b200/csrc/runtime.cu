@@ -145,7 +145,7 @@ static std::vector<cudaError_t (*)(long long)>& wait_limit_setters() {
 void register_wait_limit_setter(cudaError_t (*setter)(long long)) { wait_limit_setters().push_back(setter); }
 
 int* stream_error_word(BeaconCudaStream* stream) {
-    constexpr int kSlabWords = 1024;
+    constexpr int kSlabWords = 512 * kErrWords;
     if (stream->err_word) return stream->err_word;
     BeaconCudaContext* ctx = stream->ctx;
     std::lock_guard<std::mutex> lk(ctx->streams_mu);
@@ -168,15 +168,19 @@ int* stream_error_word(BeaconCudaStream* stream) {
         }
         ctx->err_used = 0;
     }
-    stream->err_word = ctx->err_slabs.back() + ctx->err_used++;
+    stream->err_word = ctx->err_slabs.back() + ctx->err_used;
+    ctx->err_used += kErrWords;
     return stream->err_word;
 }
 
 void check_stream_timeout(BeaconCudaStream* stream) {
     if (stream && stream->ctx && stream->err_word) {
         volatile int* w = stream->err_word;  // the stream's work is done: no kernel is writing it
-        if (*w) {
-            *w = 0;
+        const bool gave_up = w[kErrWordWait] != 0, index = w[kErrWordIndex] != 0;
+        w[kErrWordWait] = w[kErrWordIndex] = 0;
+        if (gave_up)
+            fail(BEACON_CUDA_ERR_DEVICE_TIMEOUT, "paged attention: a bounded device-side wait gave up; the op's output is invalid");
+        if (index) {
             shape_err("a sequence number, position, length or page id held in a device tensor is out of range; "
                       "the rows it names were left out");
         }

@@ -648,3 +648,34 @@ def test_two_streams_at_once(be, torch_):
         want, info = ref.attention(qs[k].f64(), ck.f64(), cv.f64(), table, lens, float(np.float32(0.1)))
         for o in outs[k]:
             close(o.numpy().astype(np.float64), want, ref.attention_bound(want, info, "f32", "f16", D))
+
+
+@pytest.mark.parametrize("new,ps", [(1, 16), (40, 16), (40, 7)])
+def test_attention_wait_timeout_is_reported(be, new, ps):
+    """A bounded wait that runs out is reported as such, and the stream works on."""
+    from beacon_cuda import EngineError
+    from beacon_cuda import _lib as L
+    rng = np.random.default_rng(33)
+    H, Hkv, D, lens = 32, 8, 128, [6000, 4100, 5000, 300]
+    B = len(lens)
+    ck, cv, table = make_cache(be, rng, -(-max(lens) // ps), lens, ps, Hkv, D, "f16")
+    starts = None if new == 1 else [new * i for i in range(B + 1)]
+    q = Dev(be, rng.standard_normal((B * new, H, D)), "f16")
+    tb, ln, st = i32(be, table), i32(be, lens), starts and i32(be, starts)
+    s = be.new_stream()
+    statuses = []
+    be.set_wait_limit(1)
+    try:
+        for _ in range(20):
+            be.paged_attention(s, q.t, ck.t, cv.t, tb.t, ln.t, 0.1, query_starts=st and st.t)
+            try:
+                s.synchronize()
+                statuses.append(L.OK)
+            except EngineError as e:
+                statuses.append(e.status)
+                break
+    finally:
+        be.set_wait_limit(0)
+    assert L.ERR_DEVICE_TIMEOUT in statuses, statuses
+    for _ in range(2):
+        check_attention(be, s, rng, q, ck, cv, table, lens, "f16", "f16", starts)
