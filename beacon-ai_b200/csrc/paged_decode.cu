@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kDecThreads)
     const Shares shares(total, part.ctas);
     const long long u0 = cta < shares.ctas ? shares.begin(cta) : 0, u1 = cta < shares.ctas ? shares.begin(cta + 1) : 0;
     pdl_trigger();
-    if (tid == 0) part.cuts[cta * 8] = -1;  // no row block of this CTA is cut at its end, until one is
+    if (tid == 0 && !part.by_row) part.cuts[cta * 8] = -1;  // no row block of this CTA is cut at its end, until one is
     if (u0 < u1) {
         if (before * a.Hkv <= u0 && u0 < (before + mine) * a.Hkv) {
             int b = cb0;
@@ -394,8 +394,8 @@ __global__ void __launch_bounds__(kDecThreads)
                     for (int n = 0; n < NT; ++n) {
                         if constexpr (SPLIT) {
                             float t[4] = {};
+                            mma16816<TK>(t, va, pl[n][0], pl[n][1]);  // small parts first: sums are cut to 24 bits
                             mma16816<TK>(t, va, ph[n][0], ph[n][1]);
-                            mma16816<TK>(t, va, pl[n][0], pl[n][1]);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) o[d][n][e] += t[e];
                         } else {
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kDecThreads)
                 const long long tile0 = u0 + j - at.tile;  // of this head, in the line
                 const int c0 = shares.of(tile0), c1 = shares.of(tile0 + at.cur.tiles - 1);
                 const bool done = c0 == c1 && at.cur.from == 0;  // no other part anywhere
-                if (tid == 0 && c0 == cta && c1 > c0) {  // the row block whose parts have to be joined
+                if (tid == 0 && c0 == cta && c1 > c0 && !part.by_row) {  // the row block whose parts have to be joined
                     int* rec = part.cuts + cta * 8;
                     rec[0] = c1;
                     rec[1] = at.b;

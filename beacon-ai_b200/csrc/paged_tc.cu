@@ -212,8 +212,18 @@ __device__ __forceinline__ int tiles_of_block(const PagedArgs& a, const Block& k
     return sum;
 }
 
-// A CTA's next piece of the line: key tiles [tile, tile + n) of row tile rt.
-struct Piece {
+// Key tiles of a piece with 32-bit queries. The matrix unit cuts its sums to 24
+// bits after every product, so a chain of n tiles shrinks them by about 1.7e-7 n
+// of themselves; pieces are joined with rounding. 4 prompts of 1024 rows over
+// 4096 keys, 32 heads on 8, D 128, off 64 bits and time: whole chains (16 tiles a
+// stream) 3.4e-6, 383 us; 10 tiles (5 a stream) 1.7e-6, 463 us; 8 tiles 1.4e-6,
+// 498 us; a plain form in 32 bits has 1.3e-6.
+constexpr int kMostSplit = 10;
+
+// A CTA's next piece of the line: key tiles [tile, tile + n) of row tile rt,
+// at most MOST of them.
+template <int MOST>
+struct PieceOf {
     Block k;
     int e = 0, entries = 0, kvh = 0, rt = 0, tile = 0;
     int tiles = 0;     // of the row tile
@@ -222,6 +232,11 @@ struct Piece {
     __device__ __forceinline__ void next(const PagedArgs& a, int block_rows, long long u1) {
         u += n;
         if (u >= u1) return;
+        if (tile + n < tiles) {
+            tile += n;
+            n = (int)min((long long)min(tiles - tile, MOST), u1 - u);
+            return;
+        }
         tile = 0;
         for (;;) {
             ++rt;
@@ -242,14 +257,14 @@ struct Piece {
             tiles = tiles_of(a, k, rt, block_rows);
             if (tiles) break;
         }
-        n = (int)min((long long)tiles, u1 - u);
+        n = (int)min((long long)min(tiles, MOST), u1 - u);
     }
 };
 
 template <typename TQ, typename T16, int DP, bool SPLIT, bool TWO>
 __global__ void __launch_bounds__(kTcThreads, 1)
     paged_tc_kernel(const PagedArgs a, const __grid_constant__ CacheMaps maps, const PartArgs prefix, const PartArgs rest, int entries,
-                    int line_ctas) {
+                    int line_ctas, int least_tiles) {
     using SM = TcSmem<DP, SPLIT, TWO>;
     constexpr int NST = SM::stages;
     constexpr int LA = TWO ? 1 : 2;              // key tiles ahead of the value tile
@@ -262,6 +277,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __shared__ volatile int failed_s;
     __shared__ float qscale_s[2][kTile];   // SPLIT: what the scores are multiplied by
     __shared__ float2 join_s[2][kTile];    // !TWO: (m, l) of both streams
+    __shared__ float2 so_far_s[2][kTile];  // SPLIT: (m, l) of the pieces of the row tile so far, each thread its own
     __shared__ long long sums_s[kTcThreads / 32];
     __shared__ long long before_s;
     __shared__ int entry_s;
@@ -319,7 +335,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     total *= a.Hkv;
     pdl_trigger();
     const int cta = blockIdx.x;
-    const Shares shares(total, line_ctas);
+    // With single rows behind the prefixes the kernel of those starts on the SMs
+    // that are free: few tiles go to half of them, four each (32 rows of a 4096-key
+    // prefix: 55.4 -> 53.2 us with both kernels at once).
+    const Shares shares(total, (int)min((long long)line_ctas, max((long long)line_ctas / 2, total / least_tiles)));
     const long long u0 = cta < shares.ctas ? shares.begin(cta) : 0, u1 = cta < shares.ctas ? shares.begin(cta + 1) : 0;
     if (u0 < u1 && before * a.Hkv <= u0 && u0 < (before + mine) * a.Hkv) {
         int e = e0;
@@ -334,10 +353,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __syncthreads();
 
     // no row block of this CTA is cut at its end, until one is
-    if (tid == 0) {
-        rest.cuts[cta * 8] = -1;
-        if (prefix.cuts) prefix.cuts[cta * 8] = -1;
-    }
+    if (tid == 0 && !rest.by_row) rest.cuts[cta * 8] = -1;
+    using Piece = PieceOf<SPLIT ? kMostSplit : 0x7FFFFFFF>;
     Piece pc;
     if (u0 < u1) {
         pc.e = entry_s;
@@ -353,7 +370,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         pc.tile = at;
         pc.u = u0;
-        pc.n = (int)min((long long)(pc.tiles - at), u1 - u0);
+        pc.n = (int)min((long long)min(pc.tiles - at, SPLIT ? kMostSplit : 0x7FFFFFFF), u1 - u0);
     }
     const long long limit_cycles = g_wait_limit;
     auto give_up = [&]() {
@@ -574,18 +591,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 wait(&full_bar[it % NST], (uint32_t)((it / NST) & 1));
                 return it++ % NST;
             };
+            constexpr int kParts = SPLIT ? 2 : 1;
             constexpr uint32_t id_qk = idesc<T16>(kTile, false), id_pv = idesc<T16>(DP, true);
             // S_s = Q K^T; then announces it and, if it was the tile's last use, frees the tile
             auto scores = [&](int s, int st, bool last) {
                 if (elect_one()) {
                     const uint32_t d = tmem + s * kTile, b = desc_lo_k(ra + st * SM::tile);
+                    // the small parts first: sums in the matrix unit are cut to 24 bits
+                    // after every product, which costs nothing while they are small
 #pragma unroll
-                    for (int part = 0; part < (SPLIT ? 2 : 1); ++part) {
-                        const uint32_t q = desc_lo_k(qa + (TWO ? s : part) * SM::tile);
+                    for (int i = 0; i < kParts; ++i) {
+                        const uint32_t q = desc_lo_k(qa + (TWO ? s : kParts - 1 - i) * SM::tile);
 #pragma unroll
                         for (int k = 0; k < DP / 16; ++k) {
                             const uint32_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
-                            mma_ss(d, q + off, kDescHi, b + off, kDescHi, id_qk, part + k > 0);
+                            mma_ss(d, q + off, kDescHi, b + off, kDescHi, id_qk, i + k > 0);
                         }
                     }
                     commit(&s_bar[s]);
@@ -600,10 +620,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (elect_one()) {
                     const uint32_t o = tmem + 2 * kTile + s * DP, p = tmem + s * kTile, b = desc_lo_n(ra + st * SM::tile);
 #pragma unroll
-                    for (int k = 0; k < kTile / 16; ++k)
+                    for (int i = 0; i < kParts; ++i)
 #pragma unroll
-                        for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
-                            mma_ts(o, p + (k >> 1) * 32 + (k & 1) * 8 + part * 16, b + k * (2048 >> 4), kDescHi, id_pv, k + part > 0 || !first);
+                        for (int k = 0; k < kTile / 16; ++k)
+                            mma_ts(o, p + (k >> 1) * 32 + (k & 1) * 8 + (kParts - 1 - i) * 16, b + k * (2048 >> 4), kDescHi, id_pv, i + k > 0 || !first);
                     if (last) commit(&empty_bar[st]);
                 }
                 __syncwarp();
@@ -654,6 +674,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t s_col = tmem + lane_at + s * kTile;
         int ns = 0, seg = 0, nj = 0;
         bool ok = true;
+        int loads = 0;  // of queries (SPLIT)
         auto wait = [&](uint64_t* bar, uint32_t par) {
             if (ok && (!wait_bar(bar, par, limit_cycles) || failed_s)) {
                 give_up();
@@ -666,7 +687,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int row = p.rt * BR + (TWO ? s * kTile : 0) + r;  // of the block
             const bool live = row < p.k.rows;
             const int tok = p.k.tok0 + row / a.G;
-            if constexpr (SPLIT) {
+            const bool goes_on = SPLIT && seg > 0 && p.tile > 0;  // the row tile of the piece before
+            if (SPLIT && !goes_on) {
+                ++loads;
                 // the block's queries as two f16 parts: 16 rows a warp, a row at a
                 // time (each lane four values), eight on their way
                 if (seg > 0) wait(&qempty_bar, (uint32_t)((seg - 1) & 1));
@@ -689,7 +712,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         const float mx = warp_max(fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w))));
                         float inv;
                         const float sc = query_scale(mx, inv);
-                        if (lane == 0) qscale_s[seg & 1][qr] = a.scale * 1.4426950408889634f * inv;
+                        if (lane == 0) qscale_s[loads & 1][qr] = a.scale * 1.4426950408889634f * inv;
                         if (lane * 4 < DP) {
                             uint2 h, l;
                             split_f16(x[k].x * sc, x[k].y * sc, h.x, l.x);
@@ -720,7 +743,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             wait(&qfull_bar, (uint32_t)(seg & 1));
             if (!ok) break;
             // above zero, so that a masked score (-inf) stays one
-            const float cs = fmaxf(SPLIT ? qscale_s[seg & 1][r] : a.scale * 1.4426950408889634f, 1e-37f);
+            const float cs = fmaxf(SPLIT ? qscale_s[loads & 1][r] : a.scale * 1.4426950408889634f, 1e-37f);
             const bool idle = __all_sync(0xffffffffu, !live);
             float m = -INFINITY, l = 0.0f;
             for (int t = TWO ? 0 : s; t < p.n; t += TWO ? 1 : 2) {
@@ -822,6 +845,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 arrive(&p_bar[s]);
             }
             if (!ok) break;
+            // more of this row tile: its next scores may be formed meanwhile
+            const bool last = !SPLIT || p.tile + p.n == p.tiles || p.u + p.n >= u1;
+            if (!last) arrive(&qfull_bar);
             wait(&ofin_bar, (uint32_t)(seg & 1));
             if (!ok) break;
             // --- results of the piece
@@ -837,10 +863,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 w1 = y.x == -INFINITY ? 0.0f : exp2_fast(y.x - M);
                 L = x.y * w0 + y.y * w1;
             }
+            float kept = 0.0f;  // weight of the sums of the pieces before
+            if (goes_on) {
+                const float2 x = so_far_s[s][r];
+                const float top = fmaxf(M, x.x), now = M == -INFINITY ? 0.0f : exp2_fast(M - top);
+                kept = x.x == -INFINITY ? 0.0f : exp2_fast(x.x - top);
+                w0 *= now;
+                w1 *= now;
+                L = L * now + x.y * kept;
+                M = top;
+            }
+            if (!last) so_far_s[s][r] = make_float2(M, L);
             const PartArgs& part = p.k.kind ? rest : prefix;
             const long long first = p.u - p.tile;
             const int c0 = shares.of(first), c1 = shares.of(first + p.tiles - 1);
-            const bool done = c0 == c1 && p.k.kind && p.k.key0 == 0;  // no other part anywhere
+            const bool whole = c0 == c1 && p.k.kind && p.k.key0 == 0;  // no other part anywhere
+            const bool done = whole && last;
             const int64_t orow = (int64_t)tok * a.H + p.kvh * a.G + row % a.G;
             const int slot_row = (TWO ? s * kTile : 0) + r;
             const int64_t slot = (int64_t)cta * part.slot_rows + slot_row;
@@ -849,7 +887,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // shared memory the warp writes 8 rows by 64 bytes per instruction
             // (a thread writing its own row touches 32 lines at once: 14,000
             // cycles for 256 rows of 128 sums).
-            if (c0 == cta && c1 > c0 && tid == 0) {  // the row block whose parts have to be joined
+            if (c0 == cta && c1 > c0 && tid == 0 && !part.by_row) {  // the row block whose parts have to be joined
                 int* rec = part.cuts + cta * 8;
                 rec[0] = c1;
                 rec[1] = p.k.tok0;
@@ -857,7 +895,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 rec[3] = p.k.rows;
                 rec[4] = p.kvh;
             }
-            const int64_t own = !live ? -1 : (done || (c0 == cta && part.by_row) ? orow : slot) * a.D;
+            const int64_t partial = !live ? -1 : (c0 == cta && part.by_row ? orow : slot) * a.D;
+            const int64_t own = live && done ? orow * a.D : partial;
             int64_t to[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) to[i] = __shfl_sync(0xffffffffu, own, i * 8 + lane / 4);
@@ -887,7 +926,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
             };
             if (!done || sizeof(TQ) == 4) {
-                float* base = done ? static_cast<float*>(a.out) : c0 == cta ? part.head : part.tail;
+                float* parts = c0 == cta ? part.head : part.tail;
+                float* base = done ? static_cast<float*>(a.out) : parts;
 #pragma unroll 1
                 for (int c = 0; c < CW; c += 16) {
                     const int col = (TWO ? 0 : s * CW) + c;
@@ -899,10 +939,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                     __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
                     __syncwarp();
                     const int d = col + (lane & 3) * 4;
+                    if (goes_on) {  // onto what the pieces before left there
+#pragma unroll 1
+                        for (int i = 0; i < 4; ++i) {
+                            const float w = __shfl_sync(0xffffffffu, done ? kept * inv : kept, i * 8 + lane / 4);
+                            const int64_t from = __shfl_sync(0xffffffffu, partial, i * 8 + lane / 4);
+                            const int64_t dst = __shfl_sync(0xffffffffu, own, i * 8 + lane / 4);
+                            if (from < 0 || d >= a.D) continue;
+                            const uint4 x = ld_shared16(get + i * 512);
+                            const float4 y = *reinterpret_cast<const float4*>(parts + from + d);  // this lane's own
+                            *reinterpret_cast<float4*>(base + dst + d) =
+                                make_float4(fmaf(y.x, w, __uint_as_float(x.x)), fmaf(y.y, w, __uint_as_float(x.y)),
+                                            fmaf(y.z, w, __uint_as_float(x.z)), fmaf(y.w, w, __uint_as_float(x.w)));
+                        }
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint4 x = ld_shared16(get + i * 512);
-                        if (to[i] >= 0 && d < a.D) *reinterpret_cast<uint4*>(base + to[i] + d) = x;
+                        for (int i = 0; i < 4; ++i) {
+                            const uint4 x = ld_shared16(get + i * 512);
+                            if (to[i] >= 0 && d < a.D) *reinterpret_cast<uint4*>(base + to[i] + d) = x;
+                        }
                     }
                     __syncwarp();
                 }
@@ -932,7 +987,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     __syncwarp();
                 }
             }
-            if (live && (TWO || s == 0)) {
+            if (live && last && (TWO || s == 0)) {
                 if (c0 == cta) part.stat[orow] = pack_stat(M, L, PartPlace{c0, c1, slot_row, p.k.key0 > 0});
                 else part.tail_stat[slot] = make_float2(M, L);
             }
@@ -961,7 +1016,7 @@ void launch_tc_t(const BeaconCudaContext* ctx, const PagedTcPlan& plan, const Pa
     allow_smem_once(kern, ctx, allowed);
     const int entries = (a.merged ? 0 : a.groups) + (plan.rest ? a.B : 0);
     launch_kernel(kern, dim3((unsigned)plan.ctas), dim3(kTcThreads), TcSmem<DP, SPLIT, TWO>::bytes, s, pdl, a, maps, prefix, rest, entries,
-                  plan.ctas);
+                  plan.ctas, plan.rest ? 1 : 4);
 }
 
 template <int DP>
