@@ -132,7 +132,7 @@ __device__ __forceinline__ void prefetch_inputs(const PagedArgs& a, int q_bytes)
         for (long long i = first; i * 128 < bytes && i < first + 4 * step; i += step)
             asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p) + i * 128));
     };
-    const int t = threadIdx.x, n = blockDim.x;
+    const int t = threadIdx.x & 31, n = 32;
     ask(a.lens, a.B * 4LL, t, n);
     if (a.qstarts) ask(a.qstarts, (a.B + 1) * 4LL, t, n);
     if (a.gstarts) {

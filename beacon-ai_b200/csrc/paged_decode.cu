@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kDecThreads)
     float* merge_m = merge_o + kDecWarps * S::rows * DP;                                              // [warp][rows]
     float* merge_l = merge_m + kDecWarps * S::rows;
     float* scale_s = merge_l + kDecWarps * S::rows;                                                    // [rows]
-    prefetch_inputs(a, sizeof(TQ));
+    if (warp == kDecWarps - 1) prefetch_inputs(a, sizeof(TQ));
     if (lane == 0) {
         for (int i = 0; i < NS; ++i) mbar_init(&bars[warp][i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -132,7 +132,6 @@ __global__ void __launch_bounds__(kDecThreads)
     const Shares shares(total, part.ctas);
     const long long u0 = cta < shares.ctas ? shares.begin(cta) : 0, u1 = cta < shares.ctas ? shares.begin(cta + 1) : 0;
     pdl_trigger();
-    if (tid == 0 && !part.by_row) part.cuts[cta * 8] = -1;  // no row block of this CTA is cut at its end, until one is
     if (u0 < u1) {
         if (before * a.Hkv <= u0 && u0 < (before + mine) * a.Hkv) {
             int b = cb0;
@@ -433,14 +432,6 @@ __global__ void __launch_bounds__(kDecThreads)
                 const long long tile0 = u0 + j - at.tile;  // of this head, in the line
                 const int c0 = shares.of(tile0), c1 = shares.of(tile0 + at.cur.tiles - 1);
                 const bool done = c0 == c1 && at.cur.from == 0;  // no other part anywhere
-                if (tid == 0 && c0 == cta && c1 > c0 && !part.by_row) {  // the row block whose parts have to be joined
-                    int* rec = part.cuts + cta * 8;
-                    rec[0] = c1;
-                    rec[1] = at.b;
-                    rec[2] = 0;
-                    rec[3] = a.G;
-                    rec[4] = at.kvh;
-                }
                 for (int g = tid / (DP / 4); g < a.G; g += QR) {
                     float mw[kDecWarps], M = -INFINITY;
 #pragma unroll
@@ -493,10 +484,10 @@ __global__ void __launch_bounds__(kDecThreads)
     pdl_wait();
 }
 
-// The parts of the query rows where there are prefixes: kind 1, kind 0 where the
-// row has it, each a first part and those of the CTAs after it. One warp per
-// row. What is where stands in the row's entry, so nothing else has to be
-// looked up first.
+// The parts of the query rows where there are prefixes or single rows: kind 1,
+// kind 0 where the row has it, each a first part and those of the CTAs after
+// it. One warp per row. What is where stands in the row's entry, so nothing
+// else has to be looked up first.
 template <typename TQ, typename T16>
 __global__ void __launch_bounds__(128) paged_join_rows_kernel(const PagedArgs a, const PartArgs prefix, const PartArgs rest) {
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -505,13 +496,13 @@ __global__ void __launch_bounds__(128) paged_join_rows_kernel(const PagedArgs a,
     if (row >= (int64_t)a.T * a.H) return;
     float4 st[2];
     st[1] = rest.stat[row];
-    st[0] = prefix.stat[row];
+    st[0] = rest.by_row ? prefix.stat[row] : st[1];
     if (a.qstarts) {  // rows of no sequence are not written
         const int t = (int)(row / a.H);
         if (t < __ldg(a.qstarts) || t >= __ldg(a.qstarts + a.B)) return;
     }
     const PartPlace place = place_of(st[1]);
-    const bool both = place.prefix;
+    const bool both = rest.by_row && place.prefix;
     if (!both && place.c0 == place.c1) return;  // written by the CTA that had all of it
     // the parts in one line, a lane each
     const PartPlace pre = place_of(st[0]);
@@ -585,7 +576,7 @@ __global__ void __launch_bounds__(128) paged_join_rows_kernel(const PagedArgs a,
     }
 }
 
-// The same without prefixes: only the row blocks that were cut have to be
+// The same for several rows of a sequence without prefixes: only the row blocks that were cut have to be
 // joined (grid: CTA, rows of its block); the blocks for other CTAs leave at
 // once. A row has two or three parts mostly, so a warp has four rows, eight
 // lanes for the parts of each, and sixteen loads in flight.
@@ -717,7 +708,7 @@ void launch_paged_decode(const BeaconCudaContext* ctx, const PagedArgs& a, const
 
 void launch_paged_combine(const PagedArgs& a, const PartArgs& prefix, const PartArgs& rest, int32_t tq, cudaStream_t s) {
     auto go = [&](auto rows, auto cuts) {
-        if (rest.by_row)
+        if (rest.by_row || !a.qstarts)
             launch_kernel(rows, dim3((unsigned)(((int64_t)a.T * a.H + 3) / 4)), dim3(128), 0, s, true, a, prefix, rest);
         else
             launch_kernel(cuts, dim3((unsigned)rest.ctas, (unsigned)((rest.slot_rows + 15) / 16)), dim3(128), 0, s, true, a, rest);
