@@ -123,27 +123,6 @@ __device__ __forceinline__ int keep_in(int v, long long most, bool& bad) {
 }
 __device__ __forceinline__ long long capacity(const PagedArgs& a) { return (long long)a.max_pages * a.page_size; }
 
-// Asks for the index arrays and the queries (a share of the larger ones per
-// CTA) before anything reads them, so that the first use of each, which depends
-// on the one before, does not wait for memory in turn. Requests only: what an
-// earlier kernel still writes is read after pdl_wait.
-__device__ __forceinline__ void prefetch_inputs(const PagedArgs& a, int q_bytes) {
-    auto ask = [](const void* p, long long bytes, long long first, long long step) {
-        for (long long i = first; i * 128 < bytes && i < first + 4 * step; i += step)
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p) + i * 128));
-    };
-    const int t = threadIdx.x & 31, n = 32;
-    ask(a.lens, a.B * 4LL, t, n);
-    if (a.qstarts) ask(a.qstarts, (a.B + 1) * 4LL, t, n);
-    if (a.gstarts) {
-        ask(a.gstarts, (a.groups + 1) * 4LL, t, n);
-        ask(a.prefix, a.groups * 4LL, t, n);
-    }
-    const long long all = (long long)gridDim.x * n, at = (long long)t * gridDim.x + blockIdx.x;
-    ask(a.table, (long long)a.B * a.max_pages * 4, at, all);
-    ask(a.q, (long long)a.T * a.H * a.D * q_bytes, at, all);
-}
-
 // The i with starts[i] <= x < starts[i + 1] of an ascending array of n + 1
 // entries; -1 if there is none.
 __device__ __forceinline__ int span_of(const int32_t* starts, int n, int x) {

@@ -99,7 +99,6 @@ __global__ void __launch_bounds__(kDecThreads)
     float* merge_m = merge_o + kDecWarps * S::rows * DP;                                              // [warp][rows]
     float* merge_l = merge_m + kDecWarps * S::rows;
     float* scale_s = merge_l + kDecWarps * S::rows;                                                    // [rows]
-    if (warp == kDecWarps - 1) prefetch_inputs(a, sizeof(TQ));
     if (lane == 0) {
         for (int i = 0; i < NS; ++i) mbar_init(&bars[warp][i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");

@@ -307,7 +307,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (warp == kLoadWarp + kLoadWarps - 1) prefetch_inputs(a, sizeof(TQ));
     pdl_wait();
 
     // this CTA's share of the line
