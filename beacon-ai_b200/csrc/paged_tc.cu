@@ -281,6 +281,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __shared__ long long sums_s[kTcThreads / 32];
     __shared__ long long before_s;
     __shared__ int entry_s;
+    __shared__ int block_s[sizeof(Block) / sizeof(int)];
     uint8_t* q_smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* ring = q_smem + SM::q_tiles * SM::tile;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -313,7 +314,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int chunk = (entries + kTcThreads - 1) / kTcThreads;
     const int e0 = min(entries, tid * chunk), e1 = min(entries, e0 + chunk);
     long long mine = 0;
-    for (int e = e0; e < e1; ++e) mine += tiles_of_block(a, block_of(a, e), BR);
+    Block own;  // the last of them
+    for (int e = e0; e < e1; ++e) {
+        own = block_of(a, e);
+        mine += tiles_of_block(a, own, BR);
+    }
     long long scan = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -341,13 +346,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const long long u0 = cta < shares.ctas ? shares.begin(cta) : 0, u1 = cta < shares.ctas ? shares.begin(cta + 1) : 0;
     if (u0 < u1 && before * a.Hkv <= u0 && u0 < (before + mine) * a.Hkv) {
         int e = e0;
-        for (; e < e1; ++e) {
-            const int n = tiles_of_block(a, block_of(a, e), BR);
-            if (u0 < (before + n) * a.Hkv) break;
+        for (; e + 1 < e1; ++e) {
+            const Block k = block_of(a, e);
+            const int n = tiles_of_block(a, k, BR);
+            if (u0 < (before + n) * a.Hkv) {
+                own = k;
+                break;
+            }
             before += n;
         }
         entry_s = e;
         before_s = before;
+        *reinterpret_cast<Block*>(block_s) = own;
     }
     __syncthreads();
 
@@ -358,7 +368,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (u0 < u1) {
         pc.e = entry_s;
         pc.entries = entries;
-        pc.k = block_of(a, pc.e);
+        pc.k = *reinterpret_cast<const Block*>(block_s);
         const long long per = tiles_of_block(a, pc.k, BR), off = u0 - before_s * a.Hkv;
         pc.kvh = (int)(off / per);
         int at = (int)(off - pc.kvh * per);
@@ -686,6 +696,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int row = p.rt * BR + (TWO ? s * kTile : 0) + r;  // of the block
             const bool live = row < p.k.rows;
             const int tok = p.k.tok0 + row / a.G;
+            int limit = 0x7FFFFFFF;  // rows behind the block: whatever comes out is not written
+            if (live) {
+                if (p.k.kind) {
+                    limit = min(p.k.len, p.k.len - p.k.nq + row / a.G + 1);
+                } else if (!a.qstarts) {
+                    limit = max(0, min(p.k.key1, __ldg(a.lens + tok)));
+                } else {
+                    const int b = span_of(a.qstarts, a.B, tok);
+                    limit = 0;
+                    if (b >= 0) {
+                        const int len = max(0, (int)min((long long)__ldg(a.lens + b), capacity(a)));
+                        limit = min(p.k.key1, len - __ldg(a.qstarts + b + 1) + tok + 1);
+                    }
+                }
+            }
             const bool goes_on = SPLIT && seg > 0 && p.tile > 0;  // the row tile of the piece before
             if (SPLIT && !goes_on) {
                 ++loads;
@@ -725,19 +750,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 arrive(&qfull_bar);
-            }
-            int limit = 0x7FFFFFFF;  // rows behind the block: whatever comes out is not written
-            if (live) {
-                if (p.k.kind) {
-                    limit = min(p.k.len, p.k.len - p.k.nq + row / a.G + 1);
-                } else {
-                    const int b = a.qstarts ? span_of(a.qstarts, a.B, tok) : tok;
-                    limit = 0;
-                    if (b >= 0) {
-                        const SeqInfo si = seq_info(a, b);
-                        limit = min(p.k.key1, min(si.len, si.len - si.nq + (tok - si.q0) + 1));
-                    }
-                }
             }
             wait(&qfull_bar, (uint32_t)(seg & 1));
             if (!ok) break;
@@ -847,6 +859,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // more of this row tile: its next scores may be formed meanwhile
             const bool last = !SPLIT || p.tile + p.n == p.tiles || p.u + p.n >= u1;
             if (!last) arrive(&qfull_bar);
+            const PartArgs& part = p.k.kind ? rest : prefix;
+            const long long first = p.u - p.tile;
+            const int c0 = shares.of(first), c1 = shares.of(first + p.tiles - 1);
+            const bool whole = c0 == c1 && p.k.kind && p.k.key0 == 0;  // no other part anywhere
             wait(&ofin_bar, (uint32_t)(seg & 1));
             if (!ok) break;
             // --- results of the piece
@@ -873,10 +889,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 M = top;
             }
             if (!last) so_far_s[s][r] = make_float2(M, L);
-            const PartArgs& part = p.k.kind ? rest : prefix;
-            const long long first = p.u - p.tile;
-            const int c0 = shares.of(first), c1 = shares.of(first + p.tiles - 1);
-            const bool whole = c0 == c1 && p.k.kind && p.k.key0 == 0;  // no other part anywhere
             const bool done = whole && last;
             const int64_t orow = (int64_t)tok * a.H + p.kvh * a.G + row % a.G;
             const int slot_row = (TWO ? s * kTile : 0) + r;
