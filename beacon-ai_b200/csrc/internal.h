@@ -163,9 +163,12 @@ struct BeaconCudaStream {
     cudaStream_t s = nullptr;
     bool owned = false;
     bc::Workspace ws;  // split-K scratch, arrival counters and error flags of ops on this stream
-    // word that kernels set when an index held in a device tensor is out of
-    // range; host memory, so reading it costs no copy. Null until first needed.
+    // words that kernels set (StreamErr); host memory, so reading them costs no
+    // copy. Null until first needed.
     int* err_word = nullptr;
+    // held while an op enqueues several kernels that hand over scratch, so that
+    // calls of two threads on one stream do not mix
+    std::mutex launch_mu;
 };
 
 struct BeaconCudaTensor {

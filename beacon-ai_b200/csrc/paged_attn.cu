@@ -33,9 +33,11 @@ __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// One query row and head per block. Each warp takes every fourth key, its
-// lanes the head's values, with its own running maximum and sum; the warps'
-// parts are joined at the end. f32 throughout.
+// 32-bit caches, heads of more than 128 values, and caches without pages. One
+// query row and head per block; each warp takes every fourth key, its lanes the
+// head's values, with its own running maximum and sum; the warps' parts are
+// joined at the end. f32 throughout. Every row reads its keys for itself: bound
+// by L2 (a batch of 16 rows over 8192 keys, 32 heads on 8 of 128 values: 3.4 ms).
 template <typename TQ, typename TK>
 __global__ void __launch_bounds__(kAnyWarps * 32) paged_attn_any_kernel(const PagedArgs a) {
     constexpr int N = kAnyMaxDim / 32;
@@ -105,7 +107,7 @@ __global__ void __launch_bounds__(kAnyWarps * 32) paged_attn_any_kernel(const Pa
 }
 
 // Scratch of one call: the stream's workspace, which later calls on the stream
-// use again in stream order. A captured call gets memory of its graph instead,
+// use again in stream order (the caller holds the stream's launch_mu). A captured call gets memory of its graph instead,
 // so graphs captured on one stream can replay at the same time.
 class CallScratch {
    public:
@@ -189,7 +191,8 @@ CUtensorMap cache_map(const PagedArgs& a, const void* cache, int32_t tk, int box
 
 void run_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream, PagedArgs a, int32_t tq, int32_t tk) {
     const int32_t F32 = BEACON_CUDA_DTYPE_F32, F16 = BEACON_CUDA_DTYPE_F16;
-    if (tk != F32 && a.D <= 128) {
+    if (tk != F32 && a.D <= 128 && a.pages > 0) {
+        std::lock_guard<std::mutex> order(stream->launch_mu);
         // single rows of few heads: paged_decode_kernel; prefixes, several rows
         // of a sequence or many heads: the tensor-core kernel, whose row block is 128
         const bool decode = !a.qstarts && a.G <= kDecodeMaxGroup, tc = a.gstarts || !decode;
@@ -208,7 +211,7 @@ void run_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream, Paged
         CallScratch scratch(ctx, stream, carve(nullptr));
         carve(scratch.data());
         CacheMaps maps{}, dmaps{};
-        if (a.pages > 0 && a.page_size % 8 == 0) {
+        if (a.page_size % 8 == 0) {
             a.box = 8;
             while (a.box < 128 && a.page_size % (2 * a.box) == 0) a.box *= 2;
             if (tc) maps = {cache_map(a, a.ck, tk, a.box), cache_map(a, a.cv, tk, a.box)};

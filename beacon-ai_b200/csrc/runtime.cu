@@ -182,7 +182,7 @@ void check_stream_timeout(BeaconCudaStream* stream) {
             fail(BEACON_CUDA_ERR_DEVICE_TIMEOUT, "paged attention: a bounded device-side wait gave up; the op's output is invalid");
         if (index) {
             shape_err("a sequence number, position, length or page id held in a device tensor is out of range; "
-                      "the rows it names were left out");
+                      "it was not used, and the results that need it are not valid");
         }
     }
     if (!stream || !stream->ws.buf) return;

@@ -301,8 +301,10 @@ int32_t beacon_cuda_quantize_blocks(BeaconCudaContext* ctx, BeaconCudaStream* st
  *
  * Positions, sequence numbers, lengths and page tables are device tensors, so
  * the kernels check them: an entry that is out of range is never used as an
- * address, and the next synchronising call on the stream (stream_synchronize,
- * tensor_eval; tensor_read_*) returns SHAPE_MISMATCH. */
+ * address, the results that need it are not valid, and the next synchronising
+ * call on the stream (stream_synchronize, tensor_eval; tensor_read_*) returns
+ * SHAPE_MISMATCH. A replayed graph reports to the stream that it was captured
+ * on, which therefore outlives it, as do the tensors and rotations it reads. */
 typedef struct BeaconCudaRope BeaconCudaRope;
 /* Which values of a head form pair i of rotary_dim/2: (2i, 2i+1), or
  * (i, i + rotary_dim/2). */
@@ -373,12 +375,21 @@ int32_t beacon_cuda_op_paged_append(BeaconCudaContext* ctx, BeaconCudaStream* st
  * 0 upwards to B; NULL: none) hold the same keys below position prefix_lens[g]
  * (I32 [G]); those are read through the page table row of the group's first
  * sequence, once for all queries of the group.
- *   scale (not negative) multiplies the scores. A query that sees no key gives zeros. Rows of
- * q behind the last sequence are not written. Cache rows at positions >=
- * kv_lens[b] are never read. Dtypes (q, caches): (F32, F16), (F16, F16), (BF16,
- * BF16) and (F32, F32); D a multiple of 8 up to 256, tensors 16-byte aligned.
- * out: q's shape and dtype. Split partial results use the stream's scratch, or
- * memory that belongs to the graph while the stream is being captured. */
+ *   scale (finite, not negative) multiplies the scores. A query that sees no key
+ * gives zeros. Rows of q behind the last sequence are not written. What the
+ * cache holds at positions >= kv_lens[b] is not used, whatever it is; a value
+ * row below that is not finite may make results of queries of the sequence (or
+ * group) that do not see it NaN as well.
+ *   Dtypes (q, caches): (F32, F16), (F16, F16), (BF16, BF16) and (F32, F32); D a
+ * multiple of 8 up to 256, tensors 16-byte aligned. out: q's shape and dtype.
+ * Scores, softmax sums and value sums have 32 bits. F32 queries over F16 caches
+ * keep 22 bits of query and weights (2e-6 off 64 bits on normal values); 16-bit
+ * queries round the weights to their type. Fast for D <= 128 and 16-bit caches
+ * whose page size is a multiple of 8 (best 16 or more); other page sizes, D >
+ * 128 and F32 caches take slower kernels.
+ *   Partial results lie in the stream's scratch; of a captured call in memory
+ * of its graph (an allocation node and its release), so graphs captured on one
+ * stream may replay at the same time on several. */
 int32_t beacon_cuda_op_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream, const BeaconCudaTensor* q,
                                        const BeaconCudaTensor* cache_k, const BeaconCudaTensor* cache_v,
                                        const BeaconCudaTensor* page_table, const BeaconCudaTensor* kv_lens,
