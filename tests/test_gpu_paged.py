@@ -679,3 +679,66 @@ def test_attention_wait_timeout_is_reported(be, new, ps):
     assert L.ERR_DEVICE_TIMEOUT in statuses, statuses
     for _ in range(2):
         check_attention(be, s, rng, q, ck, cv, table, lens, "f16", "f16", starts)
+
+
+def test_attention_without_pages(be, s):
+    """A cache without pages, or a table without entries, holds no key: zeros; a length then is an error."""
+    from beacon_cuda import ShapeMismatch
+    from beacon_cuda import _lib as L
+    rng = np.random.default_rng(34)
+    some = Dev(be, np.zeros(16), "f16")
+    for pages, max_pages in ((0, 2), (3, 0), (0, 0)):
+        full = Dev(be, np.zeros((3, 16, 2, 64)), "f16")
+        cache = full.t if pages else be.wrap(some.x.data_ptr(), (0, 16, 2, 64), L.DTYPE_F16)
+        entries = i32(be, np.zeros((3, 2)))
+        table = entries.t if max_pages else be.wrap(some.x.data_ptr(), (3, 0), L.DTYPE_I32)
+        q, o = Dev(be, rng.standard_normal((3, 8, 64))), Dev(be, np.ones((3, 8, 64)))
+        lens = i32(be, [0, 0, 0])
+        be.paged_attention(s, q.t, cache, cache, table, lens.t, 1.0, out=o.t)
+        s.synchronize()
+        assert not o.f64().any()
+        lens = i32(be, [1, 0, 0])
+        be.paged_attention(s, q.t, cache, cache, table, lens.t, 1.0, out=o.t)
+        with pytest.raises(ShapeMismatch):
+            s.synchronize()
+
+
+def test_attention_on_the_default_stream(be):
+    rng = np.random.default_rng(35)
+    lens = [300, 40, 300]
+    s = be.wrap_stream(0)
+    ck, cv, table = make_cache(be, rng, 20, lens, 16, 2, 128, "bf16", [0, 3], [32])
+    q = Dev(be, rng.standard_normal((3, 8, 128)), "bf16")
+    check_attention(be, s, rng, q, ck, cv, table, lens, "bf16", "bf16", None, [0, 3], [32])
+
+
+def test_two_threads_on_one_stream(be):
+    """Calls of several launches from two threads do not mix."""
+    import threading
+    rng = np.random.default_rng(36)
+    H, Hkv, D, ps = 32, 8, 128, 16
+    s = be.new_stream()
+    jobs = []
+    for lens in ([900, 800, 700, 650], [40, 500, 300, 513]):
+        m = min(lens) // 2
+        ck, cv, table = make_cache(be, rng, 57, lens, ps, Hkv, D, "f16", [0, 4], [m])
+        q = Dev(be, rng.standard_normal((4, H, D)), "f16")
+        outs = [Dev(be, np.zeros((4, H, D)), "f16") for _ in range(50)]
+        jobs.append((q, ck, cv, table, lens, m, i32(be, table), i32(be, lens), i32(be, [0, 4]), i32(be, [m]), outs))
+
+    def work(j):
+        q, ck, cv, _, _, _, tb, ln, gs, pl, outs = j
+        for o in outs:
+            be.paged_attention(s, q.t, ck.t, cv.t, tb.t, ln.t, 0.1, group_starts=gs.t, prefix_lens=pl.t, out=o.t)
+
+    threads = [threading.Thread(target=work, args=(j,)) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    s.synchronize()
+    for q, ck, cv, table, lens, m, *_, outs in jobs:
+        want, info = ref.attention(q.f64(), ck.f64(), cv.f64(), table, lens, float(np.float32(0.1)), None, [0, 4], [m])
+        bound = ref.attention_bound(want, info, "f16", "f16", D)
+        for o in outs:
+            close(o.f64(), want, bound)
