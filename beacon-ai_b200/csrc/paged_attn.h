@@ -47,8 +47,8 @@ struct PartArgs {
     float* head = nullptr;    // [T * H][D], or [ctas][slot_rows][D] when !by_row
     float2* tail_stat = nullptr;  // [ctas][slot_rows]
     float* tail = nullptr;        // [ctas][slot_rows][D]
-    // Without prefixes only the row blocks that are cut have to be joined: per
-    // CTA the one whose first part it has, as [8]: last CTA (-1: none), first
+    // Of several rows of a sequence without prefixes only the row blocks that are
+    // cut have to be joined: per CTA the one whose first part it has, as [8]: last CTA (-1: none), first
     // token, first row, rows of its sequence's queries, KV head.
     int* cuts = nullptr;
     int by_row = 0;    // heads are kept per row: a row has both kinds

@@ -33,8 +33,8 @@
 // rows over 4096 shared keys, bf16, 32 heads on 8 of 128: 162 us, 747 TFLOP/s of
 // 1718; 39% tensor pipe, the exponentials and their conversions are the rest (a
 // 128 x 128 tile: 1024 cycles of products, about 1400 of softmax on 256 threads).
-// 64 rows behind a prefix of 16384: 106 us of which 65 are here. 32 rows, 32-bit,
-// behind 4096 keys: 52 us, of which 25 are here for 3.5 tiles a CTA: start, first
+// 64 rows behind a prefix of 16384: 104 us of which 63 are here. 32 rows, 32-bit,
+// behind 4096 keys: 50 us, of which 19 are here for 3.5 tiles a CTA: start, first
 // use of the code and the first tile's latency.
 // Every wait is bounded; one that runs out marks the stream's error word, and
 // the CTA waits for what it issued and ends.
