@@ -27,8 +27,8 @@
 // multiprocessor: the tensor copies are what feeds the matrix unit). One
 // thread issues the products. The key tiles of all blocks form one line that the CTAs
 // share evenly (PartArgs).
-// The running maximum moves only when a tile exceeds it by 2^8: the sums are
-// rescaled in tensor memory then, and the weights stay below 2^8.
+// The reference of the exponentials moves only when a tile exceeds it by some
+// powers of two (kMost): the sums are rescaled in tensor memory then.
 // Bounds, measured with both kernels around it (CUDA events): 4 prompts of 512
 // rows over 4096 shared keys, bf16, 32 heads on 8 of 128: 162 us, 747 TFLOP/s of
 // 1718; 39% tensor pipe, the exponentials and their conversions are the rest (a
@@ -57,7 +57,13 @@ constexpr int kLoadWarp = 8, kLoadWarps = 4;
 constexpr int kMmaWarp = 12;
 constexpr int kTcThreads = 32 * (kMmaWarp + 1);
 constexpr uint32_t kTmemCols = 512;     // S 2 x 128, O 2 x DP
-constexpr float kRescale = 8.0f;        // log2 of the largest weight
+// The weights are 2^(t - m) of scores t = scale log2(e) q . k and a reference m.
+// A tile whose largest score comes to be kMost above m moves m up to it; the sums
+// so far are rescaled then, which is rare.
+constexpr float kMost = 8.0f;
+// The weights' fused operation does not round t, but m is made of a rounded one:
+// for |t| from here on the difference, up to 2^-24 |t|, is taken care of.
+constexpr float kFar = 0x1p18f;
 
 template <int DP, bool SPLIT, bool TWO>
 struct TcSmem {
@@ -812,10 +818,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     tmem_ld32(s_col + ((c + 64) & (kTile - 1)), va);  // last: the first ones again
                     top = top_of(vb, top);
                 }
-                const float mx = fmaxf(m, top * cs);
-                const bool move = m != -INFINITY && mx > m + kRescale;
+                const float high = top * cs;
+                const bool move = m != -INFINITY && high - m > kMost;
                 if (t >= (TWO ? 1 : 2) && __any_sync(0xffffffffu, move)) {
-                    const float keep = move ? exp2_fast(m - mx) : 1.0f;
+                    const float keep = move ? exp2_fast(m - high) : 1.0f;
                     l *= keep;
 #pragma unroll 1
                     for (int c = 0; c < DP; c += 16) {
@@ -829,9 +835,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         tmem_st16(o_at, x);
                     }
                 }
-                if (move || m == -INFINITY) m = mx;
-                const float ref = m == -INFINITY ? 0.0f : m;
-                const float2 cs2 = make_float2(cs, cs), ref2 = make_float2(-ref, -ref);
+                if (move || (m == -INFINITY && high != -INFINITY)) m = high;
+                float ref = m == -INFINITY ? 0.0f : m, factor = cs;
+                if (__any_sync(0xffffffffu, fabsf(high) >= kFar && high != -INFINITY)) {
+                    // far scores: the exponents, from differences of scores, take their place
+                    const float from = high == -INFINITY ? 0.0f : top, add = high == -INFINITY ? -ref : high - ref;
+#pragma unroll 1
+                    for (int c = 0; c < kTile; c += 16) {
+                        float w[16];
+                        uint32_t x[16];
+                        tmem_ld16(s_col + c, w);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(fmaf(w[i] - from, cs, add));
+                        tmem_st16(s_col + c, x);
+                    }
+                    tmem_wait_st();
+                    tmem_ld32(s_col, va);
+                    factor = 1.0f;
+                    ref = 0.0f;
+                }
+                const float2 cs2 = make_float2(factor, factor), ref2 = make_float2(-ref, -ref);
                 float2 sum[2] = {make_float2(l, 0.0f), make_float2(0.0f, 0.0f)};
                 auto weights = [&](const float (&v)[32], int c) {
                     uint32_t w[16], w2[16];
