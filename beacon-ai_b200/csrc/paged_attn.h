@@ -39,9 +39,9 @@ struct PagedArgs {
 // CTAs. The CTA that has the first of them leaves m, l and where the parts are
 // in `stat` and its sums in `head`; the CTAs after it, each of which has at
 // most one such row block, leave theirs under their own number in `tail`.
-// m is the largest score times log2(e), l the sum of 2^(score - m), and the
-// sums are of 2^(score - m) v. Every row has an entry of kind 1, also one that
-// sees no key.
+// With scores times log2(e), m is the largest or a reference some powers of two
+// off it (-inf: no score above -inf), l the sum of 2^(score - m), and the sums are
+// of 2^(score - m) v. Every row has an entry of kind 1, also one that sees no key.
 struct PartArgs {
     float4* stat = nullptr;   // [T * H]: m, l, PartPlace
     float* head = nullptr;    // [T * H][D], or [ctas][slot_rows][D] when !by_row

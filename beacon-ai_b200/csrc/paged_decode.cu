@@ -35,6 +35,11 @@ namespace {
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kDecKeys = 16 * kDecWarps;  // keys of a tile
+// Factor on the weights and their sums (kNarrowExponent): the largest weight is
+// 2^15, so one of 2^-29 of it still has all 11 bits (22 in two parts down to
+// 2^-18), and none is off by more than 2^-40 of the largest.
+template <typename T>
+constexpr float kWeightScale = kNarrowExponent<T> ? 32768.0f : 1.0f;
 
 template <int DP, int NT, bool SPLIT>
 struct DecodeSmem {
@@ -364,8 +369,8 @@ __global__ void __launch_bounds__(kDecThreads)
                         moved |= keep[n][e] != 1.0f;
                         m[n][e] = mx;
                         ref[e] = mx == -INFINITY ? 0.0f : mx;
-                        sc[n][e] = exp2_fast(sc[n][e] - ref[e]);
-                        sc[n][2 + e] = exp2_fast(sc[n][2 + e] - ref[e]);
+                        sc[n][e] = exp2_fast(sc[n][e] - ref[e]) * kWeightScale<TK>;
+                        sc[n][2 + e] = exp2_fast(sc[n][2 + e] - ref[e]) * kWeightScale<TK>;
                         l[n][e] = l[n][e] * keep[n][e] + (sc[n][e] + sc[n][2 + e]);
                     }
                     if constexpr (SPLIT) {
@@ -447,7 +452,7 @@ __global__ void __launch_bounds__(kDecThreads)
                     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                     for (int w = 0; w < kDecWarps; ++w) {
-                        const float wt = mw[w] == -INFINITY ? 0.0f : exp2_fast(mw[w] - M);
+                        const float wt = mw[w] == -INFINITY ? 0.0f : exp2_fast(mw[w] - M) * (1.0f / kWeightScale<TK>);
                         const float4 v = *reinterpret_cast<const float4*>(merge_o + (w * S::rows + g) * DP + qd);
                         acc.x = fmaf(v.x, wt, acc.x);
                         acc.y = fmaf(v.y, wt, acc.y);

@@ -29,6 +29,17 @@ struct Half2Of<__nv_bfloat16> {
     static __device__ __forceinline__ float2 unpack(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v)); }
 };
 
+// Softmax weights for the value product are rounded to the cache's type. f16
+// ends at 2^-24 (normal values at 2^-14), so weights of at most 1 would lose
+// their bits from 2^-14 down and vanish below 2^-25, while their sum kept them:
+// thousands of small ones beside one large one would be lost from the result.
+// They are taken times a power of two that brings the largest near the top of
+// the range, and their sums alike, so that nothing else changes.
+template <typename T>
+constexpr bool kNarrowExponent = false;
+template <>
+constexpr bool kNarrowExponent<__half> = true;
+
 // 2^x (relative error 2^-22; -inf gives 0).
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;

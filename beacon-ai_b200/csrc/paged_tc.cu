@@ -58,9 +58,14 @@ constexpr int kMmaWarp = 12;
 constexpr int kTcThreads = 32 * (kMmaWarp + 1);
 constexpr uint32_t kTmemCols = 512;     // S 2 x 128, O 2 x DP
 // The weights are 2^(t - m) of scores t = scale log2(e) q . k and a reference m.
-// A tile whose largest score comes to be kMost above m moves m up to it; the sums
-// so far are rescaled then, which is rare.
-constexpr float kMost = 8.0f;
+// A tile whose largest score comes to be kMost above m moves m up, to kLift
+// below that score; the sums so far are rescaled then, which is rare. f16
+// (kNarrowExponent): the largest weight is always between 2^11 and 2^15, so one
+// of 2^-25 of it has all 11 bits and none is off by more than 2^-36 of the largest.
+template <typename T>
+constexpr float kMost = kNarrowExponent<T> ? 15.0f : 8.0f;
+template <typename T>
+constexpr float kLift = kNarrowExponent<T> ? 11.0f : 0.0f;
 // The weights' fused operation does not round t, but m is made of a rounded one:
 // for |t| from here on the difference, up to 2^-24 |t|, is taken care of.
 constexpr float kFar = 0x1p18f;
@@ -819,9 +824,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     top = top_of(vb, top);
                 }
                 const float high = top * cs;
-                const bool move = m != -INFINITY && high - m > kMost;
+                const float up = fabsf(high) < 16.0f * kFar ? high - kLift<T16> : high;  // (no room for it in far ones)
+                const bool move = m != -INFINITY && high - m > kMost<T16>;
                 if (t >= (TWO ? 1 : 2) && __any_sync(0xffffffffu, move)) {
-                    const float keep = move ? exp2_fast(m - high) : 1.0f;
+                    const float keep = move ? exp2_fast(m - up) : 1.0f;
                     l *= keep;
 #pragma unroll 1
                     for (int c = 0; c < DP; c += 16) {
@@ -835,7 +841,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         tmem_st16(o_at, x);
                     }
                 }
-                if (move || (m == -INFINITY && high != -INFINITY)) m = high;
+                if (move || (m == -INFINITY && high != -INFINITY)) m = up;
                 float ref = m == -INFINITY ? 0.0f : m, factor = cs;
                 if (__any_sync(0xffffffffu, fabsf(high) >= kFar && high != -INFINITY)) {
                     // far scores: the exponents, from differences of scores, take their place
