@@ -71,9 +71,10 @@ __global__ void __launch_bounds__(kAnyWarps * 32) paged_attn_any_kernel(const Pa
         }
         dot = warp_sum(dot);
         const float mn = fmaxf(m, dot);
-        // a row whose scores so far are all -inf keeps its empty sums
-        const float keep = m == -INFINITY ? 0.0f : expf(m - mn);
-        const float e = mn == -INFINITY ? 0.0f : expf(dot - mn);
+        // a row whose scores so far are all -inf keeps its empty sums; a score that
+        // is no number is in them from the start (fmaxf leaves it out)
+        const float keep = m == -INFINITY ? 1.0f : expf(m - mn);
+        const float e = expf(dot - (mn == -INFINITY ? 0.0f : mn));
         m = mn;
         l = l * keep + e;
 #pragma unroll
