@@ -546,7 +546,9 @@ __global__ void __launch_bounds__(128) paged_join_rows_kernel(const PagedArgs a,
             }
         }
         const float mx = fmaxf(M, warp_max(m));
-        if (mx == -INFINITY) continue;
+        // parts without a key; a sum that is no number (of scores that are none,
+        // which maxima leave out) is kept
+        if (mx == -INFINITY && !__any_sync(0xffffffffu, l != 0.0f)) continue;
         const float keep = M == -INFINITY ? 0.0f : exp2_fast(M - mx);
         const float w = m == -INFINITY ? 0.0f : exp2_fast(m - mx);
         M = mx;

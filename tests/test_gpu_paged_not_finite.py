@@ -3,11 +3,9 @@ import numpy as np
 import pytest
 
 import paged_reference as ref
-from test_gpu_paged import Dev, be, close, i32, make_cache, s  # noqa: F401 (be, s: fixtures)
+from test_gpu_paged import PAIRS, Dev, be, close, i32, make_cache, s  # noqa: F401 (be, s: fixtures)
 
 pytestmark = pytest.mark.gpu
-
-PAIRS = [("f32", "f32")]
 
 # (H, Hkv, D, page size, lengths, query rows, groups, prefixes); the second
 # sequence's keys lie in several parts of the line, the third's in one
