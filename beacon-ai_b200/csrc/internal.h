@@ -136,6 +136,25 @@ struct Workspace {
     static constexpr int kTimeoutFlag = 1;
 };
 
+// Scratch that several launches of one call hand on, taken and used in the
+// order of one stream under that stream's launch_mu. Calls captured into graphs
+// take none of it, so an outgrown block goes back in stream order.
+class CallArena {
+   public:
+    CallArena() = default;
+    ~CallArena();  // (after release)
+    CallArena(const CallArena&) = delete;
+    CallArena& operator=(const CallArena&) = delete;
+    void* get(size_t bytes, cudaStream_t s);
+    // Back to the device's pool behind the work of the stream.
+    void release(cudaStream_t s);
+
+   private:
+    void* p_ = nullptr;
+    size_t bytes_ = 0;
+    int device_ = 0;
+};
+
 }  // namespace bc
 
 struct BeaconCudaContext {
@@ -166,9 +185,12 @@ struct BeaconCudaStream {
     // words that kernels set (StreamErr); host memory, so reading them costs no
     // copy. Null until first needed.
     int* err_word = nullptr;
-    // held while an op enqueues several kernels that hand over scratch, so that
-    // calls of two threads on one stream do not mix
+    // partial results of paged attention. Other ops take `ws` without a lock, so
+    // what lies between two launches of a call must not lie there. The mutex is
+    // held while such a call enqueues its launches, so that two threads' calls
+    // on one stream do not mix.
     std::mutex launch_mu;
+    bc::CallArena arena;
 };
 
 struct BeaconCudaTensor {

@@ -107,17 +107,17 @@ __global__ void __launch_bounds__(kAnyWarps * 32) paged_attn_any_kernel(const Pa
     }
 }
 
-// Scratch of one call: the stream's workspace, which later calls on the stream
-// use again in stream order (the caller holds the stream's launch_mu). A captured call gets memory of its graph instead,
-// so graphs captured on one stream can replay at the same time.
+// Scratch of one call: the stream's arena, which later calls on the stream use
+// again in stream order (the caller holds the stream's launch_mu). A captured
+// call gets memory of its graph instead, so graphs captured on one stream can
+// replay at the same time.
 class CallScratch {
    public:
-    CallScratch(BeaconCudaContext* ctx, BeaconCudaStream* stream, size_t bytes) : s_(stream->s) {
+    CallScratch(BeaconCudaStream* stream, size_t bytes) : s_(stream->s) {
         cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
         BC_CUDA(cudaStreamIsCapturing(s_, &st));
         if (st == cudaStreamCaptureStatusNone) {
-            std::lock_guard<std::mutex> lk(ctx->streams_mu);
-            p_ = stream->ws.get(bytes, s_);
+            p_ = stream->arena.get(bytes, s_);
         } else {
             BC_CUDA(cudaMallocAsync(&p_, bytes, s_));
             graph_ = true;
@@ -209,7 +209,7 @@ void run_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream, Paged
             rest = decode ? carve_part(c, a, dctas, a.G, by_row) : carve_part(c, a, plan.ctas, plan.slot_rows, by_row);
             return c.used();
         };
-        CallScratch scratch(ctx, stream, carve(nullptr));
+        CallScratch scratch(stream, carve(nullptr));
         carve(scratch.data());
         CacheMaps maps{}, dmaps{};
         if (a.page_size % 8 == 0) {

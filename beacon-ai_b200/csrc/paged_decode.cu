@@ -113,8 +113,11 @@ __global__ void __launch_bounds__(kDecThreads)
         for (int i = 0; i < NS; ++i) mbar_init(&bars[warp][i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // After the tensor-core kernel of the same call nothing here depends on it,
-    // and it began only when what came before it was done.
+    // Behind the tensor-core kernel of the same call there is nothing to wait for.
+    // That one let later kernels start only after its own wait, so all that came
+    // before it is done, whatever another thread launched in between; and this one
+    // writes only its rows of the result and the call's own scratch, which no
+    // kernel but the call's touches.
     if (!after_tc) pdl_wait();
 
     // this CTA's share of the line

@@ -137,6 +137,30 @@ void* Workspace::get(size_t data_bytes, cudaStream_t s) {
     return static_cast<uint8_t*>(buf->ptr) + kDataOffset;
 }
 
+void* CallArena::get(size_t bytes, cudaStream_t s) {
+    if (bytes > bytes_) {
+        release(s);
+        const size_t want = (bytes + (1 << 20) - 1) >> 20 << 20;
+        BC_CUDA(cudaGetDevice(&device_));
+        BC_CUDA(cudaMallocAsync(&p_, want, s));
+        bytes_ = want;
+    }
+    return p_;
+}
+void CallArena::release(cudaStream_t s) {
+    if (!p_) return;
+    int before = 0;  // (the default stream is the current device's)
+    cudaGetDevice(&before);
+    if (before != device_) cudaSetDevice(device_);
+    cudaFreeAsync(p_, s);
+    if (before != device_) cudaSetDevice(before);
+    p_ = nullptr;
+    bytes_ = 0;
+}
+CallArena::~CallArena() {
+    if (p_) cudaFree(p_);
+}
+
 // Setters of the per-translation-unit copies of the device wait limit.
 static std::vector<cudaError_t (*)(long long)>& wait_limit_setters() {
     static std::vector<cudaError_t (*)(long long)> v;
@@ -402,6 +426,7 @@ void beacon_cuda_stream_destroy(BeaconCudaStream* stream) {
         std::lock_guard<std::mutex> lk(stream->ctx->streams_mu);
         stream->ctx->streams.erase(stream);
     }
+    stream->arena.release(stream->s);
     if (stream->s) cudaStreamSynchronize(stream->s);  // its workspace may still be in use
     if (stream->owned && stream->s) cudaStreamDestroy(stream->s);
     delete stream;

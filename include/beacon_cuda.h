@@ -387,9 +387,10 @@ int32_t beacon_cuda_op_paged_append(BeaconCudaContext* ctx, BeaconCudaStream* st
  * queries round the weights to their type. Fast for D <= 128 and 16-bit caches
  * whose page size is a multiple of 8 (best 16 or more); other page sizes, D >
  * 128 and F32 caches take slower kernels.
- *   Partial results lie in the stream's scratch; of a captured call in memory
- * of its graph (an allocation node and its release), so graphs captured on one
- * stream may replay at the same time on several. */
+ *   Partial results lie in memory that the stream keeps for this operation (a
+ * larger call replaces it in stream order); of a captured call in memory of its
+ * graph (an allocation node and its release), so graphs captured on one stream
+ * may replay at the same time on several. */
 int32_t beacon_cuda_op_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream, const BeaconCudaTensor* q,
                                        const BeaconCudaTensor* cache_k, const BeaconCudaTensor* cache_v,
                                        const BeaconCudaTensor* page_table, const BeaconCudaTensor* kv_lens,
