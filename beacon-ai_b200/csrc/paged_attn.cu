@@ -280,7 +280,11 @@ extern "C" int32_t beacon_cuda_op_paged_attention(BeaconCudaContext* ctx, Beacon
         if (page_table->shape.size() != 2) shape_err("paged_attention: page_table must be [B, max_pages]");
         const int64_t B = page_table->shape[0], max_pages = page_table->shape[1];
         if (T > 0x3FFFFFFF || B > 0x3FFFFFFF || max_pages > 0x7FFFFFFF) shape_err("paged_attention: too many rows or pages");
-        if (T * H > 0x7FFFFFFF) shape_err("paged_attention: more than 2^31 - 1 query heads");
+        // positions and row numbers are 32-bit in the kernels, which step past them by a tile
+        constexpr int64_t kMostIndex = 0x7FFFF000;
+        if (T * H > kMostIndex) shape_err("paged_attention: more than 2^31 - 4096 query heads");
+        if (max_pages * cache_k->shape[1] > kMostIndex)
+            shape_err("paged_attention: page_table has room for more than 2^31 - 4096 positions of a sequence");
         check_i32(ctx, kv_lens, B, "paged_attention: kv_lens");
         if (query_starts) check_i32(ctx, query_starts, B + 1, "paged_attention: query_starts");
         else if (T != B) shape_err("paged_attention: without query_starts every sequence has one query row");

@@ -381,7 +381,8 @@ int32_t beacon_cuda_op_paged_append(BeaconCudaContext* ctx, BeaconCudaStream* st
  * row below that is not finite may make results of queries of the sequence (or
  * group) that do not see it NaN as well.
  *   Dtypes (q, caches): (F32, F16), (F16, F16), (BF16, BF16) and (F32, F32); D a
- * multiple of 8 up to 256, tensors 16-byte aligned. out: q's shape and dtype.
+ * multiple of 8 up to 256, tensors 16-byte aligned; max_pages * page_size and
+ * T * H at most 2^31 - 4096. out: q's shape and dtype.
  * Scores, softmax sums and value sums have 32 bits. F32 queries over F16 caches
  * keep 22 bits of query and weights (2e-6 off 64 bits on normal values); 16-bit
  * queries round the weights to their type. Fast for D <= 128 and 16-bit caches
