@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <memory>
 #include <mutex>
@@ -183,8 +184,9 @@ struct BeaconCudaStream {
     bool owned = false;
     bc::Workspace ws;  // split-K scratch, arrival counters and error flags of ops on this stream
     // words that kernels set (StreamErr); host memory, so reading them costs no
-    // copy. Null until first needed.
-    int* err_word = nullptr;
+    // copy. Null until first needed (made under the context's streams_mu; atomic,
+    // since other threads look for it without).
+    std::atomic<int*> err_word{nullptr};
     // partial results of paged attention. Other ops take `ws` without a lock, so
     // what lies between two launches of a call must not lie there. The mutex is
     // held while such a call enqueues its launches, so that two threads' calls

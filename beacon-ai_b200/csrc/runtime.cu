@@ -170,10 +170,10 @@ void register_wait_limit_setter(cudaError_t (*setter)(long long)) { wait_limit_s
 
 int* stream_error_word(BeaconCudaStream* stream) {
     constexpr int kSlabWords = 512 * kErrWords;
-    if (stream->err_word) return stream->err_word;
+    if (int* made = stream->err_word) return made;
     BeaconCudaContext* ctx = stream->ctx;
     std::lock_guard<std::mutex> lk(ctx->streams_mu);
-    if (stream->err_word) return stream->err_word;
+    if (int* made = stream->err_word) return made;
     if (ctx->err_slabs.empty() || ctx->err_used == kSlabWords) {
         // a capture on this thread forbids allocating unless the thread's
         // capture mode is relaxed; no stream work is enqueued here
@@ -192,14 +192,15 @@ int* stream_error_word(BeaconCudaStream* stream) {
         }
         ctx->err_used = 0;
     }
-    stream->err_word = ctx->err_slabs.back() + ctx->err_used;
+    int* made = ctx->err_slabs.back() + ctx->err_used;
     ctx->err_used += kErrWords;
-    return stream->err_word;
+    stream->err_word = made;
+    return made;
 }
 
 void check_stream_timeout(BeaconCudaStream* stream) {
-    if (stream && stream->ctx && stream->err_word) {
-        volatile int* w = stream->err_word;  // the stream's work is done: no kernel is writing it
+    volatile int* w = stream && stream->ctx ? stream->err_word.load() : nullptr;
+    if (w) {  // the stream's work is done: no kernel is writing it
         const bool gave_up = w[kErrWordWait] != 0, index = w[kErrWordIndex] != 0;
         w[kErrWordWait] = w[kErrWordIndex] = 0;
         if (gave_up)

@@ -100,3 +100,29 @@ def test_scratch_goes_back(be):
         torch.cuda.synchronize()
         free.append(torch.cuda.mem_get_info()[0])
     assert free[-1] >= free[0] - (8 << 20)            # 32 MB of sums a call
+
+
+def test_first_calls_of_many_threads(be):
+    """Threads that use a new stream at once share its error words: an index out
+    of range in one of their calls is reported, once."""
+    from beacon_cuda import ShapeMismatch
+    rng = np.random.default_rng(64)
+    k = Dev(be, rng.standard_normal((1, 2, 64)))
+    tb, good, bad = i32(be, [[0, 1]]), i32(be, [3]), i32(be, [99])
+    caches = [(Dev(be, np.zeros((2, 4, 2, 64)), "f16"), Dev(be, np.zeros((2, 4, 2, 64)), "f16")) for _ in range(8)]
+    for rnd in range(20):
+        s = be.new_stream()
+        gate = threading.Barrier(8)
+
+        def work(i):
+            gate.wait()
+            be.paged_append(s, caches[i][0].t, caches[i][1].t, k.t, k.t, tb.t, (bad if i == rnd % 8 else good).t)
+
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        with pytest.raises(ShapeMismatch):
+            s.synchronize()
+        s.synchronize()
