@@ -12,8 +12,8 @@
 // its next two tokens (64 bytes a lane, 32 warps an SM) are always in flight. The sines and
 // cosines of the block's tokens are computed once into shared memory while the
 // first loads are on their way: the angle is a 64-bit product position * f_i /
-// 2 pi reduced to one turn, then sincospif in 32 bits, so position 10^6 is as
-// exact as position 1. (Every warp computing its own: 1200 instructions a
+// 2 pi reduced to one turn, then sincospif in 32 bits with the rest of the angle
+// to first order, so position 10^6 is as exact as position 1. (Every warp computing its own: 1200 instructions a
 // token and 60 us for 8192 x 32 heads of 128 bf16 values, 20 us of memory.)
 // Measured, bf16, heads of 128: rotation of 8192 x 32 heads 28.9 us (4.65 TB/s),
 // norms and rotation of 4099 x (64 + 8) heads 34.8 us (4.3 TB/s), append of about
@@ -165,9 +165,13 @@ __device__ __forceinline__ int64_t cache_row(const RowArgs& a, int64_t t) {
 __device__ __forceinline__ float2 turn_at(const RowArgs& a, int position, int pair) {
     double turn = (double)position * __ldg(a.turns + pair);
     turn -= rint(turn);
+    // sine and cosine at the turn's 32-bit value, then turned by what that left
+    // (at most 2^-26 of a turn, so its square is nothing in 32 bits)
+    const float near = (float)turn;
+    const float left = (float)((turn - near) * 6.283185307179586);
     float s, c;
-    sincospif(2.0f * (float)turn, &s, &c);
-    return make_float2(c * a.amplitude, s * a.amplitude);
+    sincospif(2.0f * near, &s, &c);
+    return make_float2(fmaf(-s, left, c) * a.amplitude, fmaf(c, left, s) * a.amplitude);
 }
 
 // What a block computes before its heads: sines and cosines, norm weights in 32
