@@ -529,22 +529,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (Piece p = pc; ok && p.u < u1; p.next(a, BR, u1), ++seg) {
             // the first tiles are on their way while the queries are brought in
             // A key tile's pages are fetched when the one before it is requested, and
-            // its rows kept for the value tile, up to LA + 1 of them.
-            int f = 0, page = page_of(p, 0), rows[3] = {-1, -1, -1}, kept = 0;
+            // its rows kept for the value tile, up to LA of them.
+            int f = 0, page = page_of(p, 0), rows[2] = {-1, -1}, kept = 0;
             auto load_next = [&]() {
                 bool value;
                 const int t = key_tile(p, f++, value);
                 int row = rows[0];
                 if (value) {
                     rows[0] = rows[1];
-                    rows[1] = rows[2];
                     --kept;
                 } else {
                     row = row_of(p, t, page);
                     page = page_of(p, t + 1);
                     if (kept == 0) rows[0] = row;
-                    else if (kept == 1) rows[1] = row;
-                    else rows[2] = row;
+                    else rows[1] = row;
                     ++kept;
                 }
                 load_tile(p, t, value, row);

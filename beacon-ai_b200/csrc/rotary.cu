@@ -215,9 +215,9 @@ __device__ __forceinline__ void fill_tables(const RowArgs& a, const RowSegment& 
 // their partners; the lanes after those take the unrotated rest, two slots
 // each. Interleaved: slots 2l and 2l + 1, whose pairs lie inside a slot. Either
 // way lane l turns pairs l V .. l V + V - 1.
-// A block has the tokens [t0, t0 + nt) of one segment; a warp has one group of
-// heads after another (as many heads as its lanes hold) and goes through the
-// tokens, or shares them where there are fewer groups than warps.
+// A block has the tokens [t0, t0 + nt) and up to kRowWarps head groups (as many
+// heads as a warp's lanes hold) of one segment; a warp goes through the tokens of
+// one group, or shares them where there are fewer groups than warps.
 template <typename TI, typename TO, bool HALF, bool NORM>
 __global__ void __launch_bounds__(kRowThreads, 4) row_kernel(const __grid_constant__ RowArgs a) {
     constexpr int V = Slot<TI>::V;
@@ -247,14 +247,13 @@ __global__ void __launch_bounds__(kRowThreads, 4) row_kernel(const __grid_consta
     const bool has1 = at1 < a.dim;
     // the block's head groups, and the warps that share one
     const int ng = (sg.heads + groups - 1) / groups, g0 = part * a.part_groups, n = min(ng, g0 + a.part_groups) - g0;
-    const int cols = min(n, kRowWarps), share = kRowWarps / cols;
-    const int first = warp / cols < share ? warp / cols : nt;  // first token of this warp; then every share-th
-    const int stride = sg.heads * a.dim;                       // values from one token to the next
-    int g = g0 + warp % cols;
-    int h = g * groups + (threadIdx.x & 31) / a.lanes;
-    const TI* src = static_cast<const TI*>(sg.src) + t0 * stride + (int64_t)h * a.dim + at0;
+    const int share = kRowWarps / n;                     // n is at most kRowWarps
+    const int first = warp / n < share ? warp / n : nt;  // first token of this warp; then every share-th
+    const int stride = sg.heads * a.dim;                 // values from one token to the next
+    const int h = (g0 + warp % n) * groups + (threadIdx.x & 31) / a.lanes;
+    const TI* const src = static_cast<const TI*>(sg.src) + t0 * stride + (int64_t)h * a.dim + at0;
     const int to1 = at1 - at0;
-    bool live = h < sg.heads && at0 < a.dim;
+    const bool live = h < sg.heads && at0 < a.dim;
 
     uint4 x0[U], x1[U];
     auto load = [&](int u, int t) {
@@ -268,85 +267,76 @@ __global__ void __launch_bounds__(kRowThreads, 4) row_kernel(const __grid_consta
     for (int u = 0; u < U; ++u) load(u, first + u * share);
     fill_tables(a, sg, tab, t0, nt);
     __syncthreads();
-    for (;;) {
 #pragma unroll 1
-        for (int t = first; t < nt;) {
-            int at = t * hs + lane * V;  // this lane's first pair in the tables
+    for (int t = first; t < nt;) {
+        int at = t * hs + lane * V;  // this lane's first pair in the tables
 #pragma unroll
-            for (int u = 0; u < U; ++u, t += share, at += share * hs) {
-                if (t >= nt) break;  // the warp's lanes agree
-                float f0[V], f1[V];
-                Slot<TI>::unpack(x0[u], f0);
-                Slot<TI>::unpack(x1[u], f1);
-                load(u, t + U * share);
-                if (NORM) {
-                    float ss = 0.0f;
+        for (int u = 0; u < U; ++u, t += share, at += share * hs) {
+            if (t >= nt) break;  // the warp's lanes agree
+            float f0[V], f1[V];
+            Slot<TI>::unpack(x0[u], f0);
+            Slot<TI>::unpack(x1[u], f1);
+            load(u, t + U * share);
+            if (NORM) {
+                float ss = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        if (live) ss = fmaf(f0[j], f0[j], ss);
-                        if (live && has1) ss = fmaf(f1[j], f1[j], ss);
-                    }
-                    for (int o = a.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                    const float inv = rsqrtf(fmaf(ss, a.inv_dim, a.eps));
-                    if (live) {
-#pragma unroll
-                        for (int j = 0; j < V; j += 4) {
-                            const float2 in = make_float2(inv, inv);
-                            const float4 p = *reinterpret_cast<const float4*>(tab.weight + at0 + j);
-                            put2(f0 + j, mul2(get2(f0 + j), mul2(in, make_float2(p.x, p.y))));
-                            put2(f0 + j + 2, mul2(get2(f0 + j + 2), mul2(in, make_float2(p.z, p.w))));
-                            if (has1) {
-                                const float4 q = *reinterpret_cast<const float4*>(tab.weight + at1 + j);
-                                put2(f1 + j, mul2(get2(f1 + j), mul2(in, make_float2(q.x, q.y))));
-                                put2(f1 + j + 2, mul2(get2(f1 + j + 2), mul2(in, make_float2(q.z, q.w))));
-                            }
-                        }
-                    }
+                for (int j = 0; j < V; ++j) {
+                    if (live) ss = fmaf(f0[j], f0[j], ss);
+                    if (live && has1) ss = fmaf(f1[j], f1[j], ss);
                 }
-                if (turn) {
+                for (int o = a.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const float inv = rsqrtf(fmaf(ss, a.inv_dim, a.eps));
+                if (live) {
 #pragma unroll
                     for (int j = 0; j < V; j += 4) {
-                        // pairs lane V + j .. + 3 (the rotated part has a multiple of 4 values;
-                        // entries of pairs that it does not have are not used)
-                        if (!HALF && at0 + 2 * j >= a.rotary) continue;
-                        const float4 c = *reinterpret_cast<const float4*>(tab.cos + at + j), s = *reinterpret_cast<const float4*>(tab.sin + at + j);
-                        if (HALF) {
-                            const float2 c2[2] = {make_float2(c.x, c.y), make_float2(c.z, c.w)}, s2[2] = {make_float2(s.x, s.y), make_float2(s.z, s.w)};
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const float2 x = get2(f0 + j + 2 * i), y = get2(f1 + j + 2 * i);
-                                put2(f0 + j + 2 * i, fma2(make_float2(-y.x, -y.y), s2[i], mul2(x, c2[i])));
-                                put2(f1 + j + 2 * i, fma2(x, s2[i], mul2(y, c2[i])));
-                            }
-                        } else {
-                            const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                // pair j + i of the lane's 2 V values
-                                float* f = 2 * (j + i) < V ? f0 + 2 * (j + i) : f1 + 2 * (j + i) - V;
-                                if (at0 + 2 * (j + i) >= a.rotary) continue;
-                                const float x = f[0], y = f[1];
-                                f[0] = x * cv[i] - y * sv[i];
-                                f[1] = y * cv[i] + x * sv[i];
-                            }
+                        const float2 in = make_float2(inv, inv);
+                        const float4 p = *reinterpret_cast<const float4*>(tab.weight + at0 + j);
+                        put2(f0 + j, mul2(get2(f0 + j), mul2(in, make_float2(p.x, p.y))));
+                        put2(f0 + j + 2, mul2(get2(f0 + j + 2), mul2(in, make_float2(p.z, p.w))));
+                        if (has1) {
+                            const float4 q = *reinterpret_cast<const float4*>(tab.weight + at1 + j);
+                            put2(f1 + j, mul2(get2(f1 + j), mul2(in, make_float2(q.x, q.y))));
+                            put2(f1 + j + 2, mul2(get2(f1 + j + 2), mul2(in, make_float2(q.z, q.w))));
                         }
                     }
                 }
-                const int64_t row = a.table ? tab.rows[t] : t0 + t;
-                if (live && row >= 0) {
-                    TO* dst = static_cast<TO*>(sg.dst) + row * stride + (h * a.dim + at0);
-                    store_slot<TO, V>(dst, f0);
-                    if (has1) store_slot<TO, V>(dst + to1, f1);
+            }
+            if (turn) {
+#pragma unroll
+                for (int j = 0; j < V; j += 4) {
+                    // pairs lane V + j .. + 3 (the rotated part has a multiple of 4 values;
+                    // entries of pairs that it does not have are not used)
+                    if (!HALF && at0 + 2 * j >= a.rotary) continue;
+                    const float4 c = *reinterpret_cast<const float4*>(tab.cos + at + j), s = *reinterpret_cast<const float4*>(tab.sin + at + j);
+                    if (HALF) {
+                        const float2 c2[2] = {make_float2(c.x, c.y), make_float2(c.z, c.w)}, s2[2] = {make_float2(s.x, s.y), make_float2(s.z, s.w)};
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float2 x = get2(f0 + j + 2 * i), y = get2(f1 + j + 2 * i);
+                            put2(f0 + j + 2 * i, fma2(make_float2(-y.x, -y.y), s2[i], mul2(x, c2[i])));
+                            put2(f1 + j + 2 * i, fma2(x, s2[i], mul2(y, c2[i])));
+                        }
+                    } else {
+                        const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            // pair j + i of the lane's 2 V values
+                            float* f = 2 * (j + i) < V ? f0 + 2 * (j + i) : f1 + 2 * (j + i) - V;
+                            if (at0 + 2 * (j + i) >= a.rotary) continue;
+                            const float x = f[0], y = f[1];
+                            f[0] = x * cv[i] - y * sv[i];
+                            f[1] = y * cv[i] + x * sv[i];
+                        }
+                    }
                 }
             }
+            const int64_t row = a.table ? tab.rows[t] : t0 + t;
+            if (live && row >= 0) {
+                TO* dst = static_cast<TO*>(sg.dst) + row * stride + (h * a.dim + at0);
+                store_slot<TO, V>(dst, f0);
+                if (has1) store_slot<TO, V>(dst + to1, f1);
+            }
         }
-        g += cols;
-        if (g >= g0 + n) break;
-        h += cols * groups;
-        src += (int64_t)cols * groups * a.dim;
-        live = h < sg.heads && at0 < a.dim;
-#pragma unroll
-        for (int u = 0; u < U; ++u) load(u, first + u * share);
     }
 }
 
