@@ -306,13 +306,23 @@ def _backend():
     if path not in sys.path:
         sys.path.insert(0, path)
     import beacon_cuda
-    be = beacon_cuda.CudaBackend(0)
-    return be, be.wrap_stream(torch.cuda.current_stream().cuda_stream), beacon_cuda._lib
+    return beacon_cuda.CudaBackend(0), beacon_cuda._lib
+
+
+_streams = {}
+
+
+def _stream():
+    """The framework's handle of torch's current stream, kept as a program keeps it."""
+    raw = torch._C._cuda_getCurrentRawStream(0)  # (a Stream object costs microseconds)
+    if raw not in _streams:
+        _streams[raw] = _backend()[0].wrap_stream(raw)
+    return _streams[raw]
 
 
 @functools.lru_cache(maxsize=None)
 def _rope_handle(scaling, rotary, layout):
-    be, _, L = _backend()
+    be, L = _backend()
     kind, theta, factor, orig = SCALINGS[scaling]
     kinds = {"none": L.ROPE_SCALING_NONE, "linear": L.ROPE_SCALING_LINEAR, "yarn": L.ROPE_SCALING_YARN,
              "bands": L.ROPE_SCALING_BANDS}
@@ -323,7 +333,7 @@ def _rope_handle(scaling, rotary, layout):
 def _handles(s):
     """The tensors of a state as the framework's, kept with it as a program keeps them."""
     if "handles" not in s:
-        be, _, L = _backend()
+        be, L = _backend()
         kind = {torch.float32: L.DTYPE_F32, torch.float16: L.DTYPE_F16, torch.bfloat16: L.DTYPE_BF16,
                 torch.int32: L.DTYPE_I32}
         for name in ("q", "k"):
@@ -337,7 +347,7 @@ def _handles(s):
 
 
 def _own(s):
-    be, stream, _ = _backend()
+    be, stream = _backend()[0], _stream()
     t = _handles(s)
     op = s["case"]["op"]
     if op == "rope":
