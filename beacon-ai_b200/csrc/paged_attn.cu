@@ -37,7 +37,8 @@ __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bf
 // query row and head per block; each warp takes every fourth key, its lanes the
 // head's values, with its own running maximum and sum; the warps' parts are
 // joined at the end. f32 throughout. Every row reads its keys for itself: bound
-// by L2 (a batch of 16 rows over 8192 keys, 32 heads on 8 of 128 values: 3.4 ms).
+// by L2, and a row's keys stay with one block (16 rows of 8192 keys each, 32 heads
+// on 8 of 128 values: 4.8 ms; one row alone: 4.9 ms).
 template <typename TQ, typename TK>
 __global__ void __launch_bounds__(kAnyWarps * 32) paged_attn_any_kernel(const PagedArgs a) {
     constexpr int N = kAnyMaxDim / 32;
@@ -194,10 +195,18 @@ void run_paged_attention(BeaconCudaContext* ctx, BeaconCudaStream* stream, Paged
     const int32_t F32 = BEACON_CUDA_DTYPE_F32, F16 = BEACON_CUDA_DTYPE_F16;
     if (tk != F32 && a.D <= 128 && a.pages > 0) {
         std::lock_guard<std::mutex> order(stream->launch_mu);
-        // single rows of few heads: paged_decode_kernel; prefixes, several rows
-        // of a sequence or many heads: the tensor-core kernel, whose row block is 128
+        // Single rows of few heads: paged_decode_kernel; prefixes, several rows of a
+        // sequence or many heads: the tensor-core kernel, whose row block is 128.
+        // (bf16, 8 KV heads of 128, either kernel: 16 rows of 8192 keys 110 and 122 us
+        // with 2 heads a KV head, 114 and 122 with 16; 64 rows of 512 keys 42 and 63,
+        // 48 and 63; 32-bit queries 112 and 175, 122 and 189; 44 and 85, 52 and 91.)
         const bool decode = !a.qstarts && a.G <= kDecodeMaxGroup, tc = a.gstarts || !decode;
         const bool split = tq == F32;
+        // Sequences whose rows fill row blocks of 128 take prefix and rest together,
+        // others share the prefix. (8 sequences behind 2048 keys with 128 each of their
+        // own, 32 heads on 8 of 128, bf16, by rows a sequence and KV head, apart and
+        // together: 16: 28 and 38 us, 64: 42 and 40, 128: 54 and 40, 512: 169 and 75. 63
+        // single rows and one prompt of 512 rows: 120 and 159; of 2000 rows: 292 and 298.)
         a.merged = a.qstarts && (int64_t)a.T * a.G >= 128LL * a.B;
         const bool by_row = a.gstarts && !a.merged;
         const PagedTcPlan plan = tc ? plan_paged_tc(ctx, a, split, !decode) : PagedTcPlan{};

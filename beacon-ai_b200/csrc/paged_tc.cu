@@ -30,12 +30,12 @@
 // The reference of the exponentials moves only when a tile exceeds it by some
 // powers of two (kMost): the sums are rescaled in tensor memory then.
 // Bounds, measured with both kernels around it (CUDA events): 4 prompts of 512
-// rows over 4096 shared keys, bf16, 32 heads on 8 of 128: 162 us, 747 TFLOP/s of
-// 1718; 39% tensor pipe, the exponentials and their conversions are the rest (a
-// 128 x 128 tile: 1024 cycles of products, about 1400 of softmax on 256 threads).
-// 64 rows behind a prefix of 16384: 104 us of which 63 are here. 32 rows, 32-bit,
-// behind 4096 keys: 50 us, of which 19 are here for 3.5 tiles a CTA: start, first
-// use of the code and the first tile's latency.
+// rows over 4096 shared keys, bf16, 32 heads on 8 of 128: 163 us, 745 TFLOP/s of
+// 1718, 39% tensor pipe. A pair of 128 x 128 tiles takes about 5,700 cycles, 2,048
+// of them products; how the rest divides between the softmax threads and the
+// hand-overs to them is not measured. 64 rows behind a prefix of 16384: 105 us of
+// which 61 are here. 32 rows, 32-bit, behind 4096 keys: 49 us, of which 19 are here
+// for 3.5 tiles a CTA: start, first use of the code and the first tile's latency.
 // Every wait is bounded; one that runs out marks the stream's error word, and
 // the CTA waits for what it issued and ends.
 #include <algorithm>
@@ -1081,7 +1081,11 @@ void launch_tc_d(const BeaconCudaContext* ctx, const PagedTcPlan& plan, const Pa
 
 PagedTcPlan plan_paged_tc(const BeaconCudaContext* ctx, const PagedArgs& a, bool split, bool with_rest) {
     PagedTcPlan p;
-    // blocks of more than 128 rows on average share each key tile between two row tiles
+    // Blocks of more than 128 rows on average share each key tile between two row
+    // tiles. (bf16, 32 heads on 8 of 128, one row tile and two: 16 sequences over 1024
+    // keys, rows a sequence and KV head 64: 42 and 46 us, 128: 44 and 48, 160: 60 and 52,
+    // 512: 89 and 81, 2048: 224 and 181; 4 over 2048, which leave CTAs idle: 256: 42 and
+    // 44, 512: 50 and 52, 2048: 120 and 106.)
     p.two = !split && (int64_t)a.T * a.G > 128LL * (a.groups && !a.merged ? a.groups : a.B);
     p.rest = with_rest;
     p.slot_rows = p.two ? 2 * kTile : kTile;

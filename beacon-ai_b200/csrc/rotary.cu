@@ -15,9 +15,9 @@
 // 2 pi reduced to one turn, then sincospif in 32 bits with the rest of the angle
 // to first order, so position 10^6 is as exact as position 1. (Every warp computing its own: 1200 instructions a
 // token and 60 us for 8192 x 32 heads of 128 bf16 values, 20 us of memory.)
-// Measured, bf16, heads of 128: rotation of 8192 x 32 heads 28.9 us (4.65 TB/s),
+// Measured, bf16, heads of 128: rotation of 8192 x 32 heads 27.1 us (4.95 TB/s),
 // norms and rotation of 4099 x (64 + 8) heads 34.8 us (4.3 TB/s), append of about
-// 8200 rows of 8 heads 16.7 us (4.0 TB/s); a handful of tokens costs the launch.
+// 8200 rows of 8 heads 16.4 us (4.1 TB/s); a handful of tokens costs the launch.
 #include <cuda_bf16.h>
 
 #include <algorithm>

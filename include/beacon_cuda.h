@@ -374,18 +374,25 @@ int32_t beacon_cuda_op_paged_append(BeaconCudaContext* ctx, BeaconCudaStream* st
  *   Shared prefixes: sequences group_starts[g] .. group_starts[g+1] (I32 [G+1],
  * 0 upwards to B; NULL: none) hold the same keys below position prefix_lens[g]
  * (I32 [G]); those are read through the page table row of the group's first
- * sequence, once for all queries of the group.
- *   scale (finite, not negative) multiplies the scores. A query that sees no key
- * gives zeros. Rows of q behind the last sequence are not written. What the
- * cache holds at positions >= kv_lens[b] is not used, whatever it is; a value
- * row below that is not finite may make results of queries of the sequence (or
- * group) that do not see it NaN as well.
+ * sequence, and once for all queries of the group, unless the sequences have
+ * 128 and more query rows a KV head on average (T H/Hkv >= 128 B): each takes
+ * its prefix with its own keys then, as the rows of one fill the matrix unit.
+ *   scale (finite, not negative) multiplies the scores. A query that sees no key,
+ * or whose scores are all -inf, gives zeros; a score that is +inf or NaN gives
+ * NaN (with F32 queries over F16 caches any key that is not finite does). Rows of
+ * q behind the last sequence are not written. What the cache holds at positions
+ * >= kv_lens[b] is not used, whatever it is; a value row below that is not finite
+ * may make results of queries of the sequence (or group) that do not see it NaN
+ * as well.
  *   Dtypes (q, caches): (F32, F16), (F16, F16), (BF16, BF16) and (F32, F32); D a
  * multiple of 8 up to 256, tensors 16-byte aligned; max_pages * page_size and
  * T * H at most 2^31 - 4096. out: q's shape and dtype.
- * Scores, softmax sums and value sums have 32 bits. F32 queries over F16 caches
- * keep 22 bits of query and weights (2e-6 off 64 bits on normal values); 16-bit
- * queries round the weights to their type. Fast for D <= 128 and 16-bit caches
+ * Scores, softmax sums and value sums have 32 bits. For the value sums the
+ * softmax weights are rounded: to the type of 16-bit queries (2^-11 or 2^-8 of
+ * each), to 22 bits with F32 queries over F16 caches, which keep 22 bits of the
+ * query too (2e-6 off 64 bits on normal values). F16 weights have fewer bits below
+ * 2^-25 (22 of them: 2^-14) of the row's largest and are off by 2^-36 of that at
+ * most. Fast for D <= 128 and 16-bit caches
  * whose page size is a multiple of 8 (best 16 or more); other page sizes, D >
  * 128 and F32 caches take slower kernels.
  *   Partial results lie in memory that the stream keeps for this operation (a
