@@ -126,3 +126,55 @@ def test_first_calls_of_many_threads(be):
         with pytest.raises(ShapeMismatch):
             s.synchronize()
         s.synchronize()
+
+
+@pytest.mark.parametrize("new", [None, 2])
+def test_inputs_that_change_on_the_stream(be, new):
+    """Queries, lengths, tables and cache rows written by kernels right before
+    each call, with no wait between: every call reads what stands there then."""
+    import torch
+    rng = np.random.default_rng(65)
+    H, Hkv, D, ps, B, N = 32, 8, 128, 16, 6, 60
+    lens = [700, 640, 513, 777, 600, 530]
+    ck, cv, table = make_cache(be, rng, 50, lens, ps, Hkv, D, "f16", [0, B], [512])
+    for c in (ck, cv):
+        c.x.nan_to_num_()
+    side = torch.cuda.Stream()
+    s = be.wrap_stream(side.cuda_stream)
+    T = B * (new or 1)
+    q, tb, ln = Dev(be, np.zeros((T, H, D)), "f16"), i32(be, table), i32(be, lens)
+    gs, pl = i32(be, [0, B]), i32(be, [512])
+    st = None if new is None else i32(be, np.arange(B + 1) * new)
+    qs = torch.randn(N, T, H, D, device="cuda").half()
+    ls = torch.tensor(np.array([[max(513, x - int(rng.integers(0, 200))) for x in lens] for _ in range(N)], dtype=np.int32), device="cuda")
+    rows = torch.randn(N, Hkv, D, device="cuda").half()
+    first = [int(table[0, 3]), 5]                      # a key of the prefix
+
+    def step(i, out):
+        q.x.copy_(qs[i])
+        ln.x.copy_(ls[i])
+        ck.x[first[0], first[1]] = rows[i]
+        cv.x[first[0], first[1]] = rows[i]
+        be.paged_attention(s, q.t, ck.t, cv.t, tb.t, ln.t, 0.1, query_starts=st and st.t, group_starts=gs.t, prefix_lens=pl.t, out=out.t)
+
+    outs = [[Dev(be, np.zeros((T, H, D)), "f16") for _ in range(N)] for _ in range(2)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for i in range(N):
+            step(i, outs[0][i])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for i in range(N):
+            torch.cuda.synchronize()
+            step(i, outs[1][i])
+    s.synchronize()
+    for a, b in zip(*outs):
+        assert torch.equal(a.x, b.x)
+    for i in (0, N - 1):
+        q.x.copy_(qs[i])
+        for c in (ck, cv):
+            c.x[first[0], first[1]] = rows[i]
+        starts = None if new is None else np.arange(B + 1) * new
+        args = (q.f64(), ck.f64(), cv.f64(), table, ls[i].cpu().numpy(), float(np.float32(0.1)), starts, [0, B], [512])
+        want, info = ref.attention(*args)
+        close(outs[0][i].f64(), want, ref.attention_bound(want, info, "f16", "f16", D))
